@@ -125,6 +125,19 @@ pub struct s1c_server_stats {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct s1c_cache {
+    pub k_codes: *mut c_void,
+    pub v_codes: *mut c_void,
+    pub k_scales: *mut f32,
+    pub v_scales: *mut f32,
+    pub num_pages: i32,
+    pub page: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+}
+
+#[repr(C)]
 pub struct s1c_act_head {
     pub d_in: i32,
     pub hidden: i32,
@@ -200,6 +213,28 @@ extern "C" {
                                    n: i32, k: i32, d_bias: *const f32, act: i32, out_f32: i32, d_pos: *const i32,
                                    rope_theta: f32, rope_cols: i32, out_cols: i32,
                                    stream: *mut c_void) -> s1c_status;
+
+    // ---- token-step operators ----
+    pub fn s1c_nibble_gemm(dtype: i32, d_x: *const c_void, x_stride: i64, d_codes: *const c_void, code_pitch: i64,
+                           d_scales: *const c_void, d_zeros: *const c_void, scale_stride: i64, group: i32,
+                           d_out: *mut c_void, out_stride: i64, m: i32, n: i32, k: i32, d_bias: *const f32, act: i32,
+                           out_f32: i32, stream: *mut c_void) -> s1c_status;
+    pub fn s1c_cache_write(cache: *const s1c_cache, dtype: i32, d_k: *const c_void, k_stride: i64, d_v: *const c_void,
+                           v_stride: i64, d_cu: *const i32, d_start: *const i32, d_pages: *const i32, max_pages: i32,
+                           n: i32, max_new: i32, stream: *mut c_void) -> s1c_status;
+    pub fn s1c_cache_read(cache: *const s1c_cache, dtype: i32, d_k: *mut c_void, k_stride: i64, d_v: *mut c_void,
+                          v_stride: i64, d_cu: *const i32, d_start: *const i32, d_pages: *const i32, max_pages: i32,
+                          n: i32, max_rows: i32, stream: *mut c_void) -> s1c_status;
+    pub fn s1c_cache_attention_workspace(cache: *const s1c_cache, heads: i32, n: i32, max_q: i32, max_kv: i32) -> usize;
+    pub fn s1c_cache_attention(cache: *const s1c_cache, dtype: i32, d_q: *const c_void, q_stride: i64,
+                               d_out: *mut c_void, out_stride: i64, d_lse: *mut f32, heads: i32, d_cu: *const i32,
+                               d_len: *const i32, d_pages: *const i32, max_pages: i32, n: i32, max_q: i32, max_kv: i32,
+                               window: i32, scale: f32, d_workspace: *mut c_void, workspace_bytes: usize,
+                               stream: *mut c_void) -> s1c_status;
+    pub fn s1c_sample(dtype: i32, d_logits: *const c_void, row_stride: i64, rows: i32, vocab: i32,
+                      d_temperature: *const f32, d_top_k: *const i32, d_top_p: *const f32, d_min_p: *const f32,
+                      d_uniform: *const f32, d_token: *mut i32, d_prob: *mut f32, stream: *mut c_void) -> s1c_status;
+
     pub fn s1c_selftest_wait_timeout(device: i32, budget_ns: i64, codes: *mut i32) -> s1c_status;
 
     // ---- checkpoint files (laya_core::Weights) ----

@@ -98,6 +98,11 @@ class CAnswer(C.Structure):
                 ("act_probability", C.c_float)]
 
 
+class CCache(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+                ("num_pages", C.c_int32), ("page", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
 # s1c_server_forward_fn
 SERVER_FORWARD_FN = C.CFUNCTYPE(C.c_int32, C.c_void_p, C.POINTER(CVarlen), C.POINTER(C.c_float),
                                 C.POINTER(C.c_float), C.POINTER(C.c_char_p))
@@ -139,6 +144,13 @@ def lib() -> C.CDLL:
         "s1c_profile": (I32, [P, I32]),
         "s1c_profile_report": (SZ, [P, C.c_char_p, SZ]),
         "s1c_gemm_splitk_noalloc": (I32, [I32, P, P, P, I32, I32, I32, P, I32, I32, P, F32, I32, I32, P]),
+        "s1c_nibble_gemm": (I32, [I32, P, I64, P, I64, P, P, I64, I32, P, I64, I32, I32, I32, P, I32, I32, P]),
+        "s1c_cache_write": (I32, [C.POINTER(CCache), I32, P, I64, P, I64, P, P, P, I32, I32, I32, P]),
+        "s1c_cache_read": (I32, [C.POINTER(CCache), I32, P, I64, P, I64, P, P, P, I32, I32, I32, P]),
+        "s1c_cache_attention_workspace": (SZ, [C.POINTER(CCache), I32, I32, I32, I32]),
+        "s1c_cache_attention": (I32, [C.POINTER(CCache), I32, P, I64, P, I64, P, I32, P, P, P, I32, I32, I32, I32, I32,
+                                      F32, P, SZ, P]),
+        "s1c_sample": (I32, [I32, P, I64, I32, I32, P, P, P, P, P, P, P, P]),
         "s1c_weights_open": (I32, [C.c_char_p, C.POINTER(P)]),
         "s1c_weights_close": (None, [P]),
         "s1c_weights_count": (I32, [P]),

@@ -1,8 +1,8 @@
 """Build ``libs1c.so`` in-tree with nvcc for sm_100a.
 
 ``python -m sys1rust_b200.build`` (or ``__graft_entry__.build()``) compiles
-``sys1rust_b200/csrc/s1c.cu`` into ``sys1rust_b200/libs1c.so``. The library links only the CUDA
-runtime; the driver's tensor-map encoder is looked up at run time.
+``sys1rust_b200/csrc/s1c.cu`` and ``operators.cu`` (side by side) into ``sys1rust_b200/libs1c.so``.
+The library links only the CUDA runtime; the driver's tensor-map encoder is looked up at run time.
 """
 from __future__ import annotations
 
@@ -16,6 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libs1c.so")
+UNITS = ("s1c.cu", "operators.cu")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -59,16 +60,29 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 def _compile(verbose: bool) -> str:
     tmp = f"{LIB}.{os.getpid()}.tmp"
-    cmd = [nvcc(), *NVCC_FLAGS, "-shared", "-o", tmp, os.path.join(CSRC, "s1c.cu"), "-lcudart"]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), file=sys.stderr)
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
-    if verbose:
-        print(r.stderr, file=sys.stderr)
-    os.replace(tmp, LIB)
+    objs = {u: f"{tmp}.{u}.o" for u in UNITS}
+    cmds = [[nvcc(), *NVCC_FLAGS, "-c", "-o", o, os.path.join(CSRC, u)] for u, o in objs.items()]
+    link = [nvcc(), *NVCC_FLAGS, "-shared", "-o", tmp, *objs.values(), "-lcudart"]
+    try:
+        if verbose:
+            for c in cmds:
+                c.insert(1, "-Xptxas=-v")
+                print(" ".join(c), file=sys.stderr)
+        procs = [subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True) for c in cmds]
+        done = [(p, *p.communicate()) for p in procs]
+        for p, out, err in done:
+            if p.returncode != 0:
+                raise RuntimeError(f"nvcc failed ({p.returncode}):\n{out}\n{err}")
+            if verbose:
+                print(err, file=sys.stderr)
+        r = subprocess.run(link, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
+        os.replace(tmp, LIB)
+    finally:
+        for o in objs.values():
+            if os.path.exists(o):
+                os.remove(o)
     return LIB
 
 

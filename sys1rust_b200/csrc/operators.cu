@@ -1,0 +1,224 @@
+// Host side of the token-step operators of include/s1c.h: products with 4-bit weights, the 8-bit paged
+// cache, attention over it, and sampling. Each call checks its arguments, runs on the device that
+// holds its output, enqueues its kernels on the caller's stream and allocates nothing.
+#include <cuda_runtime.h>
+
+#include <climits>
+#include <cmath>
+#include <string>
+
+#include "errors.h"
+#include "cache_attention.cuh"
+#include "kvcache.cuh"
+#include "nibble.cuh"
+#include "sample.cuh"
+
+using namespace s1c;
+
+namespace {
+
+void need(bool ok, const char* what) {
+  if (!ok) throw S1cError(S1C_ERR_ARG, what);
+}
+
+bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// Makes the device that holds `p` current for the call, so that a caller with several devices needs no
+// cudaSetDevice; put back at the end. Host memory that the device cannot be shown to reach is refused.
+struct OnDeviceOf {
+  int was = -1;
+  explicit OnDeviceOf(const void* p) {
+    cudaPointerAttributes at;
+    CK(cudaPointerGetAttributes(&at, p));
+    need(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, "outputs must be device memory");
+    int now = 0;
+    CK(cudaGetDevice(&now));
+    if (at.device != now) {
+      CK(cudaSetDevice(at.device));
+      was = now;
+    }
+  }
+  ~OnDeviceOf() {
+    if (was >= 0) cudaSetDevice(was);
+  }
+};
+
+template <typename F>
+s1c_status enter(F&& f) {
+  try {
+    f();
+    return S1C_OK;
+  } catch (const S1cError& e) {
+    set_create_error(e.what());
+    return e.code;
+  } catch (const std::exception& e) {
+    set_create_error(e.what());
+    return S1C_ERR_ARG;
+  } catch (...) {
+    set_create_error("unknown error");
+    return S1C_ERR_ARG;
+  }
+}
+
+void check_half(int dtype) { need(dtype == S1C_DT_F16 || dtype == S1C_DT_BF16, "dtype must be S1C_DT_F16 or S1C_DT_BF16"); }
+
+CacheView check_cache(const s1c_cache* c) {
+  need(c && c->k_codes && c->v_codes && c->k_scales && c->v_scales, "null cache or cache buffer");
+  need(c->num_pages > 0 && c->kv_heads > 0 && c->kv_heads <= 65535, "num_pages and kv_heads must be positive (kv_heads at most 65535)");
+  need(c->page == 16 || c->page == 32 || c->page == 64, "page must be 16, 32 or 64");
+  need(c->head_dim == 64 || c->head_dim == 128, "head_dim must be 64 or 128");
+  need(aligned(c->k_codes, 16) && aligned(c->v_codes, 16), "cache codes must be 16-byte aligned");
+  need((int64_t)c->num_pages * c->kv_heads * c->page <= INT_MAX, "num_pages * kv_heads * page must stay below 2^31");
+  return CacheView{{static_cast<int8_t*>(c->k_codes), static_cast<int8_t*>(c->v_codes)}, {c->k_scales, c->v_scales},
+                   c->num_pages, c->page, c->kv_heads, c->head_dim};
+}
+
+CacheRows check_rows(const CacheView& c, const void* k, int64_t k_stride, const void* v, int64_t v_stride, const int32_t* cu,
+                     const int32_t* start, const int32_t* table, int32_t max_pages, int32_t n, int32_t most) {
+  need(k && v && cu && start && table, "null argument");
+  need(n >= 0 && most >= 0 && max_pages > 0, "n and the row bound must not be negative, max_pages positive");
+  need(k_stride >= (int64_t)c.heads * c.dim && v_stride >= (int64_t)c.heads * c.dim && k_stride % 8 == 0 && v_stride % 8 == 0,
+       "row strides must hold kv_heads * head_dim values and be multiples of 8");
+  need(aligned(k, 16) && aligned(v, 16), "rows must be 16-byte aligned");
+  CacheRows r{};
+  r.rows[0] = const_cast<void*>(k), r.rows[1] = const_cast<void*>(v);
+  r.stride[0] = k_stride, r.stride[1] = v_stride;
+  r.cu = cu, r.start = start, r.table = table, r.max_pages = max_pages, r.most = most;
+  return r;
+}
+
+template <typename T, int D>
+void launch_attention(const CacheView& c, const CacheAttnArgs& a, int n, cudaStream_t st) {
+  cache_attention_rows_kernel<T, D><<<dim3((unsigned)n * a.max_q, (a.heads + 3) / 4), 128, 0, st>>>(c, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+s1c_status s1c_nibble_gemm(int32_t dtype, const void* d_x, int64_t x_stride, const void* d_codes, int64_t code_pitch,
+                           const void* d_scales, const void* d_zeros, int64_t scale_stride, int32_t group, void* d_out,
+                           int64_t out_stride, int32_t M, int32_t N, int32_t K, const float* d_bias, int32_t act,
+                           int32_t out_f32, void* stream) {
+  return enter([&] {
+    check_half(dtype);
+    need(d_x && d_codes && d_scales && d_out, "null argument");
+    need(M >= 0 && M <= 64 && N > 0 && K > 0, "M must be 0 to 64, N and K positive");
+    need(group == 32 || group == 64 || group == 128, "group must be 32, 64 or 128");
+    const int64_t groups = ((int64_t)K + group - 1) / group;
+    need(code_pitch % 16 == 0 && code_pitch >= ((int64_t)K + 31) / 32 * 16 && aligned(d_codes, 16),
+         "codes must be 16-byte aligned, their row pitch a multiple of 16 bytes that holds K rounded up to 32 codes");
+    need(x_stride >= K && out_stride >= N && scale_stride >= groups, "a row stride is shorter than its row");
+    need(act >= 0 && act <= 2, "act must be 0 (none), 1 (ReLU) or 2 (GELU)");
+    if (M == 0) return;
+    OnDeviceOf dev(d_out);
+    const NibbleArgs a{d_x, static_cast<const uint8_t*>(d_codes), d_scales, d_zeros, d_out, d_bias, x_stride, code_pitch,
+                       scale_stride, out_stride, M, N, K, group, act, out_f32};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == S1C_DT_F16)
+      nibble_kernel<__half><<<(N + 7) / 8, 256, 0, st>>>(a);
+    else
+      nibble_kernel<__nv_bfloat16><<<(N + 7) / 8, 256, 0, st>>>(a);
+    CK(cudaGetLastError());
+  });
+}
+
+s1c_status s1c_cache_write(const s1c_cache* cache, int32_t dtype, const void* d_k, int64_t k_stride, const void* d_v,
+                           int64_t v_stride, const int32_t* d_cu, const int32_t* d_start, const int32_t* d_pages,
+                           int32_t max_pages, int32_t n, int32_t max_new, void* stream) {
+  return enter([&] {
+    const CacheView c = check_cache(cache);
+    check_half(dtype);
+    CacheRows r = check_rows(c, d_k, k_stride, d_v, v_stride, d_cu, d_start, d_pages, max_pages, n, max_new);
+    if (n == 0 || max_new == 0) return;
+    r.units = (int)(((int64_t)max_new + c.page - 2) / c.page + 1);
+    need((int64_t)n * r.units <= INT_MAX, "n * pages must stay below 2^31");
+    OnDeviceOf dev(cache->k_codes);
+    const dim3 grid((unsigned)(n * r.units), (unsigned)c.heads, 2);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == S1C_DT_F16)
+      cache_write_kernel<__half><<<grid, 128, 0, st>>>(c, r);
+    else
+      cache_write_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(c, r);
+    CK(cudaGetLastError());
+  });
+}
+
+s1c_status s1c_cache_read(const s1c_cache* cache, int32_t dtype, void* d_k, int64_t k_stride, void* d_v, int64_t v_stride,
+                          const int32_t* d_cu, const int32_t* d_start, const int32_t* d_pages, int32_t max_pages, int32_t n,
+                          int32_t max_rows, void* stream) {
+  return enter([&] {
+    const CacheView c = check_cache(cache);
+    check_half(dtype);
+    CacheRows r = check_rows(c, d_k, k_stride, d_v, v_stride, d_cu, d_start, d_pages, max_pages, n, max_rows);
+    if (n == 0 || max_rows == 0) return;
+    const int64_t units = ((int64_t)max_rows * c.heads * (c.dim / 16) + 255) / 256;
+    need(n * units <= INT_MAX, "n * max_rows * kv_heads is too large for one call");
+    r.units = (int)units;
+    OnDeviceOf dev(d_k);
+    const dim3 grid((unsigned)(n * units), 2);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == S1C_DT_F16)
+      cache_read_kernel<__half><<<grid, 256, 0, st>>>(c, r);
+    else
+      cache_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(c, r);
+    CK(cudaGetLastError());
+  });
+}
+
+size_t s1c_cache_attention_workspace(const s1c_cache* cache, int32_t heads, int32_t n, int32_t max_q, int32_t max_kv) {
+  return 0;
+}
+
+s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, const void* d_q, int64_t q_stride, void* d_out,
+                               int64_t out_stride, float* d_lse, int32_t heads, const int32_t* d_cu, const int32_t* d_len,
+                               const int32_t* d_pages, int32_t max_pages, int32_t n, int32_t max_q, int32_t max_kv,
+                               int32_t window, float scale, void* d_workspace, size_t workspace_bytes, void* stream) {
+  return enter([&] {
+    const CacheView c = check_cache(cache);
+    check_half(dtype);
+    need(d_q && d_out && d_cu && d_len && d_pages, "null argument");
+    need(heads > 0 && heads % c.heads == 0, "heads must be a multiple of kv_heads");
+    need(n >= 0 && max_q >= 0 && max_kv >= 0 && max_pages > 0, "n, max_q and max_kv must not be negative, max_pages positive");
+    const int64_t width = (int64_t)heads * c.dim;
+    need(q_stride >= width && out_stride >= width && q_stride % 8 == 0 && out_stride % 8 == 0 && aligned(d_q, 16) && aligned(d_out, 16),
+         "q and out must be 16-byte aligned, their row strides multiples of 8 that hold heads * head_dim values");
+    need(std::isfinite(scale), "scale must be finite");
+    need(workspace_bytes >= s1c_cache_attention_workspace(cache, heads, n, max_q, max_kv), "workspace too small");
+    if (n == 0 || max_q == 0) return;
+    need((int64_t)n * max_q <= INT_MAX, "n * max_q must stay below 2^31");
+    OnDeviceOf dev(d_out);
+    const CacheAttnArgs a{d_q, d_out, d_lse, q_stride, out_stride, d_cu, d_len, d_pages, heads, max_pages, max_q, window,
+                          scale * 1.4426950408889634f};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == S1C_DT_F16)
+      c.dim == 64 ? launch_attention<__half, 64>(c, a, n, st) : launch_attention<__half, 128>(c, a, n, st);
+    else
+      c.dim == 64 ? launch_attention<__nv_bfloat16, 64>(c, a, n, st) : launch_attention<__nv_bfloat16, 128>(c, a, n, st);
+    CK(cudaGetLastError());
+  });
+}
+
+s1c_status s1c_sample(int32_t dtype, const void* d_logits, int64_t row_stride, int32_t rows, int32_t vocab,
+                      const float* d_temperature, const int32_t* d_top_k, const float* d_top_p, const float* d_min_p,
+                      const float* d_uniform, int32_t* d_token, float* d_prob, void* stream) {
+  return enter([&] {
+    need(dtype == S1C_DT_F32 || dtype == S1C_DT_F16 || dtype == S1C_DT_BF16, "dtype must be S1C_DT_F32, F16 or BF16");
+    need(d_logits && d_uniform && d_token, "null argument");
+    need(rows >= 0 && vocab > 0 && vocab <= (1 << 20), "rows must not be negative, vocab 1 to 2^20");
+    need(row_stride >= vocab, "a row stride is shorter than its row");
+    if (rows == 0) return;
+    OnDeviceOf dev(d_token);
+    const SampleArgs a{d_logits, row_stride, vocab, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_token, d_prob};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == S1C_DT_F32)
+      sample_kernel<float><<<rows, SMP_THREADS, 0, st>>>(a);
+    else if (dtype == S1C_DT_F16)
+      sample_kernel<__half><<<rows, SMP_THREADS, 0, st>>>(a);
+    else
+      sample_kernel<__nv_bfloat16><<<rows, SMP_THREADS, 0, st>>>(a);
+    CK(cudaGetLastError());
+  });
+}
+
+}  // extern "C"

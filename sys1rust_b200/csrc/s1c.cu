@@ -29,6 +29,7 @@
 #include <vector>
 
 #include "../../include/s1c.h"
+#include "errors.h"
 #include "attention.cuh"
 #include "attention_tc.cuh"
 #include "gemm_sm100.cuh"
@@ -47,18 +48,6 @@ namespace {
 
 // ---------------------------------------------------------------------------------------------
 // errors
-
-struct S1cError : std::runtime_error {
-  s1c_status code;
-  S1cError(s1c_status c, const std::string& m) : std::runtime_error(m), code(c) {}
-};
-
-#define CK(call)                                                                                  \
-  do {                                                                                            \
-    cudaError_t e_ = (call);                                                                      \
-    if (e_ != cudaSuccess)                                                                        \
-      throw S1cError(S1C_ERR_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_));          \
-  } while (0)
 
 thread_local std::string g_create_error;
 
@@ -2190,6 +2179,8 @@ NoAllocDevice& noalloc_device(int dev) {
 }
 
 }  // namespace
+
+void s1c::set_create_error(const char* text) { g_create_error = text; }
 
 // =============================================================================================
 // C ABI

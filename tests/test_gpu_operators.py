@@ -1,0 +1,787 @@
+"""The token-step operators on the GPU against plain computations in 64 bits.
+
+Tolerances, derived: storing a result of type t is off by at most u_t = eps_t / 2 of it (bf16 2^-8, f16 2^-11,
+fp32 2^-24). A sum of K products held in fp32, in any order and with truncating adders (at most 2^-23
+a step), is off by at most K 2^-22 of the sum of the products' magnitudes. Where a bound has more
+parts, the test that uses it names them.
+"""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+@pytest.fixture(scope="module")
+def ops(cuda_lib):
+    from sys1rust_b200 import operators
+    return operators
+
+
+def _code(ops, dt):
+    return {torch.bfloat16: ops.DT_BF16, torch.float16: ops.DT_F16, torch.float32: ops.DT_F32}[dt]
+
+
+def _u(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+# ---------------------------------------------------------------------------------------------
+# products with 4-bit weights
+
+
+def _nibble_inputs(M, N, K, group, dt, zeros, seed, pad=0):
+    g = _gen(seed)
+    pitch = -(-K // 32) * 16 + 16 * pad
+    groups = -(-K // group)
+    x = torch.randn(M, K + 3 * pad, generator=g, device="cuda").to(dt)[:, :K]
+    codes = torch.randint(0, 256, (N, pitch), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (torch.rand(N, groups + pad, generator=g, device="cuda") + 0.25).to(dt)[:, :groups]
+    z = (torch.rand(N, groups + pad, generator=g, device="cuda") * 15).to(dt)[:, :groups] if zeros else None
+    return x, codes, scales, z
+
+
+def _nibble_weights(codes, scales, zeros, K, group):
+    q = torch.stack((codes & 15, codes >> 4), -1).flatten(1)[:, :K].double()
+    at = torch.arange(K, device="cuda") // group
+    return (q - (zeros.double()[:, at] if zeros is not None else 8.0)) * scales.double()[:, at]
+
+
+def _nibble(ops, x, codes, scales, zeros, out, K, group, bias=None, act=0, stream=None):
+    M, N = out.shape
+    ops.nibble_gemm(_code(ops, x.dtype), x.data_ptr(), x.stride(0), codes.data_ptr(), codes.stride(0), scales.data_ptr(),
+                    scales.stride(0), out.data_ptr(), out.stride(0), M, N, K, group, zeros_ptr=_ptr(zeros),
+                    bias_ptr=_ptr(bias), act=act, out_f32=out.dtype == torch.float32, stream=_stream() if stream is None else stream)
+
+
+def _act(y, act):
+    return y if act == 0 else torch.relu(y) if act == 1 else torch.nn.functional.gelu(y)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("M,N,K,group", [
+    (1, 1, 1, 32), (1, 7, 31, 32), (2, 16, 32, 64), (1, 64, 33, 128), (1, 1024, 1024, 128), (3, 130, 257, 32),
+    (5, 1000, 2624, 64), (8, 33, 4097, 128), (9, 300, 640, 32), (16, 257, 1100, 64), (17, 129, 129, 128), (33, 65, 2047, 32),
+    (64, 200, 1024, 128), (64, 31, 5000, 64), (1, 5000, 96, 32), (4, 20000, 160, 64), (2, 48, 20000, 128)])
+def test_nibble_gemm(ops, M, N, K, group, dt):
+    """Every combination of zero points, bias, activation and output type at one or another size. The
+    error is the sum's, the zero point's and bias's place in it, and one rounding; GELU's slope is at most 1.13."""
+    for i, (zeros, bias, act, f32) in enumerate([(False, False, 0, False), (True, True, 0, True), (True, False, 1, False),
+                                                 (False, True, 2, True), (True, True, 2, False)]):
+        x, codes, scales, z = _nibble_inputs(M, N, K, group, DT[dt], zeros, 100 + i, pad=i % 2)
+        b = torch.randn(N, generator=_gen(7), device="cuda") if bias else None
+        odt = torch.float32 if f32 else DT[dt]
+        full = torch.full((M, N + 5), 7.0, dtype=odt, device="cuda")
+        out = full[:, :N]
+        _nibble(ops, x, codes, scales, z, out, K, group, b, act)
+        w = _nibble_weights(codes, scales, z, K, group)
+        y = x.double() @ w.t() + (b.double() if bias else 0)
+        ref = _act(y, act)
+        # codes and zero points stand apart in the sum: |q| + |z| up to 30 a product, times the scale
+        at = torch.arange(K, device="cuda") // group
+        mag = x.double().abs() @ (scales.double()[:, at] * 30).t() + (b.double().abs() if bias else 0)
+        bound = _u(odt) * ref.abs() + 1.13 * (K + 64) * 2.0 ** -22 * mag + torch.finfo(odt).tiny
+        err = (out.double() - ref).abs()
+        assert (err <= bound).all(), (i, (err / bound).max().item())
+        assert (full[:, N:] == 7).all()
+
+
+def test_nibble_gemm_extreme_codes_and_values(ops):
+    """All codes 0 or 15 with the largest finite x of f16 in fp32 output; zero scales give zero; a NaN or
+    infinite row of x stays in its own row; bytes behind the last column do not count."""
+    M, N, K, group = 3, 40, 200, 32
+    x, codes, scales, _ = _nibble_inputs(M, N, K, group, torch.float16, False, 5)
+    codes[:20] = 0
+    codes[20:] = 255
+    codes[:, 100:] = 0x5A  # behind column 200
+    x[0] = 65504.0
+    scales[3] = 0
+    out = torch.empty(M, N, device="cuda")
+    _nibble(ops, x, codes, scales, None, out, K, group)
+    w = _nibble_weights(codes, scales, None, K, group)
+    ref = x.double() @ w.t()
+    bound = (K + 64) * 2.0 ** -22 * (x.double().abs() @ (scales.double()[:, torch.arange(K, device="cuda") // group] * 30).t()) + 1e-30
+    assert ((out.double() - ref).abs() <= bound).all()
+    assert (out[:, 3] == 0).all()
+    x2 = x.clone()
+    x2[1, 7] = float("nan")
+    x2[2, 0] = float("inf")
+    out2 = torch.empty_like(out)
+    _nibble(ops, x2, codes, scales, None, out2, K, group)
+    assert torch.equal(out2[0], out[0])
+    keep = torch.arange(N, device="cuda") != 3
+    assert torch.isnan(out2[1][keep]).all() and not torch.isfinite(out2[2][keep]).any()
+
+
+def test_nibble_gemm_is_bitwise_repeatable_and_row_independent(ops):
+    """The same call gives the same bits; the packer's codes give its weights' products."""
+    x, codes, scales, z = _nibble_inputs(7, 515, 3001, 64, torch.bfloat16, True, 9)
+    outs = []
+    for _ in range(2):
+        out = torch.empty(7, 515, device="cuda")
+        _nibble(ops, x, codes, scales, z, out, 3001, 64)
+        outs.append(out)
+    assert torch.equal(*outs)
+    w = torch.randn(50, 300, generator=torch.Generator().manual_seed(3)).numpy()
+    packed, s = ops.nibble_pack(w, 64, np.float16)
+    packed, s = torch.from_numpy(packed).cuda(), torch.from_numpy(s).cuda()
+    xs = torch.randn(2, 300, generator=_gen(4), device="cuda").half()
+    out = torch.empty(2, 50, device="cuda")
+    _nibble(ops, xs, packed, s, None, out, 300, 64)
+    # each weight is off by at most half a step (and the scale's f16 rounding within it, clipped at 7)
+    step = s.double()[:, torch.arange(300, device="cuda") // 64]
+    ref = xs.double() @ torch.from_numpy(w).cuda().double().t()
+    assert ((out.double() - ref).abs() <= xs.double().abs() @ (0.51 * step).t() + 1e-3).all()
+
+
+# ---------------------------------------------------------------------------------------------
+# the cache
+
+
+class Paged:
+    """A cache on the GPU and the values it should hold, kept by a plain computation in 64 bits."""
+
+    def __init__(self, ops, n, longest, H, D, page, seed, spare=3):
+        per = -(-longest // page)
+        self.count = n * per + spare
+        g = _gen(seed)
+        self.H, self.D, self.page, self.n, self.ops = H, D, page, n, ops
+        self.table = torch.randperm(self.count, generator=g, device="cuda")[: n * per].view(n, per).to(torch.int32).contiguous()
+        shape = (self.count, H, page, D)
+        self.codes = [torch.randint(-127, 128, shape, generator=g, device="cuda", dtype=torch.int8) for _ in range(2)]
+        self.scales = [torch.rand(self.count, H, generator=g, device="cuda") * 0.02 + 0.01 for _ in range(2)]
+        self.handle = ops.Cache(self.codes[0].data_ptr(), self.codes[1].data_ptr(), self.scales[0].data_ptr(),
+                                self.scales[1].data_ptr(), self.count, page, H, D)
+        self.expect()
+
+    def expect(self):
+        self.want_codes = [c.double().cpu() for c in self.codes]
+        self.want_scales = [s.double().cpu() for s in self.scales]
+
+    def write(self, k, v, lens, starts, most=None):
+        cu = _i32(np.concatenate([[0], np.cumsum(lens)]).tolist())
+        st = _i32(starts)
+        self.ops.cache_write(self.handle, _code(self.ops, k.dtype), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+                             cu.data_ptr(), st.data_ptr(), self.table.data_ptr(), self.table.shape[1], self.n,
+                             max(lens) if most is None else most, stream=_stream())
+        torch.cuda.synchronize()
+        table = self.table.cpu()
+        for which, x in enumerate((k, v)):
+            x = x.double().cpu().view(x.shape[0], self.H, self.D)
+            base = 0
+            for i, (c, a) in enumerate(zip(lens, starts)):
+                c2 = c if most is None else min(c, most)
+                for p in range(a // self.page, -(-(a + c2) // self.page) if c2 else 0):
+                    lo, hi = max(a, p * self.page), min(a + c2, (p + 1) * self.page)
+                    if p >= table.shape[1] or not 0 <= int(table[i, p]) < self.count:
+                        continue
+                    pid, part = int(table[i, p]), x[base + lo - a: base + hi - a].transpose(0, 1)
+                    W, S = self.want_codes[which], self.want_scales[which]
+                    keep = lo - p * self.page
+                    for h in range(self.H):
+                        new = part[h]
+                        fin = torch.isfinite(new)
+                        top = new[fin].abs().max().item() if fin.any() else 0.0
+                        s = float(np.float32(top) / np.float32(127))
+                        if keep:
+                            s = max(s, S[pid, h].item())
+                        if keep and s > S[pid, h].item():
+                            W[pid, h, :keep] = (W[pid, h, :keep] * S[pid, h] / s).round()
+                        q = (torch.where(fin, new, 0.0) / (s if s > 0 else 1.0)).round().clamp(-127, 127)
+                        q = torch.where(new == math.inf, 127.0, torch.where(new == -math.inf, -127.0, q))
+                        W[pid, h, keep: keep + hi - lo] = q
+                        S[pid, h] = s
+                base += c
+
+    def check(self):
+        for which in range(2):
+            assert torch.equal(self.scales[which].double().cpu(), self.want_scales[which])
+            assert torch.equal(self.codes[which].double().cpu(), self.want_codes[which])
+
+    def read(self, lens, starts, dt, most=None):
+        cu, st = _i32(np.concatenate([[0], np.cumsum(lens)]).tolist()), _i32(starts)
+        out = [torch.full((sum(lens) + 2, self.H * self.D + 8), 9.0, dtype=dt, device="cuda") for _ in range(2)]
+        self.ops.cache_read(self.handle, _code(self.ops, dt), out[0].data_ptr(), out[0].stride(0), out[1].data_ptr(),
+                            out[1].stride(0), cu.data_ptr(), st.data_ptr(), self.table.data_ptr(), self.table.shape[1],
+                            self.n, max(lens) if most is None else most, stream=_stream())
+        torch.cuda.synchronize()
+        return out
+
+    def rows(self, which, i, L):
+        """Values of sequence i's first L positions, [L, H, D] in 64 bits, and which of them have a page."""
+        at = torch.arange(L)
+        per = self.table.shape[1]
+        pid = self.table.cpu()[i][(at // self.page).clamp(max=per - 1)].long()
+        ok = (at // self.page < per) & (pid >= 0) & (pid < self.count)
+        pid = pid.clamp(0, self.count - 1)
+        c, s = self.codes[which].cpu(), self.scales[which].double().cpu()
+        return torch.where(ok[:, None, None], c[pid, :, at % self.page].double() * s[pid][:, :, None], 0.0), ok
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("H,D,page", [(1, 64, 16), (3, 64, 32), (2, 128, 16), (5, 128, 64), (16, 64, 64)])
+def test_cache_write_codes_and_scales(ops, H, D, page, dt):
+    """Codes and scales are equal to the definition's, bit for bit: first rows behind nothing, runs that
+    end inside a page, single rows whose values outgrow the page's scale and shrink again."""
+    n = 4
+    c = Paged(ops, n, 300, H, D, page, 11)
+    g = _gen(12)
+    at = [0, 0, page - 1, 5]
+    for step, lens in enumerate([[70, 1, 200, 17], [1, 1, 1, 1], [0, 2, 1, 33], [page, 0, 3, 1]]):
+        T = sum(lens)
+        size = [1.0, 3.0, 0.1, 10.0][step]
+        k = (torch.randn(T, H * D, generator=g, device="cuda") * size).to(DT[dt])
+        v = (torch.randn(T, H * D + 8, generator=g, device="cuda") * size).to(DT[dt])[:, : H * D]
+        c.write(k, v, lens, at)
+        c.check()
+        at = [a + l for a, l in zip(at, lens)]
+    dst = torch.bfloat16 if dt == "f16" else torch.float16  # read back in either type
+    for out_dt in (DT[dt], dst):
+        lens, starts = [a - min(a, 40) if i % 2 else a for i, a in enumerate(at)], [min(a, 40) if i % 2 else 0 for i, a in enumerate(at)]
+        got = c.read(lens, starts, out_dt)
+        for which in range(2):
+            want = torch.cat([c.rows(which, i, s + l)[0][s:] for i, (l, s) in enumerate(zip(lens, starts))]).reshape(sum(lens), -1)
+            have = got[which][: sum(lens), : H * D].double().cpu()
+            # one product in fp32 and one rounding
+            assert ((have - want).abs() <= (_u(out_dt) * (1 + 2.0 ** -10) + 2.0 ** -24) * want.abs() + torch.finfo(out_dt).tiny * _u(out_dt)).all()
+            assert (got[which][sum(lens):] == 9).all() and (got[which][:, H * D:] == 9).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_cache_write_ties_and_odd_values(ops, dt):
+    """Quotients at and next to a half, subnormal values, zeros, infinities and NaN."""
+    H, D, page = 2, 64, 16
+    c = Paged(ops, 1, 64, H, D, page, 21)
+    k = torch.zeros(40, H, D, dtype=DT[dt], device="cuda")
+    half = torch.arange(D, device="cuda").float() - 31.5  # scale 1: every value a tie
+    k[0, 0] = half.to(DT[dt])
+    k[1, 0, 0] = 127.0
+    k[2, 0] = (torch.arange(D, device="cuda").float() * 0.5 + 0.5 * 2 ** -7).to(DT[dt])
+    k[3, 1, 5] = float("inf")
+    k[4, 1, 6] = -float("inf")
+    k[5, 1, 7] = float("nan")
+    k[6, 1, 8] = 2.5
+    k[17, 0, 1] = torch.finfo(DT[dt]).smallest_normal / 4
+    k[17, 0, 2] = -torch.finfo(DT[dt]).smallest_normal / 8
+    k[18, 1, 3] = float("inf")  # nothing finite but zeros
+    k[33] = torch.finfo(DT[dt]).max
+    v = (torch.randn(40, H, D, generator=_gen(3), device="cuda") * 2.0 ** -20).to(DT[dt])
+    c.write(k.view(40, -1), v.view(40, -1), [40], [0])
+    c.check()
+
+
+def test_cache_skips_bad_pages_and_bounds(ops):
+    """Pages outside the cache, positions past the table, negative starts and rows past the bound are
+    left out of writes and read back as 0; nothing else changes."""
+    H, D, page = 2, 64, 16
+    c = Paged(ops, 3, 96, H, D, page, 31)
+    c.table[0, 1] = -1
+    c.table[1, 2] = c.count
+    c.table[2, 5] = 2 ** 31 - 1
+    g = _gen(32)
+    lens, starts = [60, 50, 40], [3, 0, 70]  # the last runs past its table of 96 positions
+    k, v = [torch.randn(150, H * D, generator=g, device="cuda").half() for _ in range(2)]
+    c.write(k, v, lens, starts)
+    c.check()
+    got = c.read([80, 70, 60], [0, 0, 60], torch.float16)
+    base = 0
+    for i, (l, s) in enumerate([(80, 0), (70, 0), (60, 60)]):
+        want, ok = c.rows(0, i, s + l)
+        have = got[0][base: base + l, : H * D].double().cpu().view(l, H, D)
+        assert (have[~ok[s:]] == 0).all() and (~ok[s:]).any()
+        assert ((have - want[s:]).abs() <= 1.01 * _u(torch.float16) * want[s:].abs() + 1e-7).all()
+        base += l
+    c.write(k, v, [20, 0, 9], [40, 7, 33], most=5)  # rows past the bound
+    c.check()
+    before = [x.clone() for x in c.codes + c.scales]
+    cu, start = _i32([0, 5, 5, 5]), _i32([-2, 0, 0])
+    ops.cache_write(c.handle, ops.DT_F16, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), cu.data_ptr(),
+                    start.data_ptr(), c.table.data_ptr(), c.table.shape[1], 3, 5, stream=_stream())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, c.codes + c.scales))
+
+
+# ---------------------------------------------------------------------------------------------
+# attention over the cache
+
+
+def _attention(ops, c, q, heads, lens, keys, scale, window=-1, most=None, max_kv=None, stream=None):
+    T = sum(lens)
+    out = torch.full((T + 1, heads * c.D + 8), 5.0, dtype=q.dtype, device="cuda")
+    lse = torch.full((T + 1, heads), 5.0, device="cuda")
+    cu, ln = _i32(np.concatenate([[0], np.cumsum(lens)]).tolist()), _i32(keys)
+    mq, mk = max(lens) if most is None else most, max(keys) if max_kv is None else max_kv
+    ws = torch.empty(max(1, ops.cache_attention_workspace(c.handle, heads, c.n, mq, mk)), dtype=torch.uint8, device="cuda")
+    ops.cache_attention(c.handle, _code(ops, q.dtype), q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), heads,
+                        cu.data_ptr(), ln.data_ptr(), c.table.data_ptr(), c.table.shape[1], c.n, mq, mk, scale, window=window,
+                        lse_ptr=lse.data_ptr(), workspace_ptr=ws.data_ptr(), workspace_bytes=ws.numel(),
+                        stream=_stream() if stream is None else stream)
+    torch.cuda.synchronize()
+    return out, lse
+
+
+def _check_attention(c, q, heads, lens, keys, scale, window, out, lse):
+    """Bounds: a score is off by at most d = (D + 8) 2^-22 of the sum of its products' magnitudes (fp32
+    sum; q's scaling and the key's scale are roundings within it), which moves its weight by the factor 1 + 2 d; a
+    weight is rounded to 11 bits, summed over the keys, once; sums over L keys add L 2^-22; one rounding of the result."""
+    G, base = heads // c.H, 0
+    for i, (n, L) in enumerate(zip(lens, keys)):
+        K, ok = c.rows(0, i, L)
+        V, _ = c.rows(1, i, L)
+        K, V, ok = K.cuda(), V.cuda(), ok.cuda()
+        x = q[base: base + n, : heads * c.D].double().view(n, heads, c.D)
+        pos = torch.arange(L - n, L, device="cuda")[:, None]
+        j = torch.arange(L, device="cuda")[None]
+        seen = (j <= pos) & ok[None]
+        if window >= 0:
+            seen &= j >= pos - window
+        for h in range(heads):
+            s = (x[:, h] @ K[:, h // G].t() * scale).masked_fill(~seen, -math.inf)
+            d = (c.D + 8) * 2.0 ** -22 * abs(scale) * ((x[:, h].abs() @ K[:, h // G].abs().t()).masked_fill(~seen, 0).amax(1) if L else x.new_zeros(n))
+            none = ~seen.any(1)
+            p = torch.softmax(s, 1).nan_to_num(0.0) if L else s
+            want, mass = p @ V[:, h // G], p @ V[:, h // G].abs()
+            have = out[base: base + n, h * c.D: (h + 1) * c.D].double()
+            bound = _u(q.dtype) * want.abs() + mass * (2.0 ** -11 + 4 * d[:, None] + (L + 64) * 2.0 ** -22) + torch.finfo(q.dtype).tiny
+            err = (have - want).abs()
+            assert (err <= bound).all(), (i, h, (err / bound).max().item())
+            assert (have[none] == 0).all() and (lse[base: base + n, h][none] == -math.inf).all()
+            wl = torch.logsumexp(s, 1)[~none] if L else s.new_zeros(0)
+            hl = lse[base: base + n, h][~none].double()
+            assert ((hl - wl).abs() <= 2 * d[~none] + (L + 64) * 2.0 ** -22 + 2.0 ** -21 * (1 + wl.abs())).all()
+        base += n
+    assert (out[base:] == 5).all() and (out[:, heads * c.D:] == 5).all() and (lse[base:] == 5).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("H,G,D,page,lens,keys,window", [
+    (1, 1, 64, 16, [1], [1], -1), (2, 1, 64, 16, [1], [17], -1), (1, 8, 128, 32, [1], [700], -1),
+    (2, 4, 128, 16, [1, 1, 1, 1], [1, 15, 16, 1000], -1), (3, 5, 64, 64, [1, 1, 1], [63, 64, 65], -1),
+    (2, 3, 64, 32, [1, 1, 1], [0, 300, 129], -1), (1, 16, 128, 64, [1, 1], [4000, 2], -1),
+    (1, 40, 64, 16, [1, 2], [333, 20], -1), (2, 2, 128, 16, [5, 1, 3], [5, 40, 200], -1),
+    (2, 1, 64, 64, [130, 17], [130, 400], -1), (1, 4, 128, 32, [64, 65, 1], [64, 1000, 77], -1),
+    (2, 2, 64, 16, [3, 70, 1], [2, 100, 50], -1), (2, 2, 64, 16, [1, 40, 9], [900, 40, 300], 0),
+    (1, 3, 128, 32, [1, 40, 100], [900, 500, 300], 64), (2, 1, 64, 16, [1, 33], [5000, 2100], 1000)])
+def test_cache_attention(ops, H, G, D, page, lens, keys, window, dt):
+    n, heads = len(lens), H * G
+    c = Paged(ops, n, max(keys) + 1, H, D, page, 41)
+    c.scales[1][::3] *= 30  # value scales that differ from page to page
+    g = _gen(42)
+    q = torch.randn(sum(lens), heads * D + 16, generator=g, device="cuda").to(DT[dt])
+    scale = 1 / math.sqrt(D)
+    out, lse = _attention(ops, c, q, heads, lens, keys, scale, window)
+    _check_attention(c, q, heads, lens, keys, scale, window, out, lse)
+
+
+def test_cache_attention_outside_pages_and_bounds(ops):
+    """Keys on pages outside the cache are masked, a sequence of such pages alone has an empty row; what the
+    unread rows hold (largest codes and scales) does not count; bounds wider than the batch do not matter."""
+    H, D, page, heads = 2, 64, 16, 6
+    c = Paged(ops, 4, 200, H, D, page, 51)
+    c.table[0, 1] = -5
+    c.table[0, 2] = c.count + 7
+    c.table[1, :] = -1
+    lens, keys = [2, 3, 1, 7], [100, 40, 23, 200]
+    pid = int(c.table[2, 1])  # rows 7.. of this page lie behind the sequence's last
+    c.codes[0][pid, :, 7:] = 127
+    c.codes[1][pid, :, 7:] = -128
+    for t in c.scales:  # pages that nobody reads
+        used = set(c.table.cpu().flatten().tolist())
+        for p in range(c.count):
+            if p not in used:
+                t[p] = float("nan")
+    q = torch.randn(sum(lens), heads * D, generator=_gen(52), device="cuda").bfloat16()
+    for most, max_kv in [(None, None), (20, 5000), (7, 200)]:
+        out, lse = _attention(ops, c, q, heads, lens, keys, 0.125, most=most, max_kv=max_kv)
+        _check_attention(c, q, heads, lens, keys, 0.125, -1, out, lse)
+
+
+def test_cache_attention_past_its_table(ops):
+    """Positions past the page table have no page: they are masked."""
+    c = Paged(ops, 2, 64, 1, 64, 16, 53)
+    q = torch.randn(3, 2 * 64, generator=_gen(54), device="cuda").half()
+    lens, keys = [2, 1], [70, 120]
+    out, lse = _attention(ops, c, q, 2, lens, keys, 0.125)
+    _check_attention(c, q, 2, lens, keys, 0.125, -1, out, lse)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_cache_attention_scores_and_scales_far_apart(ops, dt):
+    """Scores in the hundreds that grow along the keys, queries from 2^-12 to 2^12, pages whose values are all zero
+    (scale 0), value scales 2^16 apart."""
+    H, D, page, heads = 2, 128, 16, 8
+    c = Paged(ops, 3, 600, H, D, page, 61)
+    per = c.table.shape[1]
+    for i in range(3):
+        for p in range(per):
+            pid = int(c.table[i, p])
+            c.scales[0][pid] *= 1 + 3 * p / per
+            c.scales[1][pid] *= 2.0 ** (-8 + 16 * ((p * 7) % 5) / 4)
+            if p % 9 == 4:
+                c.scales[1][pid] = 0
+                c.codes[1][pid] = 0
+    lens, keys = [1, 4, 1], [600, 555, 16 * 5]
+    q = torch.randn(sum(lens), heads * D, generator=_gen(62), device="cuda")
+    q = (q * torch.exp2(torch.linspace(-12, 5, q.shape[0], device="cuda"))[:, None]).to(DT[dt])
+    q[:, D: 2 * D] *= 2.0 ** -9
+    out, lse = _attention(ops, c, q, heads, lens, keys, 0.088)
+    _check_attention(c, q, heads, lens, keys, 0.088, -1, out, lse)
+
+
+def test_cache_attention_all_values_zero(ops):
+    c = Paged(ops, 1, 64, 1, 64, 16, 63)
+    c.codes[1].zero_()
+    c.scales[1].zero_()
+    q = torch.randn(1, 64, generator=_gen(64), device="cuda").half()
+    out, lse = _attention(ops, c, q, 1, [1], [50], 0.125)
+    _check_attention(c, q, 1, [1], [50], 0.125, -1, out, lse)
+
+
+def test_cache_attention_long_cache(ops):
+    """70001 positions, more than 2^31 bytes into the codes' array for the last pages."""
+    H, D, page, L = 8, 128, 64, 70001
+    per = -(-L // page)
+    big = 2 ** 31 // (H * page * D) + 64  # pages before the sequence's own
+    free, _ = torch.cuda.mem_get_info()
+    if free < 8 * 2 ** 30:
+        pytest.skip("needs 8 GB")
+    g = _gen(71)
+    codes = [torch.zeros(big + per, H, page, D, dtype=torch.int8, device="cuda") for _ in range(2)]
+    for x in codes:
+        x[big:] = torch.randint(-127, 128, (per, H, page, D), generator=g, device="cuda", dtype=torch.int8)
+    scales = [torch.rand(big + per, H, generator=g, device="cuda") * 0.02 for _ in range(2)]
+    table = (big + torch.randperm(per, generator=g, device="cuda")).to(torch.int32)[None].contiguous()
+    handle = ops.Cache(codes[0].data_ptr(), codes[1].data_ptr(), scales[0].data_ptr(), scales[1].data_ptr(), big + per, page, H, D)
+    c = Paged.__new__(Paged)
+    c.H, c.D, c.page, c.n, c.ops, c.count, c.table, c.handle = H, D, page, 1, ops, per, table, handle
+    q = torch.randn(2, H * 2 * D, generator=g, device="cuda").bfloat16()
+    out, lse = _attention(ops, c, q, 2 * H, [2], [L], 0.088)
+    c.table = table - big
+    c.codes, c.scales = [x[big:] for x in codes], [x[big:] for x in scales]
+    _check_attention(c, q, 2 * H, [2], [L], 0.088, -1, out, lse)
+
+
+# ---------------------------------------------------------------------------------------------
+# sampling
+
+
+def _sample_ref(x, u, T, k, p, m):
+    """(token, probability, how near u or p comes to another outcome) of one row, in 64 bits."""
+    x = x.astype(np.float64)
+    if np.isnan(x).any() or (x == np.inf).any() or x.max() == -np.inf:
+        return -1, 0.0, 1.0
+    if not T > 0:
+        return int(x.argmax()), 1.0, 1.0
+    e = np.exp((x - x.max()) / T)
+    order = np.lexsort((np.arange(x.size), -x))
+    if k > 0:
+        order = order[:k]
+    near = 1.0
+    if p < 1:
+        cum = np.cumsum(e[order])
+        cut = int(np.searchsorted(cum, p * cum[-1], side="left")) + 1 if p > 0 else 1
+        near = min(near, np.abs(cum / cum[-1] - p).min())
+        order = order[:cut]
+    if m > 0:
+        near = min(near, np.abs(e[order] / min(m, 1.0) - 1)[1:].min(initial=1.0))
+        order = order[e[order] >= min(m, 1.0)]
+    order = np.sort(order)
+    cum = np.cumsum(e[order])
+    order, cum = order[cum > 0], cum[cum > 0]
+    j = min(int(np.searchsorted(cum, u * cum[-1], side="right")), int(np.flatnonzero(e[order])[-1])) if u == u else int(np.flatnonzero(e[order])[-1])
+    if u == u:
+        near = min(near, np.abs(cum[:-1] / cum[-1] - u).min(initial=1.0)) if 0 < u < 1 else near
+    return int(order[j]), float(e[order[j]] / cum[-1]), near
+
+
+def _sample(ops, x, u, T=None, k=None, p=None, m=None, prob=True):
+    R, V = x.shape
+    token = torch.full((R + 1,), -7, dtype=torch.int32, device="cuda")
+    pr = torch.full((R + 1,), -7.0, device="cuda") if prob else None
+    ops.sample(_code(ops, x.dtype), x.data_ptr(), x.stride(0), R, V, token.data_ptr(), u.data_ptr(), temperature_ptr=_ptr(T),
+               top_k_ptr=_ptr(k), top_p_ptr=_ptr(p), min_p_ptr=_ptr(m), prob_ptr=_ptr(pr), stream=_stream())
+    torch.cuda.synchronize()
+    assert token[R] == -7 and (pr is None or pr[R] == -7)
+    return token[:R].cpu().numpy(), None if pr is None else pr[:R].cpu().numpy()
+
+
+def _check_sample(ops, x, u, T, k, p, m):
+    token, prob = _sample(ops, x, u, T, k, p, m)
+    xs = x.float().cpu().numpy()
+    R = x.shape[0]
+    get = lambda t, d: np.full(R, d) if t is None else t.cpu().numpy()  # noqa: E731
+    Ts, ks, ps, ms, us = get(T, 1.0), get(k, 0), get(p, 1.0), get(m, 0.0), u.cpu().numpy()
+    decided = 0
+    for r in range(R):
+        want, pw, near = _sample_ref(xs[r], float(us[r]), float(Ts[r]), int(ks[r]), float(ps[r]), float(ms[r]))
+        # masses carry 3e-8 each; a border nearer than 3e-7 is undecided
+        if near > 3e-7:
+            assert token[r] == want, (r, token[r], want, near)
+            # the mass kept, summed, and the rounding of the share
+            assert abs(prob[r] - pw) <= 3e-7 * pw + 1e-12, (r, prob[r], pw)
+            decided += 1
+        else:
+            assert 0 <= token[r] < x.shape[1]
+    # a row of V borders is undecided with a chance of at most 2 * 3e-7 * V: 8 % at the largest V here
+    assert decided >= R / 2 or R < 10
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V", [1, 2, 31, 32, 33, 1000, 1024, 1025, 50368, 131075])
+def test_sample(ops, V, dt):
+    """Rows with every combination of the filters, among them ones that keep a single token and ones that
+    keep all; 16-bit logits bring many equal ones, so the order of equals decides."""
+    R = 24
+    g = _gen(81 + V)
+    x = (torch.randn(R, V + 3, generator=g, device="cuda") * 2.5).to(DT[dt])[:, :V]
+    u = torch.rand(R, generator=g, device="cuda")
+    r = torch.arange(R, device="cuda")
+    T = torch.where(r % 5 == 4, 0.05, 0.3 + 0.1 * (r % 12))
+    k = torch.where(r % 2 == 0, 0, 1 + (r * r * 37) % max(V, 2)).to(torch.int32)
+    p = torch.where(r % 3 == 0, 1.0, 0.04 * r)
+    m = torch.where(r % 4 < 2, 0.0, 0.01 * r)
+    _check_sample(ops, x, u, T, k, p, m)
+    _check_sample(ops, x, u, None, None, None, None)
+    _check_sample(ops, x, u, T, k, None, None)
+    _check_sample(ops, x, u, T, None, p, None)
+    _check_sample(ops, x, u, None, None, None, m)
+    token, _ = _sample(ops, x, u, T, k, p, m, prob=False)
+    assert (token == _sample(ops, x, u, T, k, p, m)[0]).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_sample_equal_and_masked_logits(ops, dt):
+    """All logits equal (in one bin of every histogram), two values, -inf in most places, one finite logit
+    alone, zeros of both signs, temperatures from tiny to huge."""
+    V, R = 5000, 40
+    g = _gen(91)
+    x = torch.zeros(R, V, dtype=DT[dt], device="cuda")
+    x[8:16] = torch.where(torch.rand(8, V, generator=g, device="cuda") < 0.5, 1.0, -1.0).to(DT[dt])
+    x[16:24] = torch.where(torch.rand(8, V, generator=g, device="cuda") < 0.98, -math.inf, 3.0).to(DT[dt])
+    x[24:32] = -math.inf
+    x[24:32, 4321] = -5
+    x[32:40, ::2] = -0.0
+    x[0:4] = 60000.0
+    u = torch.rand(R, generator=g, device="cuda")
+    r = torch.arange(R, device="cuda")
+    T = torch.tensor([1e-6, 0.7, 1.0, 1e6], device="cuda").repeat(10)
+    k = torch.where(r % 8 < 4, 0, 1 + r * 13).to(torch.int32)
+    p = torch.where(r % 3 == 1, 0.37, 1.0)
+    _check_sample(ops, x, u, T, k, p, None)
+    _check_sample(ops, x, u, None, k, None, torch.full((R,), 0.5, device="cuda"))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_sample_rows_without_a_distribution_and_odd_parameters(ops, dt):
+    V = 700
+    g = _gen(95)
+    x = torch.randn(16, V, generator=g, device="cuda").to(DT[dt])
+    x[0, 5] = math.nan
+    x[1, 699] = math.inf
+    x[2] = -math.inf
+    x[3, 100:] = -math.inf
+    x[4, 17] = x[4, 600] = 9
+    u = torch.rand(16, generator=g, device="cuda")
+    u[5], u[6], u[7], u[8] = 1.0, math.nan, 0.0, 2.0
+    T = torch.ones(16, device="cuda")
+    T[4], T[9], T[10] = 0.0, -1.0, math.nan
+    T[0], T[11] = 0.0, math.inf
+    k = torch.zeros(16, dtype=torch.int32, device="cuda")
+    k[3], k[12], k[13] = 300, -4, 2 ** 31 - 1
+    p = torch.ones(16, device="cuda")
+    p[12], p[13], p[14] = 0.0, -1.0, math.nan
+    m = torch.zeros(16, device="cuda")
+    m[14], m[15] = math.nan, 7.0
+    xs, us = x.float().cpu().numpy(), u.cpu().numpy()
+    token, prob = _sample(ops, x, u, T, k, p, m)
+    assert list(token[:3]) == [-1, -1, -1] and (prob[:3] == 0).all()
+    assert token[4] == 17 and prob[4] == 1
+    for r in (9, 10):
+        assert token[r] == xs[r].argmax() and prob[r] == 1
+    assert token[11] == min(V - 1, int(us[11] * V)) or abs(us[11] * V - round(us[11] * V)) < 1e-3
+    assert token[12] == xs[12].argmax() and token[13] == xs[13].argmax() and token[15] == xs[15].argmax()
+    for r in (3, 5, 6, 7, 8, 14):
+        want, pw, near = _sample_ref(xs[r], float(us[r]), 1.0, int(k[r]), 1.0, 0.0)
+        assert near < 3e-7 or (token[r] == want and abs(prob[r] - pw) <= 3e-7 * pw), r
+
+
+def test_sample_values_over_the_whole_range(ops):
+    """Logits from the smallest to the largest floats: a cut far below the largest, in one bin with others."""
+    V, R = 3000, 8
+    g = _gen(97)
+    x = torch.randn(R, V, generator=g, device="cuda") * torch.exp2(torch.randint(-100, 100, (R, V), generator=g, device="cuda").float())
+    x[4:] = torch.randn(4, V, generator=g, device="cuda") * 1e-6  # all in the first bins
+    u = torch.rand(R, generator=g, device="cuda")
+    k = _i32([5, 2000, 3000, 100, 5, 1700, 0, 29])
+    p = torch.tensor([1, 0.5, 0.9, 1, 0.3, 0.77, 0.999, 0.01], device="cuda")
+    for T in (1.0, 1e-6, 1e30):
+        _check_sample(ops, x, u, torch.full((R,), T, device="cuda"), k, p, None)
+
+
+# ---------------------------------------------------------------------------------------------
+# together, on streams and in graphs
+
+
+class Step:
+    """A small layer and head: q, k, v from 4-bit products, appended, attended to, and a token sampled
+    from 4-bit logits. Buffers are kept, lengths live on the GPU, so a captured step replays."""
+
+    def __init__(self, ops, n=3, seed=7):
+        self.ops, self.n = ops, n
+        self.H, self.G, self.D, self.V = 2, 3, 64, 997
+        H, G, D, V, width = self.H, self.G, self.D, self.V, 256
+        g = _gen(seed)
+        dt = torch.bfloat16
+        sizes = {"qkv": (H * (G + 2) * D, width), "logits": (V, H * G * D)}
+        self.w = {}
+        for name, (N, K) in sizes.items():
+            w = torch.randn(N, K, generator=g, device="cuda") / math.sqrt(K) * 2
+            codes, scales = ops.nibble_pack(w.cpu().numpy(), 32)
+            self.w[name] = (torch.from_numpy(codes).cuda(), torch.from_numpy(scales).cuda().to(dt))
+        self.emb = torch.randn(V, width, generator=g, device="cuda").to(dt)
+        self.x = torch.empty(n, width, dtype=dt, device="cuda")
+        self.qkv = torch.empty(n, sizes["qkv"][0], dtype=dt, device="cuda")
+        self.att = torch.empty(n, H * G * D, dtype=dt, device="cuda")
+        self.logits = torch.empty(n, V, device="cuda")
+        self.token = torch.arange(n, dtype=torch.int32, device="cuda")
+        self.u = torch.empty(n, device="cuda")
+        self.cache = Paged(ops, n, 40, H, D, 16, seed)
+        self.cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+        self.len = _i32([0, 5, 20][:n])
+        self.ws = torch.empty(max(1, ops.cache_attention_workspace(self.cache.handle, H * G, n, 1, 40)), dtype=torch.uint8, device="cuda")
+        self.p, self.T = torch.full((n,), 0.9, device="cuda"), torch.full((n,), 0.8, device="cuda")
+        self.start = torch.empty_like(self.len)
+
+    def run(self):
+        ops, H, G, D, c, st = self.ops, self.H, self.G, self.D, self.cache, _stream()
+        self.x.copy_(self.emb[self.token.long()])
+        _nibble(ops, self.x, *self.w["qkv"], None, self.qkv, 256, 32)
+        k, v = self.qkv[:, H * G * D:], self.qkv[:, H * (G + 1) * D:]
+        self.start.copy_(self.len)
+        ops.cache_write(c.handle, ops.DT_BF16, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), self.cu.data_ptr(),
+                        self.start.data_ptr(), c.table.data_ptr(), c.table.shape[1], self.n, 1, stream=st)
+        self.len.add_(1)
+        ops.cache_attention(c.handle, ops.DT_BF16, self.qkv.data_ptr(), self.qkv.stride(0), self.att.data_ptr(),
+                            self.att.stride(0), H * G, self.cu.data_ptr(), self.len.data_ptr(), c.table.data_ptr(),
+                            c.table.shape[1], self.n, 1, 40, 0.125, workspace_ptr=self.ws.data_ptr(),
+                            workspace_bytes=self.ws.numel(), stream=st)
+        _nibble(ops, self.att, *self.w["logits"], None, self.logits, H * G * D, 32)
+        ops.sample(ops.DT_F32, self.logits.data_ptr(), self.logits.stride(0), self.n, self.V, self.token.data_ptr(),
+                   self.u.data_ptr(), temperature_ptr=self.T.data_ptr(), top_p_ptr=self.p.data_ptr(), stream=st)
+
+    def check(self):
+        """The step that has just run, part by part, each from the inputs it was given."""
+        H, G, D, c = self.H, self.G, self.D, self.cache
+        for x, (codes, scales), out, K in [(self.x, self.w["qkv"], self.qkv, 256), (self.att, self.w["logits"], self.logits, H * G * D)]:
+            w = _nibble_weights(codes, scales, None, K, 32)
+            ref = x.double() @ w.t()
+            mag = x.double().abs() @ (scales.double()[:, torch.arange(K, device="cuda") // 32] * 30).t()
+            assert ((out.double() - ref).abs() <= _u(out.dtype) * ref.abs() + (K + 64) * 2.0 ** -22 * mag).all()
+        for i in range(self.n):
+            L = int(self.len[i])
+            for which, first in ((0, H * G * D), (1, H * (G + 1) * D)):
+                row = self.qkv[i, first: first + H * D].double().view(H, D).cpu()
+                have = c.rows(which, i, L)[0][-1]
+                s = c.scales[which].double().cpu()[int(c.table[i, (L - 1) // 16])]
+                assert ((have - row).abs() <= 0.5 * s[:, None] * (1 + 1e-6)).all()
+        out = torch.full((self.n + 1, H * G * D + 8), 5.0, dtype=torch.bfloat16, device="cuda")
+        out[: self.n, : H * G * D] = self.att
+        lse = torch.full((self.n + 1, H * G), 5.0, device="cuda")
+        lens = [1] * self.n
+        o2, lse2 = _attention(self.ops, c, self.qkv, H * G, lens, self.len.tolist(), 0.125)
+        _check_attention(c, self.qkv, H * G, lens, self.len.tolist(), 0.125, -1, o2, lse2)
+        del lse
+        ref = o2[: self.n, : H * G * D].double()
+        assert ((self.att.double() - ref).abs() <= 2.0 ** -7 * ref.abs() + 1e-4).all()
+        for i in range(self.n):
+            want, _, near = _sample_ref(self.logits[i].cpu().numpy(), float(self.u[i]), float(np.float32(0.8)), 0, float(np.float32(0.9)), 0.0)
+            assert near < 3e-7 or int(self.token[i]) == want
+
+
+def test_token_steps_eager_and_replayed(ops):
+    """Steps one after another: eagerly, then the same from a captured graph on a side stream, bit for bit the same."""
+    tokens = []
+    for graph in (False, True):
+        s = Step(ops)
+        u = torch.rand(12, s.n, generator=_gen(8), device="cuda")
+        run = s.run
+        if graph:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            state = [t.clone() for t in (s.token, s.len, *s.cache.codes, *s.cache.scales)]
+            with torch.cuda.stream(side):
+                s.u.copy_(u[0])
+                s.run()  # outside the capture first, as programs do
+                side.synchronize()
+                for t, old in zip((s.token, s.len, *s.cache.codes, *s.cache.scales), state):
+                    t.copy_(old)
+                gr = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(gr, stream=side):
+                    s.run()
+            torch.cuda.synchronize()
+            run = gr.replay
+        for i in range(12):
+            s.u.copy_(u[i])
+            run()
+            torch.cuda.synchronize()
+            if not graph and i % 5 == 0:
+                s.check()
+            tokens.append((graph, s.token.tolist(), s.logits.clone()))
+    half = len(tokens) // 2
+    for a, b in zip(tokens[:half], tokens[half:]):
+        assert a[1] == b[1] and torch.equal(a[2], b[2])
+
+
+def test_two_streams_at_once(ops):
+    """Two sequences of steps on two streams, nothing waiting between them, each as if alone."""
+    alone = []
+    for seed in (1, 2):
+        s = Step(ops, seed=seed)
+        s.u.fill_(0.4)
+        for _ in range(10):
+            s.run()
+        torch.cuda.synchronize()
+        alone.append((s.token.clone(), s.logits.clone()))
+    steps = [Step(ops, seed=seed) for seed in (1, 2)]
+    streams = [torch.cuda.Stream() for _ in steps]
+    for s in steps:
+        s.u.fill_(0.4)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, st in zip(steps, streams):
+            with torch.cuda.stream(st):
+                s.run()
+    torch.cuda.synchronize()
+    for s, (token, logits) in zip(steps, alone):
+        assert torch.equal(s.token, token) and torch.equal(s.logits, logits)
+
+
+def test_host_memory_is_refused(ops):
+    from sys1rust_b200.backend import BackendError
+    x = torch.zeros(1, 64, dtype=torch.float16, device="cuda")
+    codes = torch.zeros(8, 32, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(8, 2, dtype=torch.float16, device="cuda")
+    out = torch.zeros(1, 8, dtype=torch.float16)
+    with pytest.raises(BackendError, match="device memory"):
+        _nibble(ops, x, codes, scales, None, out, 64, 32)
