@@ -1,8 +1,8 @@
 """Build ``libs1c.so`` in-tree with nvcc for sm_100a.
 
-``python -m sys1rust_b200.build`` (or ``__graft_entry__.build()``) compiles
-``sys1rust_b200/csrc/s1c.cu`` and ``operators.cu`` (side by side) into ``sys1rust_b200/libs1c.so``.
-The library links only the CUDA runtime; the driver's tensor-map encoder is looked up at run time.
+``python -m sys1rust_b200.build`` (or ``__graft_entry__.build()``) compiles the units of
+``sys1rust_b200/csrc`` (side by side) into ``sys1rust_b200/libs1c.so``. The library links only the
+CUDA runtime; the driver's tensor-map encoder is looked up at run time.
 """
 from __future__ import annotations
 
@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libs1c.so")
-UNITS = ("s1c.cu", "operators.cu")
+UNITS = ("s1c.cu", "operators.cu", "nibble_f16.cu", "nibble_bf16.cu")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -71,6 +71,19 @@ S1C_DEV uint32_t pack_f16x2(float lo, float hi) {
 }
 S1C_DEV float2 unpack_f16x2(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
+// Element types to and from fp32 (one rounding).
+S1C_DEV float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+S1C_DEV float to_f32(__half v) { return __half2float(v); }
+S1C_DEV float to_f32(float v) { return v; }
+template <typename T>
+S1C_DEV T from_f32(float v);
+template <>
+S1C_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+S1C_DEV __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+S1C_DEV float from_f32<float>(float v) { return v; }
+
 // ---------------------------------------------------------------------------------------
 // mbarrier
 S1C_DEV void mbar_init(uint64_t* bar, uint32_t count) {

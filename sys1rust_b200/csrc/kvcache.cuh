@@ -7,7 +7,7 @@
 // stand in it, else 0; a new value becomes round-half-even(x / s), and where s grew the earlier codes
 // become round-half-even(code * s_old / s), both of the exact quotient.
 #pragma once
-#include "nibble.cuh"
+#include "common.cuh"
 
 namespace s1c {
 

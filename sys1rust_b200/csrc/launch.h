@@ -1,0 +1,54 @@
+// Host helpers of the token-step operators' launches.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+#include <string>
+
+#include "errors.h"
+
+namespace s1c {
+
+// A matrix of bytes [rows, width] in boxes of `box_rows` x `box` bytes, swizzled over `box` bytes (64 or 128).
+inline CUtensorMap byte_map(const void* p, uint64_t width, uint64_t rows, uint64_t pitch, uint32_t box, uint32_t box_rows) {
+  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f) : nullptr;
+  }();
+  if (!encode) throw S1cError(S1C_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  CUtensorMap m;
+  const cuuint64_t dims[2] = {width, rows}, strides[1] = {pitch};
+  const cuuint32_t boxes[2] = {box, box_rows}, ones[2] = {1, 1};
+  const CUresult r = encode(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, boxes, ones,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, box == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw S1cError(S1C_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return m;
+}
+
+// A kernel's shared memory limit is raised once for each device.
+template <auto KERNEL>
+void allow_smem(int dev) {
+  static std::atomic<bool> done[64];
+  if (dev < 64 && done[dev].load(std::memory_order_acquire)) return;
+  CK(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+  if (dev < 64) done[dev].store(true, std::memory_order_release);
+}
+
+inline int sm_count(int dev) {
+  static std::atomic<int> counts[64];
+  int n = dev < 64 ? counts[dev].load(std::memory_order_relaxed) : 0;
+  if (!n) {
+    CK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64) counts[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+}  // namespace s1c

@@ -1,19 +1,28 @@
 // Host side of the token-step operators of include/s1c.h: products with 4-bit weights, the 8-bit paged
 // cache, attention over it, and sampling. Each call checks its arguments, runs on the device that
 // holds its output, enqueues its kernels on the caller's stream and allocates nothing.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <string>
 
 #include "errors.h"
+#include "launch.h"
 #include "cache_attention.cuh"
 #include "kvcache.cuh"
 #include "nibble.cuh"
 #include "sample.cuh"
 
 using namespace s1c;
+
+namespace s1c {
+// nibble_f16.cu, nibble_bf16.cu
+void launch_nibble_f16(const NibbleArgs& a, int group, int dev, cudaStream_t st);
+void launch_nibble_bf16(const NibbleArgs& a, int group, int dev, cudaStream_t st);
+}  // namespace s1c
 
 namespace {
 
@@ -26,12 +35,13 @@ bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) %
 // Makes the device that holds `p` current for the call, so that a caller with several devices needs no
 // cudaSetDevice; put back at the end. Host memory that the device cannot be shown to reach is refused.
 struct OnDeviceOf {
-  int was = -1;
+  int was = -1, device = 0;
   explicit OnDeviceOf(const void* p) {
     cudaPointerAttributes at;
     CK(cudaPointerGetAttributes(&at, p));
     need(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, "outputs must be device memory");
     int now = 0;
+    device = at.device;
     CK(cudaGetDevice(&now));
     if (at.device != now) {
       CK(cudaSetDevice(at.device));
@@ -112,13 +122,14 @@ s1c_status s1c_nibble_gemm(int32_t dtype, const void* d_x, int64_t x_stride, con
     need(act >= 0 && act <= 2, "act must be 0 (none), 1 (ReLU) or 2 (GELU)");
     if (M == 0) return;
     OnDeviceOf dev(d_out);
-    const NibbleArgs a{d_x, static_cast<const uint8_t*>(d_codes), d_scales, d_zeros, d_out, d_bias, x_stride, code_pitch,
-                       scale_stride, out_stride, M, N, K, group, act, out_f32};
+    NibbleArgs a{d_x, static_cast<const uint8_t*>(d_codes), d_scales, d_zeros, d_out, d_bias, x_stride, code_pitch,
+                 scale_stride, out_stride, M, N, K, (int)groups, act, out_f32};
+    a.vec = x_stride % 8 == 0 && aligned(d_x, 16);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == S1C_DT_F16)
-      nibble_kernel<__half><<<(N + 7) / 8, 256, 0, st>>>(a);
+      launch_nibble_f16(a, group, dev.device, st);
     else
-      nibble_kernel<__nv_bfloat16><<<(N + 7) / 8, 256, 0, st>>>(a);
+      launch_nibble_bf16(a, group, dev.device, st);
     CK(cudaGetLastError());
   });
 }

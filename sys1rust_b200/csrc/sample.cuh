@@ -13,7 +13,7 @@
 // Masses are integers: e = m * 2^(n - 30), m an integer of 31 bits, and all e in one bin share n. So their sums are exact and do not depend
 // on the order of atomics. Logits more than 45 powers of two below the largest have no mass.
 #pragma once
-#include "nibble.cuh"
+#include "common.cuh"
 
 namespace s1c {
 
