@@ -1,0 +1,40 @@
+// Warp-level f16 products and their operands from 16-bit and 8-bit values.
+#pragma once
+#include "common.cuh"
+
+namespace s1c {
+
+// A 16-bit value of type T in the bits of v.
+template <typename T>
+S1C_DEV float bits_f32(uint16_t v) { return to_f32(*reinterpret_cast<T*>(&v)); }
+
+// D += A B, f16 in, fp32 sums: a 16 x 16 (row), b 16 x 8 (column).
+S1C_DEV void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A word of shared memory at an address and an offset that the compiler knows.
+S1C_DEV uint32_t lds_at(uint32_t at, int off) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at + off));
+  return v;
+}
+
+// Two codes + 128 under the exponent of 1024 (1024 + 128 + code) to two f16 codes.
+S1C_DEV uint32_t code_pair(uint32_t v) {
+  const uint32_t base = 0x64806480u;  // 1152
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&base));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// 2^x to about 2^-22; 0 for -inf.
+S1C_DEV float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace s1c

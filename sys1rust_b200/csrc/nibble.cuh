@@ -27,7 +27,7 @@
 #pragma once
 #include <utility>
 
-#include "common.cuh"
+#include "mma.cuh"
 
 namespace s1c {
 
@@ -48,9 +48,6 @@ struct NibbleArgs {
   int split;  // x fits: tiles may be split between warps
 };
 
-template <typename T>
-S1C_DEV float bits_f32(uint16_t v) { return to_f32(*reinterpret_cast<T*>(&v)); }
-
 // Asynchronous copies of 4, 8 or 16 bytes to shared memory; each thread waits for its own.
 template <int BYTES>
 S1C_DEV void copy_async(uint32_t dst, const void* src) {
@@ -64,14 +61,6 @@ S1C_DEV void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory")
 template <int N>
 S1C_DEV void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// D += A B, f16 in, fp32 sums: a 16 x 16 (row), b 16 x 8 (column).
-S1C_DEV void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 template <int OFF>

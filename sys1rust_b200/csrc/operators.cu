@@ -97,9 +97,45 @@ CacheRows check_rows(const CacheView& c, const void* k, int64_t k_stride, const 
   return r;
 }
 
-template <typename T, int D>
-void launch_attention(const CacheView& c, const CacheAttnArgs& a, int n, cudaStream_t st) {
-  cache_attention_rows_kernel<T, D><<<dim3((unsigned)n * a.max_q, (a.heads + 3) / 4), 128, 0, st>>>(c, a);
+// How an attention call is laid out: rows of a block (16, or 64 shared between warps), keys of a block.
+struct AttnPlan {
+  bool share;
+  int tiles, chunk, chunks;
+};
+AttnPlan plan_attention(const CacheView& c, int heads, int n, int max_q, int max_kv) {
+  const int64_t rows = (int64_t)max_q * (heads / c.heads);
+  AttnPlan p;
+  p.share = rows > 32;
+  p.tiles = (int)((rows + (p.share ? 63 : 15)) / (p.share ? 64 : 16));
+  const int64_t units = (int64_t)n * c.heads * p.tiles;
+  const int64_t most = std::min<int64_t>(p.share ? 4096 : 1024, (int64_t)CATT_PAGES * c.page - 128);
+  const int64_t want = (units * max_kv + 1183) / 1184;  // four rounds of two blocks on 148 SMs
+  p.chunk = (int)std::max<int64_t>(128, std::min(most, (want + 127) / 128 * 128));
+  p.chunks = (int)std::max<int64_t>(1, ((int64_t)max_kv + p.chunk - 1) / p.chunk);
+  return p;
+}
+size_t attention_workspace(const AttnPlan& p, const CacheView& c, int heads, int n, int max_q) {
+  return p.chunks == 1 ? 0 : (size_t)n * max_q * heads * p.chunks * (c.dim + 1) * sizeof(float);
+}
+
+template <typename T, int D, bool SHARE>
+void launch_attention(const CacheView& c, const CacheAttnArgs& a, int dev, cudaStream_t st) {
+  constexpr auto KERNEL = cache_attention_kernel<T, D, SHARE>;
+  const uint64_t rows = (uint64_t)c.num_pages * c.heads * c.page;
+  const uint32_t box = std::min(c.page, CATT_TK);
+  const CUtensorMap k = byte_map(c.codes[0], D, rows, D, D, box), v = byte_map(c.codes[1], D, rows, D, D, box);
+  allow_smem<KERNEL>(dev);
+  KERNEL<<<dim3((unsigned)(a.n * c.heads * a.tiles), a.chunks), CATT_WARPS * 32, sizeof(CacheAttnSmem<D, SHARE>) + 1024, st>>>(k, v, c, a);
+  CK(cudaGetLastError());
+  if (a.chunks > 1)
+    cache_attention_join_kernel<T, D><<<(unsigned)(((int64_t)a.n * a.max_q * a.heads + 3) / 4), 128, 0, st>>>(c, a);
+}
+template <typename T>
+void launch_attention(const CacheView& c, const CacheAttnArgs& a, bool share, int dev, cudaStream_t st) {
+  if (c.dim == 64)
+    share ? launch_attention<T, 64, true>(c, a, dev, st) : launch_attention<T, 64, false>(c, a, dev, st);
+  else
+    share ? launch_attention<T, 128, true>(c, a, dev, st) : launch_attention<T, 128, false>(c, a, dev, st);
 }
 
 }  // namespace
@@ -178,7 +214,13 @@ s1c_status s1c_cache_read(const s1c_cache* cache, int32_t dtype, void* d_k, int6
 }
 
 size_t s1c_cache_attention_workspace(const s1c_cache* cache, int32_t heads, int32_t n, int32_t max_q, int32_t max_kv) {
-  return 0;
+  try {
+    const CacheView c = check_cache(cache);
+    if (heads <= 0 || heads % c.heads || n <= 0 || max_q <= 0 || max_kv <= 0) return 0;
+    return attention_workspace(plan_attention(c, heads, n, max_q, max_kv), c, heads, n, max_q);
+  } catch (...) {
+    return 0;  // a cache that the call refuses
+  }
 }
 
 s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, const void* d_q, int64_t q_stride, void* d_out,
@@ -195,17 +237,23 @@ s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, const void
     need(q_stride >= width && out_stride >= width && q_stride % 8 == 0 && out_stride % 8 == 0 && aligned(d_q, 16) && aligned(d_out, 16),
          "q and out must be 16-byte aligned, their row strides multiples of 8 that hold heads * head_dim values");
     need(std::isfinite(scale), "scale must be finite");
-    need(workspace_bytes >= s1c_cache_attention_workspace(cache, heads, n, max_q, max_kv), "workspace too small");
     if (n == 0 || max_q == 0) return;
-    need((int64_t)n * max_q <= INT_MAX, "n * max_q must stay below 2^31");
+    need((int64_t)n * max_q <= INT_MAX / heads, "n * max_q * heads must stay below 2^31");
+    const AttnPlan p = plan_attention(c, heads, n, max_q, max_kv);
+    const size_t bytes = attention_workspace(p, c, heads, n, max_q);
+    need(p.chunks <= 65535, "max_kv is too large");
+    need(workspace_bytes >= bytes && (!bytes || (d_workspace && aligned(d_workspace, 16))),
+         "workspace too small, null or not 16-byte aligned");
     OnDeviceOf dev(d_out);
-    const CacheAttnArgs a{d_q, d_out, d_lse, q_stride, out_stride, d_cu, d_len, d_pages, heads, max_pages, max_q, window,
-                          scale * 1.4426950408889634f};
+    CacheAttnArgs a{d_q, d_out, d_lse, q_stride, out_stride, d_cu, d_len, d_pages, n, heads, max_pages, max_q, window,
+                    p.tiles, p.chunk, p.chunks, scale * 1.4426950408889634f};
+    a.part = static_cast<float*>(d_workspace);
+    a.part_lse = a.part + (size_t)n * max_q * heads * p.chunks * c.dim;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == S1C_DT_F16)
-      c.dim == 64 ? launch_attention<__half, 64>(c, a, n, st) : launch_attention<__half, 128>(c, a, n, st);
+      launch_attention<__half>(c, a, p.share, dev.device, st);
     else
-      c.dim == 64 ? launch_attention<__nv_bfloat16, 64>(c, a, n, st) : launch_attention<__nv_bfloat16, 128>(c, a, n, st);
+      launch_attention<__nv_bfloat16>(c, a, p.share, dev.device, st);
     CK(cudaGetLastError());
   });
 }
