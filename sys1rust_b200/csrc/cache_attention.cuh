@@ -15,9 +15,10 @@
 //  - values: the sum runs over keys, so a register pairs two keys' codes of one dimension; words of two
 //    keys are interleaved by byte permutes, put under the exponent of 1024 and 1152 subtracted.
 //  - a page's value scale differs from its neighbours' inside one sum, so it goes into the weight: with t = log2(scale /
-//    largest scale of the block), the weight is exp2(s + t - m), m the running maximum of s + t, and the sum of
-//    the softmax adds weight * 2^-t. Weights are held as f16 (11 bits; at most 2^15, so that they keep them
-//    down to 2^-29 of the largest); scores, maxima, sums and outputs are fp32.
+//    largest scale of the block), the weight is exp2(s + t - m + 14.5), m a running maximum of s + t, and the sum of
+//    the softmax adds weight * 2^-t. m follows the true maximum only when that is 1.25 ahead, so outputs are
+//    seldom rescaled. Weights are held as f16: at most 2^15.75, with all 11 bits down to 2^-28 of the
+//    largest; scores, maxima, sums and outputs are fp32.
 //
 // Few query rows (bound by the cache's bytes): each warp has its own tiles of the block's keys and its own ring
 // of loads, so nothing waits inside the loop; the four warps' results are joined at the end. Many rows (bound by
@@ -49,23 +50,23 @@ struct CacheAttnArgs {
   float* part_lse;   // [n * max_q * heads, chunks]: their log2 sums
 };
 
-constexpr int CATT_WARPS = 4, CATT_TK = 32, CATT_PAGES = 256;  // keys of a tile; pages of a chunk at most
+constexpr int CATT_WARPS = 4, CATT_TK = 32, CATT_PAGES = 128;  // keys of a tile; pages of a chunk at most
 
 template <int D, bool SHARE>
 struct CacheAttnSmem {
   static constexpr int TILE = 2 * CATT_TK * D;  // keys and values of a tile
-  static constexpr int STAGES = SHARE ? 6 : D == 128 ? 3 : 5;
+  static constexpr int STAGES = SHARE ? 4 : D == 128 ? 2 : 4;
   static constexpr int RINGS = SHARE ? 1 : CATT_WARPS;
   alignas(1024) uint8_t ring[RINGS][STAGES][TILE];
+  uint4 q[SHARE ? CATT_WARPS : 1][D / 16][32];  // operands of the query rows
   uint64_t full[RINGS][STAGES], empty[STAGES];
-  int page[CATT_PAGES];
-  float k_scale[CATT_PAGES], v_log[CATT_PAGES], v_inv[CATT_PAGES];  // key scale * 2^24; t; 2^-t
+  float4 page[CATT_PAGES + 2];  // key scale * 2^24, t, 2^-t, page (-1 outside the cache: 0, -inf, 0)
   float top[CATT_WARPS];
   float row_m[CATT_WARPS][16], row_l[CATT_WARPS][16];
 };
 
 template <typename T, int D, bool SHARE>
-__global__ void __launch_bounds__(CATT_WARPS * 32, 2)
+__global__ void __launch_bounds__(CATT_WARPS * 32, 3)
 cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const CacheView c,
                        const CacheAttnArgs a) {
   using S = CacheAttnSmem<D, SHARE>;
@@ -79,6 +80,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   const int h = blockIdx.x % c.heads, seq = blockIdx.x / c.heads % a.n, qt = a.tiles - 1 - blockIdx.x / c.heads / a.n;
   const int first = a.cu[seq], count = a.cu[seq + 1] - first, L = a.len[seq];
   const int rows = min(count, a.max_q) * G, row0 = qt * ROWS;
+  pdl_trigger();
   if (row0 >= rows) return;
   const int chunk = blockIdx.y;
   // keys that some row of the block sees, in this chunk
@@ -115,62 +117,59 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     // the chunk's pages and scales
     const int p0 = lo >> shift, pages = ((hi - 1) >> shift) - p0 + 1;
     float top = 0.f;
-    for (int i = tid; i < pages; i += CATT_WARPS * 32) {
-      const int page = cache_page(a.table, a.max_pages, seq, p0 + i, c.num_pages);
+    for (int i = tid; i < pages + 2; i += CATT_WARPS * 32) {
+      const int page = i < pages ? cache_page(a.table, a.max_pages, seq, p0 + i, c.num_pages) : -1;
       float ks = 0.f, vs = 0.f;
       if (page >= 0) {
         const int64_t slot = (int64_t)page * c.heads + h;
         ks = c.scales[0][slot], vs = c.scales[1][slot];
       }
-      sm.page[i] = page, sm.k_scale[i] = ks * 0x1p24f, sm.v_log[i] = vs;
+      sm.page[i] = make_float4(ks * 0x1p24f, vs, 0.f, __int_as_float(page));
       top = fmaxf(top, vs);
     }
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) sm.top[w] = top;
     __syncthreads();
     top = fmaxf(fmaxf(sm.top[0], sm.top[1]), fmaxf(sm.top[2], sm.top[3]));
-    for (int i = tid; i < pages; i += CATT_WARPS * 32) {
+    for (int i = tid; i < pages + 2; i += CATT_WARPS * 32) {
+      float4 e = sm.page[i];
       // scales below 2^-60 of the largest (and zero ones, whose codes are zero) count as that
-      const float t = top > 0.f ? fmaxf(log2f(sm.v_log[i] / top), -60.f) : 0.f;
-      sm.v_log[i] = t, sm.v_inv[i] = exp2f(-t);
+      const float l2 = top > 0.f ? fmaxf(log2f(e.y / top), -60.f) : 0.f;
+      const bool in = __float_as_int(e.w) >= 0;
+      e.y = in ? l2 : -INFINITY, e.z = in ? exp2f(-l2) : 0.f;
+      sm.page[i] = e;
     }
     __syncthreads();
   }
   const float v_top = tiles > 0 ? fmaxf(fmaxf(sm.top[0], sm.top[1]), fmaxf(sm.top[2], sm.top[3])) : 0.f;
 
-  // loads of tile i into its slot; pages outside the cache are not read
-  const int per = c.page < CATT_TK ? c.page : CATT_TK;  // rows of a box
-  const int boxes = CATT_TK / per;
+  // Loads of tile i into its slot, by a whole warp: a lane for each page (one, or two of 16 rows). Pages outside the
+  // cache are not read.
+  const int per = min(c.page, CATT_TK), boxes = CATT_TK / per;
   const auto issue = [&](int i) {
     const int ring = SHARE ? 0 : w, slot = (SHARE ? i : i / CATT_WARPS) % S::STAGES;
-    const int key = lo + i * CATT_TK, p0 = lo >> shift;
+    const int at = lo + i * CATT_TK + lane * per;
     uint64_t* bar = &sm.full[ring][slot];
-    int bytes = 0;
-    for (int b = 0; b < boxes; ++b) {
-      const int at = key + b * per;
-      if (at < hi && sm.page[(at >> shift) - p0] >= 0) bytes += 2 * per * D;
-    }
-    if (bytes)
-      mbar_arrive_expect_tx(bar, bytes);
-    else
-      mbar_arrive(bar);
-    for (int b = 0; b < boxes; ++b) {
-      const int at = key + b * per;
-      const int page = at < hi ? sm.page[(at >> shift) - p0] : -1;
-      if (page < 0) continue;
+    const int page = lane < boxes && at < hi ? __float_as_int(sm.page[(at >> shift) - (lo >> shift)].w) : -1;
+    const int count = __popc(__ballot_sync(0xffffffffu, page >= 0));
+    if (lane == 0) mbar_arrive_expect_tx(bar, count * 2 * per * D);
+    __syncwarp();
+    if (page >= 0) {
       const int y = (page * c.heads + h) * c.page + (at & (c.page - 1));
-      tma_load_2d(sm.ring[ring][slot] + b * per * D, &k_map, bar, 0, y);
-      tma_load_2d(sm.ring[ring][slot] + CATT_TK * D + b * per * D, &v_map, bar, 0, y);
+      tma_load_2d(sm.ring[ring][slot] + lane * per * D, &k_map, bar, 0, y);
+      tma_load_2d(sm.ring[ring][slot] + CATT_TK * D + lane * per * D, &v_map, bar, 0, y);
     }
+    __syncwarp();
   };
   const int step = SHARE ? 1 : CATT_WARPS, begin = SHARE ? 0 : w;
-  if (lane == 0 && (!SHARE || w == 0))
+  if (!SHARE || w == 0)
     for (int s = 0; s < (SHARE ? S::STAGES - 1 : S::STAGES); ++s)
       if (begin + s * step < tiles) issue(begin + s * step);
 
   // q as operands: lane (g, cq) holds dimensions 16 i + 4 cq .. + 3 of rows g and g + 8
-  uint32_t qa[QK][4];
   float factor[2], start[2];
+  {
+  uint32_t qa[QK][4];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const T* q = static_cast<const T*>(a.q) + at_row[e] * a.q_stride + head[e] * D + cq * 4;
@@ -197,6 +196,15 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     factor[e] = a.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
     start[e] = sum * -0x1p-17f;  // -128 * 2^-24
   }
+  if (SHARE || w == 0)
+#pragma unroll
+    for (int i = 0; i < QK; ++i) sm.q[SHARE ? w : 0][i][lane] = make_uint4(qa[i][0], qa[i][1], qa[i][2], qa[i][3]);
+  if (SHARE)
+    __syncwarp();
+  else
+    __syncthreads();
+  }
+  const uint32_t q_at = smem_u32(&sm.q[SHARE ? w : 0][0][lane]);
 
   // shared offsets in a slot: the swizzle moves a row's 16-byte pieces by the row (128-byte rows) or by half of it
   const int kr = D == 128 ? g : (g & 4) | (g & 1) << 1 | (g >> 1 & 1);
@@ -228,8 +236,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       // the slot of tile i - 1, when all warps are through with it
       const int prev = (i + S::STAGES - 1) % S::STAGES;
       if (i > 0 && !broken && !mbar_wait_warp(&sm.empty[prev], ((i - 1) / S::STAGES) & 1, nullptr, 0, nullptr)) broken = true;
-      if (lane == 0 && !broken) issue(i + S::STAGES - 1);
-      __syncwarp();
+      if (!broken) issue(i + S::STAGES - 1);
     }
     if (!broken && !mbar_wait_warp(&sm.full[SHARE ? 0 : w][slot], phase, nullptr, 0, nullptr)) broken = true;
     if (broken) break;
@@ -239,41 +246,51 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     // scores, in units of the key scale * factor
     float s[4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[j][0] = s[j][1] = start[0], s[j][2] = s[j][3] = start[1];
-#pragma unroll
-      for (int d = 0; d < QK; ++d) {
-        const uint32_t v = lds_at(base + k_at[d], j * 8 * D) ^ 0x80808080u;
-        mma_f16(s[j], qa[d], __byte_perm(v, 0, 0x4140), __byte_perm(v, 0, 0x4342));
-      }
-    }
+    for (int j = 0; j < 4; ++j) s[j][0] = s[j][1] = start[0], s[j][2] = s[j][3] = start[1];
+    static_for<QK>([&](auto DD) {
+      constexpr int d = decltype(DD)::value;
+      const uint32_t at = base + k_at[d];
+      const uint4 qv = lds_v4<d * 512>(q_at);
+      const uint32_t qa[4] = {qv.x, qv.y, qv.z, qv.w};
+      static_for<4>([&](auto J) {
+        constexpr int j = decltype(J)::value;
+        const uint32_t v = lds_u32<j * 8 * D>(at) ^ 0x80808080u;
+        mma_f16(s[j], qa, __byte_perm(v, 0, 0x4140), __byte_perm(v, 0, 0x4342));
+      });
+    });
     // log2 of the weights; masked where the tile is not seen in whole
     const bool open = key + CATT_TK - 1 <= qpos[0] && key >= qpos[1] - window && key + CATT_TK <= hi;
     float top[2] = {-INFINITY, -INFINITY}, inv[4];
-    const bool all = __all_sync(0xffffffffu, open);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int p = pg + (((key & (c.page - 1)) + j * 8) >> shift);
-      // the last tile's rows behind the chunk's last page have none
-      const bool ok = key + j * 8 < hi && sm.page[p] >= 0;
-      const float ks = ok ? sm.k_scale[p] : 0.f, t = ok ? sm.v_log[p] : -INFINITY;
-      inv[j] = ok ? sm.v_inv[p] : 0.f;
+      const float4 p = sm.page[pg + (((key & (c.page - 1)) + j * 8) >> shift)];
+      inv[j] = p.z;
+      const float f0 = factor[0] * p.x, f1 = factor[1] * p.x;
+      s[j][0] = fmaf(s[j][0], f0, p.y), s[j][1] = fmaf(s[j][1], f0, p.y);
+      s[j][2] = fmaf(s[j][2], f1, p.y), s[j][3] = fmaf(s[j][3], f1, p.y);
+    }
+    if (!__all_sync(0xffffffffu, open)) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[j][e] = fmaf(s[j][e], factor[e / 2] * ks, t);
-        if (!all) {
-          const int at = key + j * 8 + (e % 2 ? kc1 : kc0);
-          if (at > qpos[e / 2] || at >= hi || at < qpos[e / 2] - window) s[j][e] = -INFINITY;
+      for (int e = 0; e < 2; ++e) {
+        // key + 8 j + kc within [qpos - window, min(qpos, hi - 1)]
+        const int last = min(qpos[e], hi - 1) - key, from = qpos[e] - window - key;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (j * 8 + kc0 > last || j * 8 + kc0 < from) s[j][2 * e] = -INFINITY;
+          if (j * 8 + kc1 > last || j * 8 + kc1 < from) s[j][2 * e + 1] = -INFINITY;
         }
-        top[e / 2] = fmaxf(top[e / 2], s[j][e]);
       }
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top[e / 2] = fmaxf(top[e / 2], s[j][e]);
     bool grows = false;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
       top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-      grows |= top[e] > m[e];
+      grows |= top[e] > m[e] + 1.25f;
     }
     if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
@@ -284,8 +301,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         for (int i2 = 0; i2 < SEG * 4; ++i2) o[i2][2 * e] *= keep, o[i2][2 * e + 1] *= keep;
       }
     }
-    // weights times 2^15, and their sum without the value scales
-    const float off[2] = {m[0] == -INFINITY ? 0.f : 15.f - m[0], m[1] == -INFINITY ? 0.f : 15.f - m[1]};
+    // weights times 2^14.5, and their sum without the value scales
+    const float off[2] = {m[0] == -INFINITY ? 0.f : 14.5f - m[0], m[1] == -INFINITY ? 0.f : 14.5f - m[1]};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -294,31 +311,35 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         l[e / 2] = fmaf(s[j][e], inv[j], l[e / 2]);
       }
     // outputs
+    uint32_t pa[2][4];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const uint32_t pa[4] = {pack_f16x2(s[2 * k][0], s[2 * k][1]), pack_f16x2(s[2 * k][2], s[2 * k][3]),
-                              pack_f16x2(s[2 * k + 1][0], s[2 * k + 1][1]), pack_f16x2(s[2 * k + 1][2], s[2 * k + 1][3])};
+      pa[k][0] = pack_f16x2(s[2 * k][0], s[2 * k][1]), pa[k][1] = pack_f16x2(s[2 * k][2], s[2 * k][3]);
+      pa[k][2] = pack_f16x2(s[2 * k + 1][0], s[2 * k + 1][1]), pa[k][3] = pack_f16x2(s[2 * k + 1][2], s[2 * k + 1][3]);
+    }
 #pragma unroll
-      for (int q = 0; q < SEG; ++q) {
+    for (int q = 0; q < SEG; ++q) {
+      const uint32_t at0 = base + v_at[0][q], at1 = base + v_at[1][q];
+      static_for<2>([&](auto KK) {
+        constexpr int k = decltype(KK)::value;
         uint32_t b[4][2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t x = lds_at(base + v_at[0][q], (k * 16 + e * 8) * D) ^ 0x80808080u;
-          const uint32_t y = lds_at(base + v_at[1][q], (k * 16 + e * 8) * D) ^ 0x80808080u;
+        static_for<2>([&](auto E) {
+          constexpr int e = decltype(E)::value;
+          const uint32_t x = lds_u32<(k * 16 + e * 8) * D>(at0) ^ 0x80808080u, y = lds_u32<(k * 16 + e * 8) * D>(at1) ^ 0x80808080u;
           const uint32_t even = __byte_perm(x, y, 0x6420), odd = __byte_perm(x, y, 0x7531);
           b[0][e] = code_pair(__byte_perm(even, 0x64646464u, 0x4240)), b[1][e] = code_pair(__byte_perm(odd, 0x64646464u, 0x4240));
           b[2][e] = code_pair(__byte_perm(even, 0x64646464u, 0x4341)), b[3][e] = code_pair(__byte_perm(odd, 0x64646464u, 0x4341));
-        }
+        });
 #pragma unroll
-        for (int d = 0; d < 4; ++d) mma_f16(o[q * 4 + d], pa, b[d][0], b[d][1]);
-      }
+        for (int d = 0; d < 4; ++d) mma_f16(o[q * 4 + d], pa[k], b[d][0], b[d][1]);
+      });
     }
     if (SHARE) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.empty[slot]);
     } else {
       __syncwarp();
-      if (lane == 0 && i + S::STAGES * step < tiles) issue(i + S::STAGES * step);
+      if (i + S::STAGES * step < tiles) issue(i + S::STAGES * step);
     }
   }
 #pragma unroll
@@ -329,7 +350,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 
   // One row's result: o / l and log2 of the sum. Without a key l is 0: o = 0 and -inf.
   const auto put = [&](int64_t grow, int hd, int d, const float* v, int n, float sum, float max_) {
-    const float by = sum == 0.f ? 0.f : v_top / sum, log_sum = sum == 0.f ? -INFINITY : max_ - 15.f + log2f(sum);
+    const float by = sum == 0.f ? 0.f : v_top / sum, log_sum = sum == 0.f ? -INFINITY : max_ - 14.5f + log2f(sum);
     if (a.chunks > 1) {
       const int64_t at = ((int64_t)(seq * a.max_q + (grow - first)) * a.heads + hd) * a.chunks + chunk;
       for (int i = 0; i < n; ++i) a.part[at * D + d + i] = v[i] * by;
@@ -386,35 +407,53 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   }
 }
 
-// Joins the chunks of a row: weights 2^(lse - max). One warp for each row and head.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) cache_attention_join_kernel(const CacheView c, const CacheAttnArgs a) {
+// Joins the chunks of a row: weights 2^(lse - max). One block for each row and head; its warps share the
+// chunks, several loads of each in flight, and are summed in order.
+template <typename T, int D, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) cache_attention_join_kernel(const CacheAttnArgs a) {
   constexpr int E = D / 32;
-  const int lane = threadIdx.x % 32;
-  const int64_t item = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;  // (seq, row, head)
+  __shared__ float tops[WARPS], sums[WARPS], outs[WARPS][D];
+  const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t item = blockIdx.x;  // (sequence, row, head)
   const int head = (int)(item % a.heads), i = (int)(item / a.heads % a.max_q);
   const int64_t seq = item / a.heads / a.max_q;
-  if (seq >= a.n || i >= a.cu[seq + 1] - a.cu[seq]) return;
+  pdl_wait();
+  const int first = a.cu[seq];
+  if (i >= a.cu[seq + 1] - first) return;
   const float* lse = a.part_lse + item * a.chunks;
   float top = -INFINITY;
-  for (int s = lane; s < a.chunks; s += 32) top = fmaxf(top, lse[s]);
+  for (int s = threadIdx.x; s < a.chunks; s += WARPS * 32) top = fmaxf(top, lse[s]);
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) tops[w] = top;
+  __syncthreads();
+  for (int j = 0; j < WARPS; ++j) top = fmaxf(top, tops[j]);
   float sum = 0.f, o[E] = {};
   if (top != -INFINITY) {
-    for (int s = 0; s < a.chunks; ++s) {
+#pragma unroll 8
+    for (int s = w; s < a.chunks; s += WARPS) {
       const float by = exp2f(lse[s] - top);
-      if (by == 0.f) continue;  // also chunks without a key, whose outputs are not written
-      sum += by;
       const float* p = a.part + (item * a.chunks + s) * D + lane * E;
+      float v[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] += by * p[e];
+      for (int e = 0; e < E; ++e) v[e] = p[e];
+      sum += by;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] += by == 0.f ? 0.f : by * v[e];  // a chunk without a key has written no output
     }
   }
-  const int64_t row = a.cu[seq] + i;
-  T* out = static_cast<T*>(a.out) + row * a.out_stride + head * D + lane * E;
+  if (lane == 0) sums[w] = sum;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[e] = from_f32<T>(sum == 0.f ? 0.f : o[e] / sum);
-  if (a.lse && lane == 0) a.lse[row * a.heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+  for (int e = 0; e < E; ++e) outs[w][lane * E + e] = o[e];
+  __syncthreads();
+  sum = 0.f;
+  for (int j = 0; j < WARPS; ++j) sum += sums[j];
+  const int64_t row = first + i;
+  for (int d = threadIdx.x; d < D; d += WARPS * 32) {
+    float v = 0.f;
+    for (int j = 0; j < WARPS; ++j) v += outs[j][d];
+    static_cast<T*>(a.out)[row * a.out_stride + head * D + d] = from_f32<T>(sum == 0.f ? 0.f : v / sum);
+  }
+  if (a.lse && threadIdx.x == 0) a.lse[row * a.heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
 
 }  // namespace s1c

@@ -51,4 +51,17 @@ inline int sm_count(int dev) {
   return n;
 }
 
+// Launches a kernel that may start while the one before it on the stream ends (it calls pdl_wait before
+// it reads what that one writes).
+template <typename... P, typename... A>
+void launch_after(void (*kernel)(P...), unsigned blocks, unsigned threads, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks), cfg.blockDim = dim3(threads), cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  CK(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
 }  // namespace s1c

@@ -1,5 +1,7 @@
 // Warp-level f16 products and their operands from 16-bit and 8-bit values.
 #pragma once
+#include <utility>
+
 #include "common.cuh"
 
 namespace s1c {
@@ -16,11 +18,33 @@ S1C_DEV void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A word of shared memory at an address and an offset that the compiler knows.
-S1C_DEV uint32_t lds_at(uint32_t at, int off) {
+// Loads from shared memory at an address and a constant offset.
+template <int OFF>
+S1C_DEV uint32_t lds_u32(uint32_t at) {
   uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at + off));
+  asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(v) : "r"(at), "n"(OFF));
   return v;
+}
+template <int OFF>
+S1C_DEV float lds_f32(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1 + %2];" : "=f"(v) : "r"(at), "n"(OFF));
+  return v;
+}
+template <int OFF>
+S1C_DEV uint4 lds_v4(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at), "n"(OFF));
+  return v;
+}
+// f(integral_constant 0), ..., f(integral_constant N - 1).
+template <typename F, int... I>
+S1C_DEV void static_for_(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+S1C_DEV void static_for(F&& f) {
+  static_for_(f, std::make_integer_sequence<int, N>{});
 }
 
 // Two codes + 128 under the exponent of 1024 (1024 + 128 + code) to two f16 codes.

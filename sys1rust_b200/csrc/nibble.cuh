@@ -25,8 +25,6 @@
 //    in the warps' order, hence the same bits in each call;
 //  - otherwise each warp has whole tiles, and x passes through shared memory in blocks of columns.
 #pragma once
-#include <utility>
-
 #include "mma.cuh"
 
 namespace s1c {
@@ -61,27 +59,6 @@ S1C_DEV void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory")
 template <int N>
 S1C_DEV void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-template <int OFF>
-S1C_DEV float lds_f32(uint32_t at) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1 + %2];" : "=f"(v) : "r"(at), "n"(OFF));
-  return v;
-}
-template <int OFF>
-S1C_DEV uint4 lds_v4(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at), "n"(OFF));
-  return v;
-}
-template <typename F, int... I>
-S1C_DEV void static_for_(F&& f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-S1C_DEV void static_for(F&& f) {
-  static_for_(f, std::make_integer_sequence<int, N>{});
 }
 
 // Shared memory of one block, in bytes.

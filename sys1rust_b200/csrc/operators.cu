@@ -108,7 +108,7 @@ AttnPlan plan_attention(const CacheView& c, int heads, int n, int max_q, int max
   p.share = rows > 32;
   p.tiles = (int)((rows + (p.share ? 63 : 15)) / (p.share ? 64 : 16));
   const int64_t units = (int64_t)n * c.heads * p.tiles;
-  const int64_t most = std::min<int64_t>(p.share ? 4096 : 1024, (int64_t)CATT_PAGES * c.page - 128);
+  const int64_t most = std::min<int64_t>(p.share ? 4096 : 2048, (int64_t)CATT_PAGES * c.page - 128);
   const int64_t want = (units * max_kv + 1183) / 1184;  // four rounds of two blocks on 148 SMs
   p.chunk = (int)std::max<int64_t>(128, std::min(most, (want + 127) / 128 * 128));
   p.chunks = (int)std::max<int64_t>(1, ((int64_t)max_kv + p.chunk - 1) / p.chunk);
@@ -127,8 +127,13 @@ void launch_attention(const CacheView& c, const CacheAttnArgs& a, int dev, cudaS
   allow_smem<KERNEL>(dev);
   KERNEL<<<dim3((unsigned)(a.n * c.heads * a.tiles), a.chunks), CATT_WARPS * 32, sizeof(CacheAttnSmem<D, SHARE>) + 1024, st>>>(k, v, c, a);
   CK(cudaGetLastError());
-  if (a.chunks > 1)
-    cache_attention_join_kernel<T, D><<<(unsigned)(((int64_t)a.n * a.max_q * a.heads + 3) / 4), 128, 0, st>>>(c, a);
+  if (a.chunks > 1) {
+    const unsigned rows_ = (unsigned)((int64_t)a.n * a.max_q * a.heads);
+    if (a.chunks > 16)
+      launch_after(cache_attention_join_kernel<T, D, 16>, rows_, 512, st, a);
+    else
+      launch_after(cache_attention_join_kernel<T, D, 4>, rows_, 128, st, a);
+  }
 }
 template <typename T>
 void launch_attention(const CacheView& c, const CacheAttnArgs& a, bool share, int dev, cudaStream_t st) {
@@ -232,7 +237,8 @@ s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, const void
     check_half(dtype);
     need(d_q && d_out && d_cu && d_len && d_pages, "null argument");
     need(heads > 0 && heads % c.heads == 0, "heads must be a multiple of kv_heads");
-    need(n >= 0 && max_q >= 0 && max_kv >= 0 && max_pages > 0, "n, max_q and max_kv must not be negative, max_pages positive");
+    need(n >= 0 && max_q >= 0 && max_kv >= 0 && max_kv <= (1 << 30) && max_pages > 0,
+         "n, max_q and max_kv must not be negative, max_kv at most 2^30, max_pages positive");
     const int64_t width = (int64_t)heads * c.dim;
     need(q_stride >= width && out_stride >= width && q_stride % 8 == 0 && out_stride % 8 == 0 && aligned(d_q, 16) && aligned(d_out, 16),
          "q and out must be 16-byte aligned, their row strides multiples of 8 that hold heads * head_dim values");
