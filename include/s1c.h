@@ -335,7 +335,7 @@ S1C_API s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, co
  * summed so far exceeds u times the kept mass (u >= 1 or NaN: the last kept one); prob (nullable) is its share of the kept mass.
  * T <= 0 or NaN takes the largest logit, the lowest index among equals, with prob 1. temperature, top_k, top_p and min_p hold
  * a value for each row and are nullable (1, off, off, off). Logits of -inf are never chosen; a row with a
- * NaN or +inf, or with nothing above -inf, gets token -1 and prob 0. vocab is at most 2^20. */
+ * NaN or +inf, or with nothing above -inf, gets token -1 and prob 0. vocab is at most 2^18. */
 S1C_API s1c_status s1c_sample(int32_t dtype, const void* d_logits, int64_t row_stride, int32_t rows, int32_t vocab,
                               const float* d_temperature, const int32_t* d_top_k, const float* d_top_p,
                               const float* d_min_p, const float* d_uniform, int32_t* d_token, float* d_prob,

@@ -143,6 +143,28 @@ void launch_attention(const CacheView& c, const CacheAttnArgs& a, bool share, in
     share ? launch_attention<T, 128, true>(c, a, dev, st) : launch_attention<T, 128, false>(c, a, dev, st);
 }
 
+// A row is shared by a cluster of up to eight blocks: so many that a block's part fits in shared memory, and
+// more while there are SMs for them and each keeps a thousand logits.
+template <typename T>
+void launch_sample(SampleArgs a, int rows, int dev, cudaStream_t st) {
+  constexpr int FIXED = (sizeof(SampleShared) + 15) / 16 * 16, ROOM = (227 * 1024 - FIXED) / (int)sizeof(T);
+  int blocks = 1;
+  const auto slice = [&] { return ((a.vocab + blocks - 1) / blocks + 7) / 8 * 8; };
+  while (blocks < SMP_CLUSTER && (slice() > ROOM || (2 * blocks * rows <= sm_count(dev) && slice() >= 2048))) blocks *= 2;
+  a.slice = slice();
+  need(a.slice <= ROOM, "vocab is too large for this type");
+  a.vec = aligned(a.logits, 16) && a.stride * (int64_t)sizeof(T) % 16 == 0;
+  allow_smem<sample_kernel<T>>(dev);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(rows * blocks)), cfg.blockDim = dim3(SMP_THREADS), cfg.stream = st;
+  cfg.dynamicSmemBytes = FIXED + a.slice * sizeof(T);
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = blocks, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  CK(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a));
+}
+
 }  // namespace
 
 extern "C" {
@@ -270,18 +292,19 @@ s1c_status s1c_sample(int32_t dtype, const void* d_logits, int64_t row_stride, i
   return enter([&] {
     need(dtype == S1C_DT_F32 || dtype == S1C_DT_F16 || dtype == S1C_DT_BF16, "dtype must be S1C_DT_F32, F16 or BF16");
     need(d_logits && d_uniform && d_token, "null argument");
-    need(rows >= 0 && vocab > 0 && vocab <= (1 << 20), "rows must not be negative, vocab 1 to 2^20");
+    need(rows >= 0 && vocab > 0 && vocab <= (1 << 18), "rows must not be negative, vocab 1 to 2^18");
+    need(rows <= INT_MAX / SMP_CLUSTER, "too many rows");
     need(row_stride >= vocab, "a row stride is shorter than its row");
     if (rows == 0) return;
     OnDeviceOf dev(d_token);
-    const SampleArgs a{d_logits, row_stride, vocab, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_token, d_prob};
+    SampleArgs a{d_logits, row_stride, vocab, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_token, d_prob};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == S1C_DT_F32)
-      sample_kernel<float><<<rows, SMP_THREADS, 0, st>>>(a);
+      launch_sample<float>(a, rows, dev.device, st);
     else if (dtype == S1C_DT_F16)
-      sample_kernel<__half><<<rows, SMP_THREADS, 0, st>>>(a);
+      launch_sample<__half>(a, rows, dev.device, st);
     else
-      sample_kernel<__nv_bfloat16><<<rows, SMP_THREADS, 0, st>>>(a);
+      launch_sample<__nv_bfloat16>(a, rows, dev.device, st);
     CK(cudaGetLastError());
   });
 }
