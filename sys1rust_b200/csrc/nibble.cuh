@@ -281,7 +281,6 @@ S1C_DEV void nibble_stage(const NibbleArgs& a, __half* xs, float* sums, float* r
                           int first, int passes, int groups) {
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int parts = a.M >= WARPS ? 1 : WARPS / a.M;
-  const T* x = static_cast<const T*>(a.x);
   // where the lane's eight columns go among the 16 pieces of their 128: word j of lane c
   const int i = lane % 16;
   const int j = GROUP == 128 ? i % 4 : GROUP == 64 ? i / 8 * 2 + i % 2 : i / 4, c = GROUP == 128 ? i / 4 : GROUP == 64 ? i % 8 / 2 : i % 4;

@@ -143,21 +143,18 @@ void launch_attention(const CacheView& c, const CacheAttnArgs& a, bool share, in
     share ? launch_attention<T, 128, true>(c, a, dev, st) : launch_attention<T, 128, false>(c, a, dev, st);
 }
 
-// A row is shared by a cluster of up to eight blocks: so many that a block's part fits in shared memory, and
-// more while there are SMs for them and each keeps a thousand logits.
+// A row is shared by a cluster of up to eight blocks, as long as there are SMs for them and each keeps a
+// thousand logits.
 template <typename T>
 void launch_sample(SampleArgs a, int rows, int dev, cudaStream_t st) {
-  constexpr int FIXED = (sizeof(SampleShared) + 15) / 16 * 16, ROOM = (227 * 1024 - FIXED) / (int)sizeof(T);
   int blocks = 1;
-  const auto slice = [&] { return ((a.vocab + blocks - 1) / blocks + 7) / 8 * 8; };
-  while (blocks < SMP_CLUSTER && (slice() > ROOM || (2 * blocks * rows <= sm_count(dev) && slice() >= 2048))) blocks *= 2;
-  a.slice = slice();
-  need(a.slice <= ROOM, "vocab is too large for this type");
+  while (blocks < SMP_CLUSTER && 2 * blocks * rows <= sm_count(dev) && a.vocab >= 2048 * blocks) blocks *= 2;
+  a.slice = ((a.vocab + blocks - 1) / blocks + 7) / 8 * 8;
   a.vec = aligned(a.logits, 16) && a.stride * (int64_t)sizeof(T) % 16 == 0;
   allow_smem<sample_kernel<T>>(dev);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * blocks)), cfg.blockDim = dim3(SMP_THREADS), cfg.stream = st;
-  cfg.dynamicSmemBytes = FIXED + a.slice * sizeof(T);
+  cfg.dynamicSmemBytes = sizeof(SampleShared);
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = blocks, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;

@@ -8,13 +8,14 @@
 // No sort is needed: both filters cut the order at one value, so each is a threshold (a logit, and how
 // many of its equals are kept, by index). A cluster of blocks shares a row:
 //
-//  1. each block copies its part to shared memory and finds the largest logit;
+//  1. each block finds the largest logit of its part (which it reads again, from the cache, in each step: two
+//     blocks on an SM, whose waits overlap, are worth more than a copy in shared memory);
 //  2. the counts of the logits in bins of z, 1/32 of a power of two wide, and where top-p needs it the exact
 //     mass of all, give a bin below which nothing can be kept;
-//  3. what stands above, a few hundred of fifty thousand as a rule, is gathered in the order of the indexes in the first
-//     block, which finds the thresholds exactly, by histograms over bins of z and, inside the bin
-//     that holds the cut, over the order-preserving integer of the logit, 2048 ways at a time, until one
-//     value is left; and then sums and walks what is kept. More than fit are worked on in place.
+//  3. what stands above is gathered in the order of the indexes in the first block. Up to 512 of them are
+//     sorted, one by each thread. More have their thresholds found by histograms over bins of z and, inside the bin that holds the cut, over the order-preserving integer
+//     of the logit, 2048 ways at a time, until one value is left. What is kept is summed and walked. More
+//     than fit in the list are worked on in place.
 //
 // Masses are integers: e = m * 2^(n - 24), m an integer of 25 bits, and all e in one bin share n. So their sums are
 // exact and depend neither on the order of atomics nor on how a row is shared. Logits more than 45 powers of two
@@ -22,7 +23,7 @@
 #pragma once
 #include <cooperative_groups.h>
 
-#include "common.cuh"
+#include "mma.cuh"
 
 namespace s1c {
 
@@ -41,8 +42,8 @@ struct SampleArgs {
   int vec;      // rows are 16-byte aligned
 };
 
-constexpr int SMP_THREADS = 1024, SMP_WARPS = SMP_THREADS / 32, SMP_BINS = 2048, SMP_ZBINS = 45 * 32, SMP_LIST = 8192;
-constexpr int SMP_CLUSTER = 8;
+constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32, SMP_BINS = 2048, SMP_ZBINS = 45 * 32, SMP_LIST = 4096;
+constexpr int SMP_PER = SMP_BINS / SMP_THREADS, SMP_CLUSTER = 8;
 
 // The order-preserving integer of a logit: a > b as floats exactly if it is so for the keys.
 S1C_DEV uint32_t logit_key(float l) {
@@ -51,21 +52,28 @@ S1C_DEV uint32_t logit_key(float l) {
 }
 S1C_DEV float key_logit(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
+// The larger of two; NaN where one is.
+S1C_DEV float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
 S1C_DEV double pow2(int e) { return __hiloint2double((1023 + e) << 20, 0); }
 
 // exp as an integer: the bin of z and m with e = m * 2^(n - 24), n from the bin. The bin comes from the rounded product (it
 // only has to be monotonic); the mass adds what the difference and the product lost. 2^f by the Taylor series of
-// exp(f ln 2), |f| <= 1/2: its tenth term is below 1e-10, and rounding to fp32 leaves about 5e-8.
+// exp(f ln 2), |f| <= 0.52: its tenth term is below 1e-10, and rounding to fp32 leaves about 5e-8.
 struct SampleMass {
   float top, rate, rate_lo;  // max l, log2(e) / T in two parts
   S1C_DEV SampleMass(float top_, float T) : top(top_) {
     const double r = fmin(1.4426950408889634 / (double)T, 1e38);
     rate = (float)r, rate_lo = (float)(r - (double)rate);
   }
-  S1C_DEV int bin(float l) const {
-    const float t = (top - l) * rate * 32.f;
-    return t < (float)SMP_ZBINS ? (int)t : SMP_ZBINS;
-  }
+  S1C_DEV float z(float l) const { return (top - l) * rate; }
+  // 32 z to the nearest integer, by the place that adding 2^23 gives it
+  static S1C_DEV int bin_of(float z) { return z < 44.5f ? __float_as_int(fmaf(z, 32.f, 8388608.f)) & 0xfff : SMP_ZBINS; }
+  S1C_DEV int bin(float l) const { return bin_of(z(l)); }
   static S1C_DEV int power(int bin) { return -((bin + 16) >> 5); }
   S1C_DEV uint32_t mass(float l, int bin) const {
     const float d = top - l, lost = (top - d) - l, z = d * rate;
@@ -87,7 +95,7 @@ struct SampleMass {
   S1C_DEV unsigned long long fixed(float l, int bin) const { return ((unsigned long long)mass(l, bin) << 20) >> -power(bin); }
 };
 
-struct SampleShared {
+struct alignas(16) SampleShared {
   // elements of a bin; sums of the low 12 and the high 13 bits of their masses (below 2^32 for 2^18 elements)
   uint32_t count[SMP_BINS], lo[SMP_BINS], hi[SMP_BINS];
   float value[SMP_LIST];  // what step 3 works on
@@ -101,7 +109,7 @@ struct SampleShared {
   double found_mass;
   // read by the other blocks of the cluster
   float top;
-  int at, bad;
+  int at;
   uint32_t listed;
   unsigned long long sum;
   S1C_DEV unsigned long long mass(int b) const { return ((unsigned long long)hi[b] << 12) + lo[b]; }
@@ -127,17 +135,18 @@ struct SampleItems {
 template <bool MASS>
 S1C_DEV void sample_find(SampleShared& s, int bins, double want, bool zbins, double scale) {
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-  const int b0 = 2 * t;
-  double m[2] = {0, 0};
-  uint32_t c[2] = {0, 0};
+  const int b0 = SMP_PER * t;
+  double m[SMP_PER], dm = 0;
+  uint32_t c[SMP_PER], dc = 0;
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
-    if (b0 + j < bins) {
-      c[j] = s.count[b0 + j];
-      if (MASS) m[j] = (double)s.mass(b0 + j) * (zbins ? pow2(SampleMass::power(b0 + j) - 24) : scale);
-    }
-  double dm = m[0] + m[1];
-  uint32_t dc = c[0] + c[1];
+  for (int j = 0; j < SMP_PER; ++j) {
+    const bool in = b0 + j < bins;
+    c[j] = in ? s.count[b0 + j] : 0u;
+    m[j] = MASS && in ? (double)s.mass(b0 + j) * (zbins ? pow2(SampleMass::power(b0 + j) - 24) : scale) : 0.0;
+    dm += m[j], dc += c[j];
+  }
+  const double sum_m = dm;
+  const uint32_t sum_c = dc;
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t pc = __shfl_up_sync(0xffffffffu, dc, o);
     if (lane >= o) dc += pc;
@@ -149,27 +158,37 @@ S1C_DEV void sample_find(SampleShared& s, int bins, double want, bool zbins, dou
   if (lane == 31) s.warp_d[w] = dm, s.warp_a[w] = dc;
   if (t == 0) s.found_bin = -1;
   __syncthreads();
-  double base_m = 0;
-  uint32_t base_c = 0;
-  for (int i = 0; i < w; ++i) base_m += s.warp_d[i], base_c += s.warp_a[i];
-  const double from_m = base_m + dm - (m[0] + m[1]);
-  const uint32_t from_c = base_c + dc - (c[0] + c[1]);
-  double before_m = from_m;
-  uint32_t before_c = from_c;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    if (c[j]) {
-      const bool here = MASS ? before_m < want : before_c < want && before_c + c[j] >= want;
-      if (here) atomicMax(&s.found_bin, b0 + j);
+  if (w == 0) {
+    uint32_t c0 = lane < SMP_WARPS ? s.warp_a[lane] : 0u;
+    double m0 = lane < SMP_WARPS ? s.warp_d[lane] : 0.0;
+    const uint32_t c1 = c0;
+    const double m1 = m0;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t pc = __shfl_up_sync(0xffffffffu, c0, o);
+      if (lane >= o) c0 += pc;
+      if (MASS) {
+        const double pm = __shfl_up_sync(0xffffffffu, m0, o);
+        if (lane >= o) m0 += pm;
+      }
     }
-    before_m += m[j], before_c += c[j];
+    if (lane < SMP_WARPS) s.warp_a[lane] = c0 - c1, s.warp_d[lane] = m0 - m1;
   }
   __syncthreads();
-  if (s.found_bin >= 0 && s.found_bin >> 1 == t) {
-    const int j = s.found_bin & 1;
-    s.found_mass = from_m + (j ? m[0] : 0.0);
-    s.found_count = from_c + (j ? c[0] : 0u);
+  const double base_m = s.warp_d[w];
+  const uint32_t base_c = s.warp_a[w];
+  double before_m = base_m + dm - sum_m;
+  uint32_t before_c = base_c + dc - sum_c;
+  int here = -1;  // the last of this thread's bins that qualifies, and what is before it
+  double here_m = 0;
+  uint32_t here_c = 0;
+#pragma unroll
+  for (int j = 0; j < SMP_PER; ++j) {
+    if (c[j] && (MASS ? before_m < want : before_c < want && before_c + c[j] >= want)) here = b0 + j, here_m = before_m, here_c = before_c;
+    before_m += m[j], before_c += c[j];
   }
+  if (here >= 0) atomicMax(&s.found_bin, here);
+  __syncthreads();
+  if (here >= 0 && s.found_bin == here) s.found_mass = here_m, s.found_count = here_c;
   __syncthreads();
 }
 
@@ -248,9 +267,89 @@ S1C_DEV unsigned long long sample_sum(SampleShared& s, unsigned long long v) {
   __syncthreads();
   if (threadIdx.x % 32 == 0) s.warp_u[threadIdx.x / 32] = v;
   __syncthreads();
-  v = 0;
-  for (int i = 0; i < SMP_WARPS; ++i) v += s.warp_u[i];
+  v = threadIdx.x % 32 < SMP_WARPS ? s.warp_u[threadIdx.x % 32] : 0ull;
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// Sum of v over the threads up to this one; all threads call.
+S1C_DEV unsigned long long sample_scan(SampleShared& s, unsigned long long v, unsigned long long& all) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  __syncthreads();
+  if (lane == 31) s.warp_u[w] = v;
+  __syncthreads();
+  const unsigned long long own = lane < SMP_WARPS ? s.warp_u[lane] : 0ull;
+  unsigned long long sum = own;
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long u = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += u;
+  }
+  all = __shfl_sync(0xffffffffu, sum, 31);
+  return v + __shfl_sync(0xffffffffu, sum - own, w);
+}
+
+// Step 3 for a list of up to 512, by one block: a bitonic sort of (key, place) with an element for each thread, then
+// ranks and masses are at hand.
+S1C_DEV void sample_choose_sorted(SampleShared& s, const SampleArgs& a, int r, const SampleMass& f, int n, int k, float p, double least,
+                                  unsigned long long total) {
+  const int t = threadIdx.x;
+  const bool by_k = k > 0 && k < a.vocab, by_p = p < 1.f;
+  unsigned long long* masses = reinterpret_cast<unsigned long long*>(s.count);  // [512]
+  unsigned long long* other = reinterpret_cast<unsigned long long*>(s.lo);      // [512]
+  unsigned long long v = 0;  // past the list: last in the order
+  if (t < n) v = ((unsigned long long)logit_key(s.value[t]) << 32) | (uint32_t)~t;
+  int width = 32;  // threads that sort: a power of two
+  while (width < n) width *= 2;
+  const int names = width / 32;  // warps; they meet at a barrier of their own
+  if (t < width)
+    for (int size = 2; size <= width; size <<= 1)
+      for (int step = size / 2; step; step >>= 1) {
+        unsigned long long u;
+        if (step >= 32) {
+          asm volatile("bar.sync 1, %0;" ::"r"(names * 32) : "memory");
+          other[t] = v;
+          asm volatile("bar.sync 1, %0;" ::"r"(names * 32) : "memory");
+          u = other[t ^ step];
+        } else {
+          u = __shfl_xor_sync(0xffffffffu, v, step);
+        }
+        const bool larger = !(t & step) == !(t & size);  // descending runs first
+        if (larger ? u > v : u < v) v = u;
+      }
+  // thread t now has the element of rank t
+  const int place = (int)~(uint32_t)v;
+  const float l = key_logit((uint32_t)(v >> 32));
+  const int b = t < n ? f.bin(l) : SMP_ZBINS;
+  const unsigned long long mass = b < SMP_ZBINS ? f.fixed(l, b) : 0ull;
+  bool keep = mass && (double)l >= least && !(by_k && t >= k);
+  if (by_p) {
+    unsigned long long all;
+    const unsigned long long ahead = sample_scan(s, by_k && t >= k ? 0ull : mass, all) - mass;
+    if (by_k) total = all;  // mass of what top-k keeps
+    if (t && !((double)ahead < (double)p * (double)total)) keep = false;
+  }
+  if (t < n) masses[place] = keep ? mass : 0ull;
+  if (t == 0) s.found_bin = n, s.key_hi = 0;
+  __syncthreads();
+  const unsigned long long mine = t < n ? masses[t] : 0ull;
+  unsigned long long whole;
+  const unsigned long long upto = sample_scan(s, mine, whole);
+  const double goal = (double)a.uniform[r] * (double)whole;
+  const uint32_t over = __ballot_sync(0xffffffffu, mine && (double)upto > goal), any = __ballot_sync(0xffffffffu, mine != 0);
+  if (!(t & 31)) {
+    if (over) atomicMin(&s.found_bin, t + __ffs(over) - 1);
+    if (any) atomicMax(&s.key_hi, (uint32_t)(t + 31 - __clz(any)));  // the last one: for u >= 1 or NaN
+  }
+  __syncthreads();
+  const int pick = s.found_bin < n ? s.found_bin : (int)s.key_hi;
+  if (t == pick) {
+    a.token[r] = s.index[pick];
+    if (a.prob) a.prob[r] = (float)((double)mine / (double)whole);
+  }
 }
 
 // Step 3, by one block. total: the mass of all logits, where top-p applies without top-k.
@@ -298,8 +397,7 @@ S1C_DEV void sample_choose(SampleShared& s, const SampleArgs& a, int r, const Sa
       if (by_p) {
         const int bins = min(last + 1, SMP_ZBINS);
         double mine = 0;
-        for (int j = 0; j < 2; ++j)
-          if (2 * t + j < bins) mine += (double)s.mass(2 * t + j) * pow2(SampleMass::power(2 * t + j) - 24);
+        for (int j = SMP_PER * t; j < min(bins, SMP_PER * (t + 1)); ++j) mine += (double)s.mass(j) * pow2(SampleMass::power(j) - 24);
         for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
         if (lane == 0) s.warp_d[w] = mine;
         __syncthreads();
@@ -399,10 +497,9 @@ S1C_DEV void sample_choose(SampleShared& s, const SampleArgs& a, int r, const Sa
 }
 
 template <typename T>
-__global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   SampleShared& s = *reinterpret_cast<SampleShared*>(raw);
-  T* part = reinterpret_cast<T*>(raw + (sizeof(SampleShared) + 15) / 16 * 16);
   auto cluster = cooperative_groups::this_cluster();
   const int blocks = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
   const int r = blockIdx.x / blocks, t = threadIdx.x, lane = t & 31, w = t >> 5;
@@ -410,57 +507,64 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
   const int first = min(a.vocab, me * a.slice), n = min(a.vocab, first + a.slice) - first;
   const float T_ = a.temperature ? a.temperature[r] : 1.f;
 
-  // 1. Largest logit and its first index; a NaN or +inf leaves no distribution.
-  float top = -INFINITY;
-  int at = a.vocab;
-  bool bad = false;
-  const auto look = [&](float l, int i) {
-    bad |= !(l < INFINITY);
-    if (l > top) top = l, at = i;
-  };
-  if (a.vec) {
-    constexpr int E = 16 / sizeof(T);
-    for (int i = t * E; i < n; i += SMP_THREADS * E) {
-      if (i + E <= n) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + first + i));
-        *reinterpret_cast<uint4*>(part + i) = v;
-        const T* x = reinterpret_cast<const T*>(&v);
+  // E logits of the part from the i-th on, -inf past its end
+  constexpr int E = 16 / sizeof(T);
+  const T* part = row + first;
+  const auto load = [&](float (&x)[E], int i) {
+    if (a.vec && i + E <= n) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(part + i));
 #pragma unroll
-        for (int e = 0; e < E; ++e) look(to_f32(x[e]) + 0.f, first + i + e);
-      } else {
-        for (int e = i; e < n; ++e) part[e] = row[first + e], look(to_f32(part[e]) + 0.f, first + e);
-      }
+      for (int e = 0; e < E; ++e) x[e] = to_f32(reinterpret_cast<const T*>(&v)[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = i + e < n ? to_f32(part[i + e]) : -INFINITY;
     }
-  } else {
-    for (int i = t; i < n; i += SMP_THREADS) part[i] = row[first + i], look(to_f32(part[i]) + 0.f, first + i);
-  }
-  for (int o = 16; o; o >>= 1) {
-    const float l = __shfl_xor_sync(0xffffffffu, top, o);
-    const int i = __shfl_xor_sync(0xffffffffu, at, o);
-    if (l > top || (l == top && i < at)) top = l, at = i;
-  }
-  if (lane == 0) s.warp_a[w] = __float_as_uint(top), s.warp_b[w] = (uint32_t)at;
-  for (int b = t; b < SMP_ZBINS; b += SMP_THREADS) s.count[b] = 0;
-  bad = __syncthreads_or(bad);
-  const auto better = [&](float l, int j) {
-    if (l > top || (l == top && j < at)) top = l, at = j;
   };
-  for (int i = 0; i < SMP_WARPS; ++i) better(__uint_as_float(s.warp_a[i]), (int)s.warp_b[i]);
-  if (blocks > 1) {
-    if (t == 0) s.top = top, s.at = at, s.bad = bad;
-    cluster.sync();
-    for (int i = 0; i < blocks; ++i) {
-      const SampleShared* o = cluster.map_shared_rank(&s, i);
-      better(o->top, o->at), bad |= o->bad != 0;
-    }
+
+  // 1. The largest logit; a NaN (which the maximum keeps) or +inf leaves no distribution.
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int i = t * E; i < n; i += SMP_THREADS * E) {
+    float x[E];
+    load(x, i);
+#pragma unroll
+    for (int e = 0; e < E; ++e) top = max_nan(top, x[e]);
   }
-  if (bad || top == -INFINITY || !(T_ > 0.f)) {
+  for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s.warp_a[w] = __float_as_uint(top);
+  for (int b = t; b < SMP_ZBINS; b += SMP_THREADS) s.count[b] = 0;
+  __syncthreads();
+  top = __uint_as_float(s.warp_a[lane % SMP_WARPS]);
+  for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (blocks > 1) {
+    if (t == 0) s.top = top;
+    cluster.sync();
+    for (int i = 0; i < blocks; ++i) top = max_nan(top, cluster.map_shared_rank(&s, i)->top);
+  }
+  top += 0.f;  // -0 and 0 are equal
+  const bool none = !(top < INFINITY) || top == -INFINITY;
+  if (none || !(T_ > 0.f)) {
+    // the first index of the largest
+    int at = a.vocab;
+    if (!none)
+      for (int i = t; i < n; i += SMP_THREADS)
+        if (to_f32(part[i]) == top) at = min(at, first + i);
+    at = __reduce_min_sync(0xffffffffu, at);
+    __syncthreads();
+    if (lane == 0) s.warp_b[w] = (uint32_t)at;
+    __syncthreads();
+    at = (int)__reduce_min_sync(0xffffffffu, s.warp_b[lane % SMP_WARPS]);
+    if (blocks > 1) {
+      if (t == 0) s.at = at;
+      cluster.sync();
+      if (me == 0)
+        for (int i = 0; i < blocks; ++i) at = min(at, cluster.map_shared_rank(&s, i)->at);
+      cluster.sync();  // nobody leaves while others read it
+    }
     if (t == 0 && me == 0) {
-      const bool none = bad || top == -INFINITY;
       a.token[r] = none ? -1 : at;
       if (a.prob) a.prob[r] = none ? 0.f : 1.f;
     }
-    if (blocks > 1) cluster.sync();  // nobody leaves while others read it
     return;
   }
   const SampleMass f(top, T_);
@@ -477,65 +581,88 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
   int bound = SMP_ZBINS - 1;
   if (by_k || by_p || by_m) {
     const bool sums = by_p && !by_k;
-    for (int i = t; i < n; i += SMP_THREADS) {
-      const float l = to_f32(part[i]) + 0.f;
-      const int b = f.bin(l);
-      if (b < SMP_ZBINS) {
-        atomicAdd(&s.count[b], 1u);
-        if (sums) total += f.fixed(l, b);
+    // what min-p drops is not counted, unless top-p needs the mass of all that top-k keeps
+    if (by_m && !(by_k && by_p)) bound = min(bound, (int)fmin(-log2(fmin((double)mp, 1.0)) * 32.0, (double)SMP_ZBINS) + 1);
+    float small = 0.f;  // masses below 1/16, by the hardware's exp2: errors of 2^-22 of them are far below the sum's own
+    const float reach = (bound + 1) * 0.03125f;
+#pragma unroll 2
+    for (int i = t * E; i < n; i += SMP_THREADS * E) {
+      float x[E];
+      load(x, i);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float z = f.z(x[e]);
+        if (z < reach) {
+          const int b = SampleMass::bin_of(z);
+          if (b <= bound) atomicAdd(&s.count[b], 1u);
+          if (sums && z < 4.f) total += f.fixed(x[e], b);
+        }
+        if (sums && !(z < fminf(4.f, reach))) small += exp2_approx(-fminf(z, 200.f));
       }
     }
-    if (sums) total = sample_sum(s, total);
+    if (sums) total = sample_sum(s, total + (unsigned long long)(small * 0x1p44f));
     __syncthreads();
-    uint32_t own[2] = {0, 0}, all[2] = {0, 0};  // counts of this thread's two bins
-    for (int j = 0; j < 2; ++j)
-      if (2 * t + j < SMP_ZBINS) all[j] = own[j] = s.count[2 * t + j];
+    // the counts of this thread's bins, in this block and in all
+    constexpr int PER = (SMP_ZBINS + SMP_THREADS * 4 - 1) / (SMP_THREADS * 4) * 4;
+    static_assert(PER == 4, "one vector of counts for each thread");
+    const bool have = PER * t < SMP_ZBINS;
+    uint4 own4 = have ? *reinterpret_cast<const uint4*>(&s.count[PER * t]) : make_uint4(0, 0, 0, 0), all4 = own4;
     if (blocks > 1) {
       if (t == 0) s.sum = total;
       cluster.sync();
-      total = 0;
-      all[0] = all[1] = 0;
-      for (int i = 0; i < blocks; ++i) {
-        const SampleShared* o = cluster.map_shared_rank(&s, i);
-        total += o->sum;
-        for (int j = 0; j < 2; ++j)
-          if (2 * t + j < SMP_ZBINS) all[j] += o->count[2 * t + j];
+      unsigned long long sums_[SMP_CLUSTER];
+      uint4 counts[SMP_CLUSTER];
+#pragma unroll
+      for (int i = 0; i < SMP_CLUSTER; ++i) {  // all in flight together
+        const SampleShared* o = cluster.map_shared_rank(&s, min(i, blocks - 1));
+        sums_[i] = o->sum;
+        counts[i] = have ? *reinterpret_cast<const uint4*>(&o->count[PER * t]) : make_uint4(0, 0, 0, 0);
       }
+      total = 0;
+      all4 = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < SMP_CLUSTER; ++i)
+        if (i < blocks)
+          total += sums_[i], all4.x += counts[i].x, all4.y += counts[i].y, all4.z += counts[i].z, all4.w += counts[i].w;
     }
-    // running counts, and the least mass they can have: a bin's every e is above 2^(-(bin + 1) / 32)
-    float low[2];
-    for (int j = 0; j < 2; ++j) low[j] = (float)all[j] * exp2f(-(2 * t + j + 1) * 0.03125f);
-    uint32_t c = all[0] + all[1];
-    float m = low[0] + low[1];
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t pc = __shfl_up_sync(0xffffffffu, c, o);
-      const float pm = __shfl_up_sync(0xffffffffu, m, o);
-      if (lane >= o) c += pc, m += pm;
-    }
-    __syncthreads();
-    if (lane == 31) s.warp_a[w] = c, s.warp_d[w] = m;
-    if (t == 0) s.found_bin = SMP_ZBINS - 1;
-    __syncthreads();
-    for (int i = 0; i < w; ++i) c += s.warp_a[i], m += (float)s.warp_d[i];
+    const uint32_t own[PER] = {own4.x, own4.y, own4.z, own4.w}, all[PER] = {all4.x, all4.y, all4.z, all4.w};
     if (by_k || by_p) {
+      // running counts, and the least mass they can have: a bin's every e is above 2^(-(bin + 1) / 32)
+      float low[PER], m = 0.f;
+      uint32_t c = 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) low[j] = (float)all[j] * exp2_approx(-(PER * t + j + 1) * 0.03125f), c += all[j], m += low[j];
+      const uint32_t c1 = c;
+      const float m1 = m;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t pc = __shfl_up_sync(0xffffffffu, c, o);
+        const float pm = __shfl_up_sync(0xffffffffu, m, o);
+        if (lane >= o) c += pc, m += pm;
+      }
+      __syncthreads();
+      if (lane == 31) s.warp_a[w] = c, s.warp_b[w] = __float_as_uint(m);
+      if (t == 0) s.found_bin = SMP_ZBINS - 1;
+      __syncthreads();
+      uint32_t c0 = lane < w ? s.warp_a[lane] : 0u;
+      float m0 = lane < w ? __uint_as_float(s.warp_b[lane]) : 0.f;
+      for (int o = 16; o; o >>= 1) c0 += __shfl_xor_sync(0xffffffffu, c0, o), m0 += __shfl_xor_sync(0xffffffffu, m0, o);
+      c += c0 - c1, m += m0 - m1;  // before this thread's bins
       const double goal = (double)p * (double)total * pow2(-44) * 1.00001;  // beyond the rounding of `low`
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t upto_c = j ? c : c - all[1];
-        const float upto_m = j ? m : m - low[1];
-        if (2 * t + j < SMP_ZBINS && (by_k ? upto_c >= (uint32_t)k : upto_m >= goal)) {
-          atomicMin(&s.found_bin, 2 * t + j);
+      for (int j = 0; j < PER; ++j) {
+        c += all[j], m += low[j];
+        if (have && (by_k ? c >= (uint32_t)k : m >= goal)) {
+          atomicMin(&s.found_bin, PER * t + j);
           break;
         }
       }
       __syncthreads();
-      bound = s.found_bin;
+      bound = min(bound, s.found_bin);
     }
-    // what min-p drops is not listed, unless top-p needs the mass of all that top-k keeps
-    if (by_m && !(by_k && by_p)) bound = min(bound, (int)fmin(-log2(fmin((double)mp, 1.0)) * 32.0, (double)SMP_ZBINS) + 1);
     unsigned long long both = 0;  // listed elements: of all blocks, of this one
-    for (int j = 0; j < 2; ++j)
-      if (2 * t + j <= bound) both += ((unsigned long long)all[j] << 32) + own[j];
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (PER * t + j <= bound) both += ((unsigned long long)all[j] << 32) + own[j];
     both = sample_sum(s, both);
     listed = (uint32_t)(both >> 32), mine = (uint32_t)both;
     list = listed <= SMP_LIST;
@@ -549,35 +676,67 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
   // 3. The list, in order, in the first block; each warp has a run of the indexes.
   if (list) {
     SampleShared* to = blocks > 1 ? cluster.map_shared_rank(&s, 0) : &s;
-    const int share = ((n + SMP_WARPS - 1) / SMP_WARPS + 31) / 32 * 32, i0 = min(n, w * share), i1 = min(n, i0 + share);
+    // the smallest key that is listed, 32 ways at a time: bins only grow as keys fall
+    if (w == 0) {
+      uint32_t low = 0, size = logit_key(top);  // low + size is listed
+      while (size) {
+        const uint32_t step = size / 32 + 1, probe = (uint32_t)min((unsigned long long)size, (unsigned long long)step * lane);
+        const uint32_t in = __ballot_sync(0xffffffffu, f.bin(key_logit(low + probe)) <= bound);
+        const uint32_t j = in ? __ffs(in) - 1 : 32;  // the first probe that is listed
+        const unsigned long long from = j ? (unsigned long long)step * (j - 1) + 1 : 0, upto = j < 32 ? (unsigned long long)step * j : size;
+        low += (uint32_t)from, size = j ? (uint32_t)(min(upto, (unsigned long long)size) - from) : 0;
+      }
+      if (lane == 0) s.key_lo = low;
+    }
+    __syncthreads();
+    const float least_in = key_logit(s.key_lo);
+    const int share = ((n + SMP_WARPS - 1) / SMP_WARPS + E - 1) / E * E, i0 = min(n, w * share), i1 = min(n, i0 + share);
     uint32_t c = 0;
-    for (int i = i0 + lane; i < i1; i += 32) c += f.bin(to_f32(part[i]) + 0.f) <= bound;
+#pragma unroll 2
+    for (int i = i0 + lane * E; i < i1; i += 32 * E) {
+      float x[E];
+      load(x, i);
+#pragma unroll
+      for (int e = 0; e < E; ++e) c += x[e] >= least_in;
+    }
     c = __reduce_add_sync(0xffffffffu, c);
     __syncthreads();
     if (lane == 0) s.warp_a[w] = c;
     __syncthreads();
-    uint32_t at_ = before;
-    for (int i = 0; i < w; ++i) at_ += s.warp_a[i];
+    uint32_t slot = before + __reduce_add_sync(0xffffffffu, lane < w ? s.warp_a[lane] : 0u);
     if (c)
-      for (int j = i0; j < i1; j += 32) {
-        const int i = j + lane;
-        const float l = i < i1 ? to_f32(part[i]) + 0.f : -INFINITY;
-        const bool in = i < i1 && f.bin(l) <= bound;
-        const uint32_t ins = __ballot_sync(0xffffffffu, in);
-        if (in) {
-          const uint32_t slot = at_ + __popc(ins & ((1u << lane) - 1));
-          to->value[slot] = l, to->index[slot] = first + i;
+#pragma unroll 2
+      for (int j = i0; j < i1; j += 32 * E) {
+        const int i = j + lane * E;
+        float x[E];
+        uint32_t in = 0;
+        if (i < i1) {
+          load(x, i);
+#pragma unroll
+          for (int e = 0; e < E; ++e) in |= (uint32_t)(x[e] >= least_in) << e;
         }
-        at_ += __popc(ins);
+        if (!__any_sync(0xffffffffu, in)) continue;
+        uint32_t upto = __popc(in);
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += u;
+        }
+        uint32_t at = slot + upto - __popc(in);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (in >> e & 1) to->value[at] = x[e] + 0.f, to->index[at] = first + i + e, ++at;
+        slot += __shfl_sync(0xffffffffu, upto, 31);
       }
   }
   if (blocks > 1) cluster.sync();
   if (me) return;
   __syncthreads();
-  if (list)
+  if (list && listed <= SMP_THREADS)
+    sample_choose_sorted(s, a, r, f, (int)listed, k, p, least, total);
+  else if (list)
     sample_choose<T>(s, a, r, f, SampleItems<T>{s.value, nullptr, (int)listed}, s.index, k, p, least, total);
   else
-    sample_choose<T>(s, a, r, f, SampleItems<T>{nullptr, blocks > 1 ? row : part, a.vocab}, nullptr, k, p, least, total);
+    sample_choose<T>(s, a, r, f, SampleItems<T>{nullptr, row, a.vocab}, nullptr, k, p, least, total);
 }
 
 }  // namespace s1c
