@@ -10,6 +10,28 @@ namespace s1c {
 template <typename T>
 S1C_DEV float bits_f32(uint16_t v) { return to_f32(*reinterpret_cast<T*>(&v)); }
 
+// Two values in one word, the first in the low half, each rounded once.
+template <typename T>
+S1C_DEV uint32_t pack2(float lo, float hi);
+template <>
+S1C_DEV uint32_t pack2<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
+template <>
+S1C_DEV uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+
+// The larger of two; NaN where one is.
+S1C_DEV float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
+// 16 bytes that are read once.
+S1C_DEV uint4 ld_once(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // D += A B, f16 in, fp32 sums: a 16 x 16 (row), b 16 x 8 (column).
 S1C_DEV void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(

@@ -223,11 +223,12 @@ s1c_status s1c_cache_read(const s1c_cache* cache, int32_t dtype, void* d_k, int6
     check_half(dtype);
     CacheRows r = check_rows(c, d_k, k_stride, d_v, v_stride, d_cu, d_start, d_pages, max_pages, n, max_rows);
     if (n == 0 || max_rows == 0) return;
-    const int64_t units = ((int64_t)max_rows * c.heads * (c.dim / 16) + 255) / 256;
-    need(n * units <= INT_MAX, "n * max_rows * kv_heads is too large for one call");
+    const int rows = 4 * 256 / (c.dim / 16);  // of a block
+    const int64_t units = ((int64_t)max_rows + rows - 1) / rows;
+    need(n * units <= INT_MAX, "n * max_rows is too large for one call");
     r.units = (int)units;
     OnDeviceOf dev(d_k);
-    const dim3 grid((unsigned)(n * units), 2);
+    const dim3 grid((unsigned)(n * units), (unsigned)c.heads, 2);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == S1C_DT_F16)
       cache_read_kernel<__half><<<grid, 256, 0, st>>>(c, r);

@@ -52,13 +52,6 @@ S1C_DEV uint32_t logit_key(float l) {
 }
 S1C_DEV float key_logit(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// The larger of two; NaN where one is.
-S1C_DEV float max_nan(float a, float b) {
-  float m;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
-  return m;
-}
-
 S1C_DEV double pow2(int e) { return __hiloint2double((1023 + e) << 20, 0); }
 
 // exp as an integer: the bin of z and m with e = m * 2^(n - 24), n from the bin. The bin comes from the rounded product (it
