@@ -95,14 +95,12 @@ __global__ void __launch_bounds__(128) cache_write_kernel(const CacheView c, con
   int8_t* dst = c.codes[kv] + slot * c.page * c.dim;
   float* scale = c.scales[kv] + slot;
 
-  const auto vec = [&](int i) {
-    const int e = threadIdx.x + i * 128;
-    return ld_once(src + (e >> vshift) * r.stride[kv] + (e & ((1 << vshift) - 1)) * 8);
-  };
   uint4 v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (threadIdx.x + i * 128 < vecs) v[i] = vec(i);
+  for (int i = 0; i < 8; ++i) {
+    const int e = threadIdx.x + i * 128;
+    if (e < vecs) v[i] = ld_once(src + (e >> vshift) * r.stride[kv] + (e & ((1 << vshift) - 1)) * 8);
+  }
   const float had = old ? *scale : 0.f;
   float top = 0.f;
 #pragma unroll
@@ -115,13 +113,14 @@ __global__ void __launch_bounds__(128) cache_write_kernel(const CacheView c, con
     }
   if (!(top < INFINITY)) {  // rare: the largest of the finite ones
     top = 0.f;
-#pragma unroll 1
-    for (int i = 0; threadIdx.x + i * 128 < vecs; ++i) {
-      float x[8];
-      unpack8<T>(vec(i), x);
-      for (int j = 0; j < 8; ++j)
-        if (fabsf(x[j]) < INFINITY) top = fmaxf(top, fabsf(x[j]));
-    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (threadIdx.x + i * 128 < vecs) {
+        float x[8];
+        unpack8<T>(v[i], x);
+        for (int j = 0; j < 8; ++j)
+          if (fabsf(x[j]) < INFINITY) top = fmaxf(top, fabsf(x[j]));
+      }
   }
   __shared__ float tops[4];
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -132,38 +131,29 @@ __global__ void __launch_bounds__(128) cache_write_kernel(const CacheView c, con
   if (threadIdx.x == 0) *scale = s;
   const float inv = 1.f / s;
   const bool fast = s >= 0x1p-100f;
-  uint32_t again = 0;  // vectors that need the exact way, which is kept out of the unrolled code
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int e = threadIdx.x + i * 128;
     if (e < vecs) {
       float x[8];
       unpack8<T>(v[i], x);
-      uint32_t q[2];
-      if (!(quantise_fast(x, inv, q) && fast)) again |= 1u << i;
+      uint32_t q[2] = {0, 0};
+      if (!(fast && quantise_fast(x, inv, q))) {
+        q[0] = q[1] = 0;
+        for (int j = 0; j < 8; ++j) {
+          int n = 0;
+          if (fabsf(x[j]) < INFINITY)
+            n = fast ? quantise(x[j], s, inv) : s > 0.f ? (int)fmin(fmax(rint((double)x[j] / s), -127.0), 127.0) : 0;
+          else if (x[j] == x[j])
+            n = x[j] > 0.f ? 127 : -127;
+          q[j / 4] |= (uint32_t)(n & 255) << (8 * (j % 4));
+        }
+      }
       *reinterpret_cast<uint2*>(dst + (old * c.dim + e * 8)) = make_uint2(q[0], q[1]);
     }
   }
-#pragma unroll 1
-  for (; again; again &= again - 1) {
-    const int i = __ffs(again) - 1;
-    float x[8];
-    unpack8<T>(vec(i), x);
-    uint32_t q[2] = {0, 0};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      int n = 0;
-      if (fabsf(x[j]) < INFINITY)
-        n = fast ? quantise(x[j], s, inv) : s > 0.f ? (int)fmin(fmax(rint((double)x[j] / s), -127.0), 127.0) : 0;
-      else if (x[j] == x[j])
-        n = x[j] > 0.f ? 127 : -127;
-      q[j / 4] |= (uint32_t)(n & 255) << (8 * (j % 4));
-    }
-    *reinterpret_cast<uint2*>(dst + (old * c.dim + (threadIdx.x + i * 128) * 8)) = make_uint2(q[0], q[1]);
-  }
   if (old && s > had) {
     const float by = had * inv;
-#pragma unroll 1
     for (int e = threadIdx.x; e < old << vshift; e += 128) {
       uint2* at8 = reinterpret_cast<uint2*>(dst + e * 8);
       const uint2 was = *at8;
@@ -171,7 +161,7 @@ __global__ void __launch_bounds__(128) cache_write_kernel(const CacheView c, con
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = (float)(int8_t)((j < 4 ? was.x : was.y) >> (8 * (j % 4)));
       uint32_t q[2];
-      if (!(quantise_fast(x, by, q) && fast)) {
+      if (!(fast && quantise_fast(x, by, q))) {
         q[0] = q[1] = 0;
         for (int j = 0; j < 8; ++j) q[j / 4] |= (uint32_t)((int)rint((double)x[j] * had / s) & 255) << (8 * (j % 4));
       }
@@ -181,42 +171,44 @@ __global__ void __launch_bounds__(128) cache_write_kernel(const CacheView c, con
 }
 
 // Rows read back: value = code * scale, rounded once. A block has 128 rows (of 64 values: 256) of one head, a
-// thread 8 neighbouring values (8 B of codes, 16 B of output, so that a warp's accesses leave no gaps) of eight of them; rows on
-// pages outside the cache are written as 0. A byte code becomes fp32 under the exponent of 2^23.
+// thread 16 values (16 B of codes, 32 B of output) of four of them; rows on pages outside the cache are written as 0.
+// A byte code becomes fp32 under the exponent of 2^23.
 template <typename T>
 __global__ void __launch_bounds__(256) cache_read_kernel(const CacheView c, const CacheRows r) {
   const int seq = blockIdx.x / r.units, h = blockIdx.y, kv = blockIdx.z;
   const int first = r.cu[seq], count = min(r.cu[seq + 1] - first, r.most), start = r.start[seq];
-  const int shift = 31 - __clz(c.page), vshift = c.dim == 128 ? 4 : 3;
-  const int d = (threadIdx.x & ((1 << vshift) - 1)) * 8, per = 256 >> vshift;
-  const int row0 = blockIdx.x % r.units * 8 * per + (threadIdx.x >> vshift);
-  uint2 q[8];
-  float s[8];
+  const int shift = 31 - __clz(c.page), vshift = c.dim == 128 ? 3 : 2;
+  const int d = (threadIdx.x & ((1 << vshift) - 1)) * 16, per = 256 >> vshift;
+  const int row0 = blockIdx.x % r.units * 4 * per + (threadIdx.x >> vshift);
+  uint4 q[4];
+  float s[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = row0 + i * per;
-    const int64_t pos = (int64_t)start + row;
-    q[i] = make_uint2(0, 0), s[i] = 0.f;
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = row0 + i * per, pos = start + row;
+    q[i] = make_uint4(0, 0, 0, 0), s[i] = 0.f;
     if (row >= count || pos < 0) continue;
     const int page = cache_page(r.table, r.max_pages, seq, pos >> shift, c.num_pages);
     if (page < 0) continue;
     const int64_t slot = (int64_t)page * c.heads + h;
-    q[i] = __ldg(reinterpret_cast<const uint2*>(c.codes[kv] + ((slot << shift) + (pos & (c.page - 1))) * c.dim + d));
+    q[i] = ld_once(c.codes[kv] + ((slot << shift) + (pos & (c.page - 1))) * c.dim + d);
     s[i] = c.scales[kv][slot];
   }
-  T* dst = static_cast<T*>(r.rows[kv]) + (first + (int64_t)row0) * r.stride[kv] + h * c.dim + d;
 #pragma unroll
-  for (int i = 0; i < 8; ++i, dst += per * r.stride[kv]) {
-    if (row0 + i * per >= count) continue;
-    uint32_t out[4];
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = row0 + i * per;
+    if (row >= count) continue;
+    const uint32_t in[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+    uint32_t out[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = (j < 2 ? q[i].x : q[i].y) ^ 0x80808080u;
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t w = in[j / 2] ^ 0x80808080u;
       const float lo = __uint_as_float(__byte_perm(w, 0x4b000000u, j % 2 ? 0x7442 : 0x7440)) - 8388736.f;
       const float hi = __uint_as_float(__byte_perm(w, 0x4b000000u, j % 2 ? 0x7443 : 0x7441)) - 8388736.f;
       out[j] = pack2<T>(lo * s[i], hi * s[i]);
     }
-    *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(r.rows[kv]) + (first + row) * r.stride[kv] + h * c.dim + d);
+    dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
+    dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
   }
 }
 

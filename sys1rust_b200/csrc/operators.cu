@@ -223,7 +223,7 @@ s1c_status s1c_cache_read(const s1c_cache* cache, int32_t dtype, void* d_k, int6
     check_half(dtype);
     CacheRows r = check_rows(c, d_k, k_stride, d_v, v_stride, d_cu, d_start, d_pages, max_pages, n, max_rows);
     if (n == 0 || max_rows == 0) return;
-    const int rows = 8 * 256 / (c.dim / 8);  // of a block
+    const int rows = 4 * 256 / (c.dim / 16);  // of a block
     const int64_t units = ((int64_t)max_rows + rows - 1) / rows;
     need(n * units <= INT_MAX, "n * max_rows is too large for one call");
     r.units = (int)units;
