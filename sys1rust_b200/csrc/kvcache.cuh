@@ -95,12 +95,14 @@ __global__ void __launch_bounds__(128) cache_write_kernel(const CacheView c, con
   int8_t* dst = c.codes[kv] + slot * c.page * c.dim;
   float* scale = c.scales[kv] + slot;
 
+  const auto vec = [&](int i) {
+    const int e = threadIdx.x + i * 128;
+    return ld_once(src + (e >> vshift) * r.stride[kv] + (e & ((1 << vshift) - 1)) * 8);
+  };
   uint4 v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int e = threadIdx.x + i * 128;
-    if (e < vecs) v[i] = ld_once(src + (e >> vshift) * r.stride[kv] + (e & ((1 << vshift) - 1)) * 8);
-  }
+  for (int i = 0; i < 8; ++i)
+    if (threadIdx.x + i * 128 < vecs) v[i] = vec(i);
   const float had = old ? *scale : 0.f;
   float top = 0.f;
 #pragma unroll
@@ -113,14 +115,13 @@ __global__ void __launch_bounds__(128) cache_write_kernel(const CacheView c, con
     }
   if (!(top < INFINITY)) {  // rare: the largest of the finite ones
     top = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (threadIdx.x + i * 128 < vecs) {
-        float x[8];
-        unpack8<T>(v[i], x);
-        for (int j = 0; j < 8; ++j)
-          if (fabsf(x[j]) < INFINITY) top = fmaxf(top, fabsf(x[j]));
-      }
+#pragma unroll 1
+    for (int i = 0; threadIdx.x + i * 128 < vecs; ++i) {
+      float x[8];
+      unpack8<T>(vec(i), x);
+      for (int j = 0; j < 8; ++j)
+        if (fabsf(x[j]) < INFINITY) top = fmaxf(top, fabsf(x[j]));
+    }
   }
   __shared__ float tops[4];
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -131,29 +132,38 @@ __global__ void __launch_bounds__(128) cache_write_kernel(const CacheView c, con
   if (threadIdx.x == 0) *scale = s;
   const float inv = 1.f / s;
   const bool fast = s >= 0x1p-100f;
+  uint32_t again = 0;  // vectors that need the exact way, which is kept out of the unrolled code
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int e = threadIdx.x + i * 128;
     if (e < vecs) {
       float x[8];
       unpack8<T>(v[i], x);
-      uint32_t q[2] = {0, 0};
-      if (!(fast && quantise_fast(x, inv, q))) {
-        q[0] = q[1] = 0;
-        for (int j = 0; j < 8; ++j) {
-          int n = 0;
-          if (fabsf(x[j]) < INFINITY)
-            n = fast ? quantise(x[j], s, inv) : s > 0.f ? (int)fmin(fmax(rint((double)x[j] / s), -127.0), 127.0) : 0;
-          else if (x[j] == x[j])
-            n = x[j] > 0.f ? 127 : -127;
-          q[j / 4] |= (uint32_t)(n & 255) << (8 * (j % 4));
-        }
-      }
+      uint32_t q[2];
+      if (!(quantise_fast(x, inv, q) && fast)) again |= 1u << i;
       *reinterpret_cast<uint2*>(dst + (old * c.dim + e * 8)) = make_uint2(q[0], q[1]);
     }
   }
+#pragma unroll 1
+  for (; again; again &= again - 1) {
+    const int i = __ffs(again) - 1;
+    float x[8];
+    unpack8<T>(vec(i), x);
+    uint32_t q[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      int n = 0;
+      if (fabsf(x[j]) < INFINITY)
+        n = fast ? quantise(x[j], s, inv) : s > 0.f ? (int)fmin(fmax(rint((double)x[j] / s), -127.0), 127.0) : 0;
+      else if (x[j] == x[j])
+        n = x[j] > 0.f ? 127 : -127;
+      q[j / 4] |= (uint32_t)(n & 255) << (8 * (j % 4));
+    }
+    *reinterpret_cast<uint2*>(dst + (old * c.dim + (threadIdx.x + i * 128) * 8)) = make_uint2(q[0], q[1]);
+  }
   if (old && s > had) {
     const float by = had * inv;
+#pragma unroll 1
     for (int e = threadIdx.x; e < old << vshift; e += 128) {
       uint2* at8 = reinterpret_cast<uint2*>(dst + e * 8);
       const uint2 was = *at8;
@@ -161,7 +171,7 @@ __global__ void __launch_bounds__(128) cache_write_kernel(const CacheView c, con
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = (float)(int8_t)((j < 4 ? was.x : was.y) >> (8 * (j % 4)));
       uint32_t q[2];
-      if (!(fast && quantise_fast(x, by, q))) {
+      if (!(quantise_fast(x, by, q) && fast)) {
         q[0] = q[1] = 0;
         for (int j = 0; j < 8; ++j) q[j / 4] |= (uint32_t)((int)rint((double)x[j] * had / s) & 255) << (8 * (j % 4));
       }
@@ -180,6 +190,7 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheView c, cons
   const int shift = 31 - __clz(c.page), vshift = c.dim == 128 ? 3 : 2;
   const int d = (threadIdx.x & ((1 << vshift) - 1)) * 16, per = 256 >> vshift;
   const int row0 = blockIdx.x % r.units * 4 * per + (threadIdx.x >> vshift);
+  const bool whole = reinterpret_cast<uintptr_t>(r.rows[kv]) % 32 == 0 && r.stride[kv] % 16 == 0;
   uint4 q[4];
   float s[4];
 #pragma unroll
@@ -207,8 +218,12 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheView c, cons
       out[j] = pack2<T>(lo * s[i], hi * s[i]);
     }
     uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(r.rows[kv]) + (first + row) * r.stride[kv] + h * c.dim + d);
-    dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
-    dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+    if (whole) {
+      st_32(dst, out);
+    } else {
+      dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
+      dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+    }
   }
 }
 

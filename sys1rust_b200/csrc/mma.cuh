@@ -32,6 +32,13 @@ S1C_DEV uint4 ld_once(const void* p) {
   return v;
 }
 
+// 32 bytes at a 32-byte boundary, in one access: a warp's stores fill whole sectors.
+S1C_DEV void st_32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // D += A B, f16 in, fp32 sums: a 16 x 16 (row), b 16 x 8 (column).
 S1C_DEV void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm(
