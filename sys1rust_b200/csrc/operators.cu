@@ -97,20 +97,23 @@ CacheRows check_rows(const CacheView& c, const void* k, int64_t k_stride, const 
   return r;
 }
 
-// How an attention call is laid out: rows of a block (16, or 64 shared between warps), keys of a block.
+// How an attention call is laid out: blocks of 16 rows, or of many that share the keys' conversion; keys of a block.
 struct AttnPlan {
-  bool share;
+  bool prompt;
   int tiles, chunk, chunks;
 };
 AttnPlan plan_attention(const CacheView& c, int heads, int n, int max_q, int max_kv) {
   const int64_t rows = (int64_t)max_q * (heads / c.heads);
   AttnPlan p;
-  p.share = rows > 32;
-  p.tiles = (int)((rows + (p.share ? 63 : 15)) / (p.share ? 64 : 16));
+  p.prompt = rows > 32;
+  const int per = p.prompt ? 16 * CATP_WARPS : 16;
+  p.tiles = (int)((rows + per - 1) / per);
   const int64_t units = (int64_t)n * c.heads * p.tiles;
-  const int64_t most = std::min<int64_t>(p.share ? 4096 : 2048, (int64_t)CATT_PAGES * c.page - 128);
-  const int64_t want = (units * max_kv + 1183) / 1184;  // four rounds of two blocks on 148 SMs
+  // few rows: four rounds of two blocks on 148 SMs; many: one round, since their joining costs more
+  const int64_t want = (units * max_kv + (p.prompt ? 295 : 1183)) / (p.prompt ? 296 : 1184);
+  const int64_t most = p.prompt ? (int64_t)CATP_PAGES * c.page - 128 : std::min<int64_t>(2048, (int64_t)CATT_PAGES * c.page);
   p.chunk = (int)std::max<int64_t>(128, std::min(most, (want + 127) / 128 * 128));
+  if (p.prompt && units >= 148 && max_kv <= most) p.chunk = (int)most;
   p.chunks = (int)std::max<int64_t>(1, ((int64_t)max_kv + p.chunk - 1) / p.chunk);
   return p;
 }
@@ -118,29 +121,31 @@ size_t attention_workspace(const AttnPlan& p, const CacheView& c, int heads, int
   return p.chunks == 1 ? 0 : (size_t)n * max_q * heads * p.chunks * (c.dim + 1) * sizeof(float);
 }
 
-template <typename T, int D, bool SHARE>
-void launch_attention(const CacheView& c, const CacheAttnArgs& a, int dev, cudaStream_t st) {
-  constexpr auto KERNEL = cache_attention_kernel<T, D, SHARE>;
+template <typename T, int D>
+void launch_attention(const CacheView& c, const CacheAttnArgs& a, bool prompt, int dev, cudaStream_t st) {
   const uint64_t rows = (uint64_t)c.num_pages * c.heads * c.page;
   const uint32_t box = std::min(c.page, CATT_TK);
   const CUtensorMap k = byte_map(c.codes[0], D, rows, D, D, box), v = byte_map(c.codes[1], D, rows, D, D, box);
-  allow_smem<KERNEL>(dev);
-  KERNEL<<<dim3((unsigned)(a.n * c.heads * a.tiles), a.chunks), CATT_WARPS * 32, sizeof(CacheAttnSmem<D, SHARE>) + 1024, st>>>(k, v, c, a);
+  const dim3 grid((unsigned)(a.n * c.heads * a.tiles), a.chunks);
+  if (prompt) {
+    allow_smem<cache_prompt_kernel<T, D>>(dev);
+    cache_prompt_kernel<T, D><<<grid, CATP_WARPS * 32, sizeof(CachePromptSmem<D>) + 1024, st>>>(k, v, c, a);
+  } else {
+    allow_smem<cache_attention_kernel<T, D>>(dev);
+    cache_attention_kernel<T, D><<<grid, CATT_WARPS * 32, sizeof(CacheAttnSmem<D>) + 1024, st>>>(k, v, c, a);
+  }
   CK(cudaGetLastError());
   if (a.chunks > 1) {
-    const unsigned rows_ = (unsigned)((int64_t)a.n * a.max_q * a.heads);
+    const unsigned items = (unsigned)((int64_t)a.n * a.max_q * a.heads);
     if (a.chunks > 16)
-      launch_after(cache_attention_join_kernel<T, D, 16>, rows_, 512, st, a);
+      launch_after(cache_attention_join_kernel<T, D, 16>, items, 512, st, a);
     else
-      launch_after(cache_attention_join_kernel<T, D, 4>, rows_, 128, st, a);
+      launch_after(cache_attention_join_kernel<T, D, 4>, items, 128, st, a);
   }
 }
 template <typename T>
-void launch_attention(const CacheView& c, const CacheAttnArgs& a, bool share, int dev, cudaStream_t st) {
-  if (c.dim == 64)
-    share ? launch_attention<T, 64, true>(c, a, dev, st) : launch_attention<T, 64, false>(c, a, dev, st);
-  else
-    share ? launch_attention<T, 128, true>(c, a, dev, st) : launch_attention<T, 128, false>(c, a, dev, st);
+void launch_attention(const CacheView& c, const CacheAttnArgs& a, bool prompt, int dev, cudaStream_t st) {
+  c.dim == 64 ? launch_attention<T, 64>(c, a, prompt, dev, st) : launch_attention<T, 128>(c, a, prompt, dev, st);
 }
 
 // A row is shared by a cluster of up to eight blocks, as long as there are SMs for them and each keeps a
@@ -277,9 +282,9 @@ s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, const void
     a.part_lse = a.part + (size_t)n * max_q * heads * p.chunks * c.dim;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == S1C_DT_F16)
-      launch_attention<__half>(c, a, p.share, dev.device, st);
+      launch_attention<__half>(c, a, p.prompt, dev.device, st);
     else
-      launch_attention<__nv_bfloat16>(c, a, p.share, dev.device, st);
+      launch_attention<__nv_bfloat16>(c, a, p.prompt, dev.device, st);
     CK(cudaGetLastError());
   });
 }
