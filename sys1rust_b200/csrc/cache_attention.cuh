@@ -22,15 +22,19 @@
 //
 // Few query rows (bound by the cache's bytes): each warp has its own tiles of the block's keys and its own ring
 // of loads, so nothing waits inside the loop; the four warps' results are joined at the end. Long caches are split
-// over blocks, whose results a second kernel joins. Many rows (bound by the tensor cores and the conversion of the
-// codes): each warp has its own 16 rows, and a block converts a tile of keys once for all of them, to f16 in
-// shared memory, while it works on the tile before.
+// over blocks, whose results a second kernel joins.
+//
+// Many rows: a block of 128 rows on the 5th-generation tensor cores. Four warps convert a tile of 64 keys once for all
+// rows, to f16 in shared memory (whole codes, so no scale enters before the scores); one thread issues S = Q K^T into one of two
+// buffers of TMEM, a tile ahead, and O += P V; four warps have a row in each thread, and write the weights P over the scores
+// they come from, where the second product reads them as its first operand.
 #pragma once
 #include <cuda.h>
 #include <limits.h>
 
 #include "kvcache.cuh"
 #include "mma.cuh"
+#include "tmem.cuh"
 
 namespace s1c {
 
@@ -51,13 +55,17 @@ struct CacheAttnArgs {
   float* part_lse;   // [n * max_q * heads, chunks]: their log2 sums
 };
 
-constexpr int CATT_TK = 32;  // keys of a tile
+constexpr int CATT_TK = 32;   // keys of a tile: few rows
+constexpr int CATP_TK = 64;   // many rows
+constexpr int CATT_BOX = 32;  // rows of a TMA box at most
+
+constexpr int ATTN_BEYOND = 4;  // entries of the list of pages behind the last page
 
 // What a block works on: `rows` rows from row0 on of one sequence and key head, keys [lo, hi) in `tiles` tiles.
 struct AttnUnit {
   int h, seq, first, count, L, rows, row0, chunk, lo, hi, tiles, window, shift, G;
 };
-template <int ROWS>
+template <int ROWS, int TK>
 S1C_DEV bool attn_unit(const CacheView& c, const CacheAttnArgs& a, AttnUnit& u) {
   // later row tiles have more keys: they come first
   u.h = blockIdx.x % c.heads, u.seq = blockIdx.x / c.heads % a.n, u.G = a.heads / c.heads;
@@ -70,19 +78,19 @@ S1C_DEV bool attn_unit(const CacheView& c, const CacheAttnArgs& a, AttnUnit& u) 
   // keys that some row sees, in this chunk
   const int pos0 = u.L - u.count + u.row0 / u.G, pos1 = u.L - u.count + (min(u.row0 + ROWS, u.rows) - 1) / u.G;
   const int reach = (int)min((int64_t)a.max_pages * c.page, (int64_t)INT_MAX / 2);
-  u.lo = max(max(0, pos0 - u.window) / CATT_TK * CATT_TK, u.chunk * a.chunk);
+  u.lo = max(max(0, pos0 - u.window) / CATT_BOX * CATT_BOX, u.chunk * a.chunk);
   u.hi = (int)min((int64_t)min(pos1 + 1, reach), ((int64_t)u.chunk + 1) * a.chunk);
-  u.tiles = u.hi > u.lo ? (u.hi - u.lo + CATT_TK - 1) / CATT_TK : 0;
+  u.tiles = u.hi > u.lo ? (u.hi - u.lo + TK - 1) / TK : 0;
   return true;
 }
 
-// The chunk's pages: (key scale * 2^24, t, 2^-t, page), two more than there are, without a page (-1) 0, -inf, 0. Returns the
+// The chunk's pages: (key scale * 2^24, t, 2^-t, page), a few more than there are, without a page (-1) 0, -inf, 0. Returns the
 // largest value scale, which the outputs are multiplied by. All threads call.
 template <int WARPS>
 S1C_DEV float attn_pages(const CacheView& c, const CacheAttnArgs& a, const AttnUnit& u, float4* list, float* tops) {
-  const int tid = threadIdx.x, p0 = u.lo >> u.shift, pages = ((u.hi - 1) >> u.shift) - p0 + 1;
+  const int tid = threadIdx.x, p0 = u.lo >> u.shift, pages = ((u.hi - 1) >> u.shift) - p0 + 1;  // and more behind them than a tile has
   float top = 0.f;
-  for (int i = tid; i < pages + 2; i += WARPS * 32) {
+  for (int i = tid; i < pages + ATTN_BEYOND; i += WARPS * 32) {
     const int page = i < pages ? cache_page(a.table, a.max_pages, u.seq, p0 + i, c.num_pages) : -1;
     float ks = 0.f, vs = 0.f;
     if (page >= 0) {
@@ -97,7 +105,7 @@ S1C_DEV float attn_pages(const CacheView& c, const CacheAttnArgs& a, const AttnU
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < WARPS; ++i) top = fmaxf(top, tops[i]);
-  for (int i = tid; i < pages + 2; i += WARPS * 32) {
+  for (int i = tid; i < pages + ATTN_BEYOND; i += WARPS * 32) {
     float4 e = list[i];
     // scales below 2^-60 of the largest (and zero ones, whose codes are zero) count as that
     const float l2 = top > 0.f ? fmaxf(log2f(e.y / top), -60.f) : 0.f;
@@ -109,13 +117,13 @@ S1C_DEV float attn_pages(const CacheView& c, const CacheAttnArgs& a, const AttnU
   return top;
 }
 
-// TMA of one tile's keys and values to `dst`, by a whole warp: a lane for each page (one, or two of 16 rows). Pages outside
+// TMA of one tile's keys and values to `dst`, by a whole warp: a lane for each page or 32 rows of one. Pages outside
 // the cache are not read.
-template <int D>
+template <int D, int TK>
 S1C_DEV void attn_issue(const CacheView& c, const AttnUnit& u, const float4* list, const CUtensorMap& k_map, const CUtensorMap& v_map, int i,
                         uint8_t* dst, uint64_t* bar) {
-  const int lane = threadIdx.x % 32, per = min(c.page, CATT_TK), boxes = CATT_TK / per;
-  const int at = u.lo + i * CATT_TK + lane * per;
+  const int lane = threadIdx.x % 32, per = min(c.page, CATT_BOX), boxes = TK / per;
+  const int at = u.lo + i * TK + lane * per;
   const int page = lane < boxes && at < u.hi ? __float_as_int(list[(at >> u.shift) - (u.lo >> u.shift)].w) : -1;
   const int count = __popc(__ballot_sync(0xffffffffu, page >= 0));
   if (lane == 0) mbar_arrive_expect_tx(bar, count * 2 * per * D);
@@ -123,9 +131,15 @@ S1C_DEV void attn_issue(const CacheView& c, const AttnUnit& u, const float4* lis
   if (page >= 0) {
     const int y = (page * c.heads + u.h) * c.page + (at & (c.page - 1));
     tma_load_2d(dst + lane * per * D, &k_map, bar, 0, y);
-    tma_load_2d(dst + CATT_TK * D + lane * per * D, &v_map, bar, 0, y);
+    tma_load_2d(dst + TK * D + lane * per * D, &v_map, bar, 0, y);
   }
   __syncwarp();
+}
+
+// The power of two that brings a row's largest value to [2^14, 2^15); rows with an infinity or NaN keep theirs.
+S1C_DEV int attn_up(float top) {
+  const int ex = (int)((__float_as_uint(top) >> 23) & 255u) - 127;
+  return ex == 128 ? 0 : min(14 - ex, 100);
 }
 
 // One thread's part of two query rows, g and g + 8 of a tile from row `r0` on (rows past the last repeat it).
@@ -143,9 +157,9 @@ struct AttnRows {
       m[e] = -INFINITY, l[e] = 0.f;
     }
   }
-  // The rows as f16 operands. The columns 2 cq, 2 cq + 1 (and those 8 on) of operand i are dimensions 16 i + 4 cq .. + 3 (QUADS, the order
-  // of a lane's word of codes), or 16 i + 2 cq, + 1 (and 8 on).
-  template <typename T, int D, bool QUADS>
+  // The rows as f16 operands. The columns 2 cq, 2 cq + 1 (and those 8 on) of operand i are dimensions 16 i + 4 cq .. + 3, the order
+  // of a lane's word of codes.
+  template <typename T, int D>
   S1C_DEV void operands(const CacheAttnArgs& a, uint32_t (&qa)[D / 16][4]) {
     const int cq = threadIdx.x % 4;
 #pragma unroll
@@ -154,21 +168,14 @@ struct AttnRows {
       float f[D / 16][4], top = 0.f, sum = 0.f;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
-        uint32_t lo, hi;
-        if (QUADS) {
-          const uint2 v = *reinterpret_cast<const uint2*>(q + i * 16 + cq * 4);
-          lo = v.x, hi = v.y;
-        } else {
-          lo = *reinterpret_cast<const uint32_t*>(q + i * 16 + cq * 2), hi = *reinterpret_cast<const uint32_t*>(q + i * 16 + 8 + cq * 2);
-        }
-        f[i][0] = bits_f32<T>((uint16_t)lo), f[i][1] = bits_f32<T>((uint16_t)(lo >> 16));
-        f[i][2] = bits_f32<T>((uint16_t)hi), f[i][3] = bits_f32<T>((uint16_t)(hi >> 16));
+        const uint2 v = *reinterpret_cast<const uint2*>(q + i * 16 + cq * 4);
+        f[i][0] = bits_f32<T>((uint16_t)v.x), f[i][1] = bits_f32<T>((uint16_t)(v.x >> 16));
+        f[i][2] = bits_f32<T>((uint16_t)v.y), f[i][3] = bits_f32<T>((uint16_t)(v.y >> 16));
 #pragma unroll
         for (int j = 0; j < 4; ++j) top = max_nan(top, fabsf(f[i][j]));
       }
       for (int o = 1; o < 4; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // 2^up brings the largest value to [2^14, 2^15); rows with an infinity or NaN keep theirs
-      const int ex = (int)(__float_as_uint(top) >> 23) - 127, up = ex == 128 ? 0 : min(14 - ex, 100);
+      const int up = attn_up(top);
       const float by = __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
@@ -263,12 +270,13 @@ S1C_DEV void attn_put(const CacheAttnArgs& a, const AttnUnit& u, int64_t row, in
   if (a.chunks > 1) {
     const int64_t at = ((u.seq * (int64_t)a.max_q + (row - u.first)) * a.heads + head) * a.chunks + u.chunk;
 #pragma unroll
-    for (int i = 0; i < N; i += 2) *reinterpret_cast<float2*>(a.part + at * D + d + i) = make_float2(v[i] * by, v[i + 1] * by);
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<float4*>(a.part + at * D + d + i) = make_float4(v[i] * by, v[i + 1] * by, v[i + 2] * by, v[i + 3] * by);
     if (d == 0) a.part_lse[at] = log_sum;
   } else {
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + row * a.out_stride + head * D + d);
+    uint2* dst = reinterpret_cast<uint2*>(static_cast<T*>(a.out) + row * a.out_stride + head * D + d);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) dst[i / 2] = pack2<T>(v[i] * by, v[i + 1] * by);
+    for (int i = 0; i < N; i += 4) dst[i / 4] = make_uint2(pack2<T>(v[i] * by, v[i + 1] * by), pack2<T>(v[i + 2] * by, v[i + 3] * by));
     if (a.lse && d == 0) a.lse[row * a.heads + head] = log_sum * 0.69314718055994531f;
   }
 }
@@ -283,7 +291,7 @@ struct CacheAttnSmem {
   alignas(1024) uint8_t ring[CATT_WARPS][STAGES][TILE];
   uint4 q[D / 16][32];  // operands of the query rows
   uint64_t full[CATT_WARPS][STAGES];
-  float4 page[CATT_PAGES + 2];
+  float4 page[CATT_PAGES + ATTN_BEYOND];
   float top[CATT_WARPS];
   float row_m[CATT_WARPS][16], row_l[CATT_WARPS][16];
 };
@@ -299,7 +307,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, g = lane >> 2, cq = lane & 3;
   pdl_trigger();
   AttnUnit u;
-  if (!attn_unit<16>(c, a, u)) return;
+  if (!attn_unit<16, CATT_TK>(c, a, u)) return;
   float v_top = 0.f;
   if (u.tiles > 0) {
     if (tid < CATT_WARPS * S::STAGES) {
@@ -310,7 +318,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   }
   const auto issue = [&](int i) {
     const int slot = i / CATT_WARPS % S::STAGES;
-    attn_issue<D>(c, u, sm.page, k_map, v_map, i, sm.ring[w][slot], &sm.full[w][slot]);
+    attn_issue<D, CATT_TK>(c, u, sm.page, k_map, v_map, i, sm.ring[w][slot], &sm.full[w][slot]);
   };
   for (int s = 0; s < S::STAGES; ++s)
     if (w + s * CATT_WARPS < u.tiles) issue(w + s * CATT_WARPS);
@@ -319,7 +327,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   row.setup(u, u.row0);
   {
     uint32_t qa[QK][4];
-    row.operands<T, D, true>(a, qa);
+    row.operands<T, D>(a, qa);
     if (w == 0)
 #pragma unroll
       for (int i = 0; i < QK; ++i) sm.q[i][lane] = make_uint4(qa[i][0], qa[i][1], qa[i][2], qa[i][3]);
@@ -425,18 +433,23 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   }
 }
 
-// Many query rows.
-constexpr int CATP_WARPS = 8, CATP_STAGES = 2, CATP_PAGES = 256;
+// Many query rows: warps 0 to 3 softmax (thread = row = TMEM lane), 4 to 7 conversion, 8 products.
+constexpr int CATP_ROWS = 128, CATP_WARPS = 9, CATP_PAGES = 256;
+// TMEM columns: scores (then weights, f16 pairs, over the first 32 columns) of even tiles [0, 64), of odd tiles [64, 128); outputs from 128 on
+constexpr uint32_t CATP_TMEM = 256, CATP_TMEM_O = 128;
 
 template <int D>
 struct CachePromptSmem {
-  alignas(1024) uint8_t ring[CATP_STAGES][2 * CATT_TK * D];  // codes of keys and values
-  // two tiles as f16, keys (codes + 128) * 2^-24, values as codes; 16-byte pieces of a row XORed with the row
-  alignas(1024) uint8_t half[2][2][CATT_TK * D * 2];
-  uint4 q[CATP_WARPS][D / 16][32];
-  uint64_t full[CATP_STAGES];
-  float4 page[CATP_PAGES + 2];
+  // blocks of 64 dimensions, rows of 128 bytes, 16-byte pieces XORed with the row: the 128-byte swizzle of the products' operands
+  alignas(1024) uint8_t q[D / 64][CATP_ROWS * 128];
+  alignas(1024) uint8_t k[D / 64][CATP_TK * 128];
+  alignas(1024) uint8_t v[2][D / 64][CATP_TK * 128];
+  alignas(1024) uint8_t codes[2 * CATP_TK * D];  // one tile's keys and values as they are in the cache
+  float4 page[CATP_PAGES + ATTN_BEYOND];
   float top[CATP_WARPS];
+  uint64_t raw_full, raw_free, q_full, k_full, k_free, v_full[2], s_full[2], p_full[2], pv_done[2], o_full, drain;
+  uint32_t tmem;
+  int abort;
 };
 
 template <typename T, int D>
@@ -446,155 +459,242 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   using S = CachePromptSmem<D>;
   extern __shared__ uint8_t raw[];
   S& sm = *reinterpret_cast<S*>(raw + (1024 - smem_u32(raw) % 1024) % 1024);
-  constexpr int QK = D / 16, ROWS = 16 * CATP_WARPS;
-  const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, g = lane >> 2, cq = lane & 3;
+  const int tid = threadIdx.x, w = tid / 32, lane = tid % 32;
   pdl_trigger();
   AttnUnit u;
-  if (!attn_unit<ROWS>(c, a, u)) return;
-  float v_top = 0.f;
-  if (u.tiles > 0) {
-    if (tid < CATP_STAGES) {
-      mbar_init(&sm.full[tid], 1);
-      fence_barrier_init();
-    }
-    v_top = attn_pages<CATP_WARPS>(c, a, u, sm.page, sm.top);
+  if (!attn_unit<CATP_ROWS, CATP_TK>(c, a, u)) return;
+  // the softmax threads' rows; those past the last repeat it
+  const int r = min(u.row0 + tid % CATP_ROWS, u.rows - 1);
+  const int64_t at_row = u.first + r / u.G;
+  const int head = u.h * u.G + r % u.G, pos = u.L - u.count + r / u.G;
+  const bool real = w < 4 && u.row0 + tid < u.rows;
+  if (u.tiles == 0) {
+    const float zero[8] = {};
+    if (real)
+      for (int d = 0; d < D; d += 8) attn_put<T, D>(a, u, at_row, head, d, zero, 0.f, 0.f, 0.f);
+    return;
   }
-  const auto issue = [&](int i) {
-    attn_issue<D>(c, u, sm.page, k_map, v_map, i, sm.ring[i % CATP_STAGES], &sm.full[i % CATP_STAGES]);
-  };
-  if (w == 0)
-    for (int s = 0; s < CATP_STAGES; ++s)
-      if (s < u.tiles) issue(s);
-
-  AttnRows row;
-  row.setup(u, u.row0 + w * 16);
-  {
-    uint32_t qa[QK][4];
-    row.operands<T, D, false>(a, qa);
-#pragma unroll
-    for (int i = 0; i < QK; ++i) sm.q[w][i][lane] = make_uint4(qa[i][0], qa[i][1], qa[i][2], qa[i][3]);
-    __syncwarp();
+  if (tid == 0) {
+    mbar_init(&sm.raw_full, 1), mbar_init(&sm.raw_free, 4), mbar_init(&sm.q_full, 4), mbar_init(&sm.k_full, 4), mbar_init(&sm.k_free, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&sm.v_full[i], 4), mbar_init(&sm.s_full[i], 1), mbar_init(&sm.p_full[i], 4), mbar_init(&sm.pv_done[i], 1);
+    mbar_init(&sm.o_full, 1), mbar_init(&sm.drain, 1);
+    sm.abort = 0;
+    fence_barrier_init();
   }
-  const uint32_t q_at = smem_u32(&sm.q[w][0][lane]);
+  if (w == 8) {
+    tmem_alloc(&sm.tmem, CATP_TMEM);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  const float v_top = attn_pages<CATP_WARPS>(c, a, u, sm.page, sm.top);  // with barriers of the block
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  volatile int* abort = &sm.abort;
 
-  // conversion: 16 codes of a row at a time
-  constexpr int ITEMS = 2 * CATT_TK * (D / 16) / (CATP_WARPS * 32);
-  static_assert(ITEMS >= 1, "a thread converts at least 16 codes");
-  const auto item = [&](int x, int& which, int& r, int& piece) {
-    const int i = tid + x * CATP_WARPS * 32;
-    which = i / (CATT_TK * (D / 16)), r = i / (D / 16) % CATT_TK, piece = i % (D / 16);
-  };
-  uint4 codes[ITEMS];
-  const auto fetch = [&](int slot) {
+  if (w == 8) {
+    if (lane == 0) {
+      constexpr uint32_t idS = idesc_f16_f32(CATP_ROWS, CATP_TK, false), idO = idesc_f16_f32(CATP_ROWS, 64, true);
+      const auto scores = [&](int i) {
+        if (!mbar_wait(&sm.k_full, i & 1, nullptr, 0, abort)) return false;
+        tc_fence_after();
 #pragma unroll
-    for (int x = 0; x < ITEMS; ++x) {
-      int which, r, piece;
-      item(x, which, r, piece);
-      codes[x] = *reinterpret_cast<const uint4*>(sm.ring[slot] + (which * CATT_TK + r) * D + ((piece ^ (D == 128 ? r & 7 : r >> 1 & 3)) << 4));
+        for (int b = 0; b < D / 64; ++b)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16(tmem + 64 * (i & 1), sdesc_kmajor_sw128(smem_u32(sm.q[b]) + k * 32), sdesc_kmajor_sw128(smem_u32(sm.k[b]) + k * 32), idS,
+                      (b | k) ? 1u : 0u);
+        umma_commit(&sm.s_full[i & 1]);
+        umma_commit(&sm.k_free);
+        return true;
+      };
+      bool ok = mbar_wait(&sm.q_full, 0, nullptr, 0, abort) && scores(0) && (u.tiles < 2 || scores(1));
+      for (int i = 0; ok && i < u.tiles; ++i) {
+        const int b = i & 1;
+        ok = mbar_wait(&sm.p_full[b], i >> 1 & 1, nullptr, 0, abort) && mbar_wait(&sm.v_full[b], i >> 1 & 1, nullptr, 0, abort);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n)
+#pragma unroll
+          for (int k = 0; k < CATP_TK / 16; ++k)
+            umma_bf16_ts(tmem + CATP_TMEM_O + 64 * n, tmem + 64 * b + 8 * k, sdesc_mnmajor_sw128(smem_u32(sm.v[b][n]) + k * 2048), idO,
+                         (i | k) ? 1u : 0u);
+        umma_commit(&sm.pv_done[b]);
+        if (i == u.tiles - 1) umma_commit(&sm.o_full);
+        // scores two tiles on, over the weights that this product, issued before them, reads
+        if (i + 2 < u.tiles) ok = scores(i + 2);
+      }
+      umma_commit(&sm.drain);
+      mbar_wait(&sm.drain, 0, nullptr, 0, nullptr);
     }
-  };
-  const auto convert = [&](int buffer) {
+  } else if (w >= 4) {
+    // 16 codes at a time: 64 x D / 16 pieces of keys and as many of values over 128 threads
+    constexpr int ITEMS = CATP_TK * (D / 16) / 128;
+    const int t = tid - 128;
+    if (w == 4) attn_issue<D, CATP_TK>(c, u, sm.page, k_map, v_map, 0, sm.codes, &sm.raw_full);
+    for (int i = 0; i < u.tiles; ++i) {
+      if (!mbar_wait_warp(&sm.raw_full, i & 1, nullptr, 0, abort)) break;
+      uint4 codes[2][ITEMS];
 #pragma unroll
-    for (int x = 0; x < ITEMS; ++x) {
-      int which, r, piece;
-      item(x, which, r, piece);
-      const uint32_t in[4] = {codes[x].x, codes[x].y, codes[x].z, codes[x].w};
-      uint32_t out[8];
+      for (int x = 0; x < 2 * ITEMS; ++x) {
+        const int j = t + x % ITEMS * 128, row = j / (D / 16), piece = j % (D / 16);
+        codes[x / ITEMS][x % ITEMS] =
+            *reinterpret_cast<const uint4*>(sm.codes + (x / ITEMS * CATP_TK + row) * D + ((piece ^ (D == 128 ? row & 7 : row >> 1 & 3)) << 4));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.raw_free);
+      if (w == 4 && i + 1 < u.tiles) {  // the next tile may come when all codes are in registers
+        if (!mbar_wait_warp(&sm.raw_free, i & 1, nullptr, 0, abort)) break;
+        attn_issue<D, CATP_TK>(c, u, sm.page, k_map, v_map, i + 1, sm.codes, &sm.raw_full);
+      }
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        // the product that read this buffer last
+        if (which == 0 && i > 0 && !mbar_wait_warp(&sm.k_free, (i - 1) & 1, nullptr, 0, abort)) goto done;
+        if (which == 1 && i > 1 && !mbar_wait_warp(&sm.pv_done[i & 1], ((i >> 1) - 1) & 1, nullptr, 0, abort)) goto done;
+#pragma unroll
+        for (int x = 0; x < ITEMS; ++x) {
+          const int j = t + x * 128, row = j / (D / 16), piece = j % (D / 16);
+          const uint4 in4 = codes[which][x];
+          const uint32_t in[4] = {in4.x, in4.y, in4.z, in4.w};
+          uint32_t out[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t v = in[e] ^ 0x80808080u;
+            out[2 * e] = code_pair(__byte_perm(v, 0x64646464u, 0x4140)), out[2 * e + 1] = code_pair(__byte_perm(v, 0x64646464u, 0x4342));
+          }
+          uint8_t* dst = (which ? sm.v[i & 1][piece / 4] : sm.k[piece / 4]) + row * 128;
+          const int p0 = piece % 4 * 2;
+          *reinterpret_cast<uint4*>(dst + ((p0 ^ (row & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+          *reinterpret_cast<uint4*>(dst + (((p0 + 1) ^ (row & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(which ? &sm.v_full[i & 1] : &sm.k_full);
+      }
+    }
+  done:;
+  } else {
+    // the row as f16, in the order of the products' operand
+    float factor;
+    {
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at_row * a.q_stride + head * D);
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        float x[8];
+        unpack8<T>(q[i], x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(x[j]));
+      }
+      const int up = attn_up(top);
+      const float by = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll 4
+      for (int i = 0; i < D / 8; ++i) {
+        float x[8];
+        unpack8<T>(q[i], x);
+        *reinterpret_cast<uint4*>(sm.q[i / 8] + tid * 128 + ((i % 8 ^ (tid & 7)) << 4)) =
+            make_uint4(pack_f16x2(x[0] * by, x[1] * by), pack_f16x2(x[2] * by, x[3] * by), pack_f16x2(x[4] * by, x[5] * by),
+                       pack_f16x2(x[6] * by, x[7] * by));
+      }
+      factor = a.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23) * 0x1p-24f;  // the list's key scales have 2^24
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.q_full);
+    }
+    const uint32_t lanes = (uint32_t)(w * 32) << 16;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int i = 0; i < u.tiles; ++i) {
+      const int b = i & 1, key = u.lo + i * CATP_TK, pg = (key >> u.shift) - (u.lo >> u.shift), in = key & (c.page - 1);
+      // columns that this row sees: [from, upto)
+      const int upto = min(pos + 1, u.hi) - key, from = pos - u.window - key;
+      if (!mbar_wait_warp(&sm.s_full[b], i >> 1 & 1, nullptr, 0, abort)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      float s[64];
+      tmem_ld32x2(tmem + lanes + 64 * b, true, true, s);
+      const bool open = __all_sync(0xffffffffu, from <= 0 && upto >= CATP_TK);
+      float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, inv[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t v = in[j] ^ 0x80808080u;
-        if (which) {
-          out[2 * j] = code_pair(__byte_perm(v, 0x64646464u, 0x4140)), out[2 * j + 1] = code_pair(__byte_perm(v, 0x64646464u, 0x4342));
-        } else {
-          out[2 * j] = __byte_perm(v, 0, 0x4140), out[2 * j + 1] = __byte_perm(v, 0, 0x4342);
+        const float4 p = sm.page[pg + ((in + 16 * j) >> u.shift)];
+        const float f = factor * p.x;
+        inv[j] = p.z;
+#pragma unroll
+        for (int x = 16 * j; x < 16 * j + 16; ++x) s[x] = fmaf(s[x], f, p.y);
+      }
+      if (!open) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int x0 = min(max(from - 32 * half, 0), 32), x1 = min(max(upto - 32 * half, 0), 32);
+          const uint32_t see = (x1 >= 32 ? 0xffffffffu : (1u << x1) - 1u) & ~(x0 >= 32 ? 0xffffffffu : (1u << x0) - 1u);
+#pragma unroll
+          for (int x = 0; x < 32; ++x) s[32 * half + x] = (see & (1u << x)) ? s[32 * half + x] : -INFINITY;
         }
       }
-      uint8_t* dst = sm.half[buffer][which] + r * D * 2;
-      *reinterpret_cast<uint4*>(dst + (((2 * piece) ^ (r & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
-      *reinterpret_cast<uint4*>(dst + (((2 * piece + 1) ^ (r & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
+#pragma unroll
+      for (int x = 0; x < 64; ++x) part[x & 3] = fmaxf(part[x & 3], s[x]);
+      const float top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+      float keep = 1.f;
+      if (top > m + 1.25f) {
+        keep = m == -INFINITY ? 0.f : exp2f(m - top);
+        l *= keep;
+        m = top;
+      }
+      if (i > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
+        // the outputs so far, when the product before has completed
+        if (!mbar_wait_warp(&sm.pv_done[b ^ 1], (i - 1) >> 1 & 1, nullptr, 0, abort)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll 1
+        for (int x = 0; x < D; x += 16) {
+          float t[16];
+          tmem_ld16(tmem + lanes + CATP_TMEM_O + x, t);
+#pragma unroll
+          for (int y = 0; y < 16; ++y) t[y] *= keep;
+          tmem_st16(tmem + lanes + CATP_TMEM_O + x, t);
+        }
+      }
+      const float off = m == -INFINITY ? 0.f : 14.5f - m;
+      float pk[32];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float sum = 0.f;
+#pragma unroll
+        for (int x = 8 * j; x < 8 * j + 8; ++x) {
+          const float p0 = exp2_approx(s[2 * x] + off), p1 = exp2_approx(s[2 * x + 1] + off);
+          sum += p0 + p1;
+          pk[x] = __uint_as_float(pack_f16x2(p0, p1));
+        }
+        l = fmaf(sum, inv[j], l);
+      }
+      tmem_st32(tmem + lanes + 64 * b, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.p_full[b]);
     }
-  };
-  bool broken = false;
-  const auto arrived = [&](int i) {
-    if (!broken && !mbar_wait_warp(&sm.full[i % CATP_STAGES], i / CATP_STAGES & 1, nullptr, 0, nullptr)) broken = true;
-  };
-
-  // addresses for ldmatrix: matrices (keys 0-7, 8 columns), (keys 0-7, next 8), (keys 8-15, ..), (keys 8-15, ..) of the keys, and
-  // of the values (keys 0-7, dims), (keys 8-15, dims), and the next dims
-  const int mr = lane & 7, mi = lane >> 3;
-  const uint32_t k_at = smem_u32(sm.half[0][0]) + ((mi >> 1) * 8 + mr) * D * 2 + (((mi & 1) ^ mr) << 4);
-  const uint32_t v_at = smem_u32(sm.half[0][1]) + ((mi & 1) * 8 + mr) * D * 2 + (((mi >> 1) ^ mr) << 4);
-  constexpr int BUFFER = 2 * CATT_TK * D * 2;
-
-  float o[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-  const int last = __reduce_max_sync(0xffffffffu, row.pos[1]), from = __reduce_min_sync(0xffffffffu, row.pos[0]) - u.window;
-
-  if (u.tiles > 0) {
-    arrived(0);
-    fetch(0);
-    convert(0);
-    __syncthreads();
+    if (ok && mbar_wait_warp(&sm.o_full, 0, nullptr, 0, abort)) {
+      tc_fence_after();
+#pragma unroll 1
+      for (int d = 0; d < D; d += 32) {
+        float t[32];
+        tmem_ld32(tmem + lanes + CATP_TMEM_O + d, t);
+        if (real) attn_put<T, D>(a, u, at_row, head, d, t, v_top, l, m);
+      }
+    }
   }
-  for (int i = 0; i < u.tiles; ++i) {
-    const int key = u.lo + i * CATT_TK, b = i & 1;
-    // the codes of tile i have been converted: their slot is free
-    if (w == 0 && i + CATP_STAGES < u.tiles) issue(i + CATP_STAGES);
-    const bool more = i + 1 < u.tiles;
-    if (more) {
-      arrived(i + 1);
-      fetch((i + 1) % CATP_STAGES);
-    }
-    const bool mine = !broken && key <= last && key + CATT_TK > from;  // some row of this warp sees a key
-    float s[4][4];
-    if (mine) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[j][0] = s[j][1] = row.start[0], s[j][2] = s[j][3] = row.start[1];
-      static_for<QK>([&](auto DD) {
-        constexpr int d = decltype(DD)::value;
-        const uint4 qv = lds_v4<d * 512>(q_at);
-        const uint32_t qa[4] = {qv.x, qv.y, qv.z, qv.w};
-        const uint32_t at = (k_at ^ (d << 5)) + b * BUFFER;
-        uint32_t k0[4], k1[4];
-        ldmatrix<0>(at, k0);
-        ldmatrix<16 * D * 2>(at, k1);
-        mma_f16(s[0], qa, k0[0], k0[1]);
-        mma_f16(s[1], qa, k0[2], k0[3]);
-        mma_f16(s[2], qa, k1[0], k1[1]);
-        mma_f16(s[3], qa, k1[2], k1[3]);
-      });
-    }
-    if (more) convert(b ^ 1);
-    if (mine) {
-      row.weights(c, u, sm.page, key, 2 * cq, 2 * cq + 1, s, o);
-      uint32_t pa[2][4];
-      attn_pack(s, pa);
-      static_for<D / 16>([&](auto DD) {
-        constexpr int d = decltype(DD)::value;
-        const uint32_t at = (v_at ^ (d << 5)) + b * BUFFER;
-        uint32_t v0[4], v1[4];
-        ldmatrix_t<0>(at, v0);
-        ldmatrix_t<16 * D * 2>(at, v1);
-        mma_f16(o[2 * d], pa[0], v0[0], v0[1]);
-        mma_f16(o[2 * d + 1], pa[0], v0[2], v0[3]);
-        mma_f16(o[2 * d], pa[1], v1[0], v1[1]);
-        mma_f16(o[2 * d + 1], pa[1], v1[2], v1[3]);
-      });
-    }
-    __syncthreads();
-  }
-  row.finish();
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    if (u.row0 + w * 16 + g + 8 * e >= u.rows) continue;
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      const float v[2] = {o[i][2 * e], o[i][2 * e + 1]};
-      attn_put<T, D>(a, u, row.at[e], row.head[e], i * 8 + cq * 2, v, v_top, row.l[e], row.m[e]);
-    }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (w == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, CATP_TMEM);
   }
 }
 

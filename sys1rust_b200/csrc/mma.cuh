@@ -66,15 +66,6 @@ S1C_DEV uint4 lds_v4(uint32_t at) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at), "n"(OFF));
   return v;
 }
-// Four 8 x 8 matrices of 16-bit values, a row's address from each lane; _t: transposed.
-template <int OFF>
-S1C_DEV void ldmatrix(uint32_t at, uint32_t (&v)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at), "n"(OFF));
-}
-template <int OFF>
-S1C_DEV void ldmatrix_t(uint32_t at, uint32_t (&v)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at), "n"(OFF));
-}
 // f(integral_constant 0), ..., f(integral_constant N - 1).
 template <typename F, int... I>
 S1C_DEV void static_for_(F&& f, std::integer_sequence<int, I...>) {

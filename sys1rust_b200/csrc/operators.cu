@@ -106,7 +106,7 @@ AttnPlan plan_attention(const CacheView& c, int heads, int n, int max_q, int max
   const int64_t rows = (int64_t)max_q * (heads / c.heads);
   AttnPlan p;
   p.prompt = rows > 32;
-  const int per = p.prompt ? 16 * CATP_WARPS : 16;
+  const int per = p.prompt ? CATP_ROWS : 16;
   p.tiles = (int)((rows + per - 1) / per);
   const int64_t units = (int64_t)n * c.heads * p.tiles;
   // few rows: four rounds of two blocks on 148 SMs; many: one round, since their joining costs more
@@ -124,7 +124,7 @@ size_t attention_workspace(const AttnPlan& p, const CacheView& c, int heads, int
 template <typename T, int D>
 void launch_attention(const CacheView& c, const CacheAttnArgs& a, bool prompt, int dev, cudaStream_t st) {
   const uint64_t rows = (uint64_t)c.num_pages * c.heads * c.page;
-  const uint32_t box = std::min(c.page, CATT_TK);
+  const uint32_t box = std::min(c.page, CATT_BOX);
   const CUtensorMap k = byte_map(c.codes[0], D, rows, D, D, box), v = byte_map(c.codes[1], D, rows, D, D, box);
   const dim3 grid((unsigned)(a.n * c.heads * a.tiles), a.chunks);
   if (prompt) {
