@@ -61,6 +61,12 @@ S1C_DEV float lds_f32(uint32_t at) {
   return v;
 }
 template <int OFF>
+S1C_DEV uint2 lds_v2(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2 + %3];" : "=r"(v.x), "=r"(v.y) : "r"(at), "n"(OFF));
+  return v;
+}
+template <int OFF>
 S1C_DEV uint4 lds_v4(uint32_t at) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at), "n"(OFF));

@@ -4,15 +4,16 @@
 // where given, a zero point z for each group of 32, 64 or 128 columns of a row (z = 8 otherwise).
 //
 // Bound by the codes' bytes up to about 16 rows. A warp takes row tiles of 16 (or 2 x 16) rows in blocks of 128
-// columns; each lane copies its own codes to its own place in shared memory (cp.async), a span of blocks
-// ahead, so it waits for nobody else, and little is spent on a code:
+// columns; it copies its codes to its own place in shared memory (cp.async), a span of blocks ahead, so it waits
+// for no other warp, and little is spent on a code:
 //
 //  - Codes go to mma.m16n8k16 as f16 without arithmetic. The bits of a code at the bottom of a half are
 //    the subnormal q * 2^-24, four places up q * 2^-20, and the tensor cores take subnormals exactly. One
 //    32-bit word gives four operand registers with one shift and four ANDs:
 //    (q0, q4), 16 (q1, q5), (q2, q6), 16 (q3, q7). x is laid out in that order, its factor 1/16 with it.
 //  - Which eight columns of a block a lane's word j holds is free as long as x is laid out alike and the
-//    four lanes of a row stay in one group: 16 bytes in a piece for groups of 128, 8 for 64, 4 for 32.
+//    four lanes of a row stay in one group: words of 16 neighbouring bytes for groups of 128, of 8 for 64, of 4 for
+//    32. A row's 64 bytes lie in shared memory so that these reads meet no bank twice.
 //  - x is brought to f16 by a power of two for each row (its largest value near 2^14), so bf16 and f16
 //    inputs keep all their bits: values below 2^-28 of the row's largest lose low bits, by at most
 //    2^-35 of the largest, far below an fp32 sum's own rounding.
@@ -46,13 +47,9 @@ struct NibbleArgs {
   int split;  // x fits: tiles may be split between warps
 };
 
-// Asynchronous copies of 4, 8 or 16 bytes to shared memory; each thread waits for its own.
-template <int BYTES>
+// Asynchronous copy of 16 bytes to shared memory; each thread waits for its own.
 S1C_DEV void copy_async(uint32_t dst, const void* src) {
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 S1C_DEV void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // All groups but the newest N have landed.
@@ -83,7 +80,7 @@ struct NibbleSmem {
 // 128 columns are copied while the span before is used; ZERO: zero points are given.
 template <typename T, int GROUP, int NT, int RT, int SPAN, int WARPS, bool ZERO>
 struct NibbleWarp {
-  static constexpr int ROWS = 16 * RT, GP = 128 / GROUP, PIECE = GROUP / 8;  // groups of a step; bytes a lane loads at once
+  static constexpr int ROWS = 16 * RT, GP = 128 / GROUP;  // groups of a step
   static constexpr int PART = RT * NT * 4 * 32;                              // floats of a tile's totals
   static constexpr int STEP = RT * 1024, RING = WARPS * 2 * SPAN * STEP;     // bytes of a step's codes; of two spans
   static constexpr int NS = (SPAN * GP + 3) / 4;  // scales of a row and span that one of its four lanes holds
@@ -94,13 +91,19 @@ struct NibbleWarp {
   const uint8_t* code[RT][2];            // next codes of the tile being loaded; rows past N read the last one
   const uint16_t* scale[RT][2];
   const uint16_t* zero[ZERO ? RT : 1][2];
-  uint32_t ring;                         // this lane's place in the first of the two spans' copies
+  // In the first of the two spans' copies: where this lane's 16 bytes of a row go (chunk c of its row), and where its words of
+  // group 0 and (XORed) of the others are. Chunks of 16 bytes are moved by the row: all of 32 bytes for groups
+  // of 64, of 16 for 32.
+  uint32_t copy_at, word_at;
   uint32_t sz[2][RT][2][NS];             // (scale, zero point) of the span in use and of the next
   float total[RT][NT][4];
 
   S1C_DEV void setup(const uint8_t* ring_, const __half* xs, const float* sums, int pitch, int sum_pitch) {
     const int g = lane >> 2, c = lane & 3;
-    ring = smem_u32(ring_) + lane * 16;
+    const uint32_t row = smem_u32(ring_) + g * 64;
+    const int move = GROUP == 128 ? 0 : GROUP == 64 ? (g >> 1 & 1) * 2 : g >> 1 & 3;  // of a chunk, by XOR
+    copy_at = row + ((c ^ move) << 4);
+    word_at = row + (GROUP == 128 ? c * 16 : GROUP == 64 ? (move << 4) + c * 8 : (move << 4) + c * 4);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       x_at[j] = smem_u32(xs + min(8 * j + g, a.M - 1) * pitch + c * 8);
@@ -114,7 +117,7 @@ struct NibbleWarp {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int64_t n = min((int64_t)tile * ROWS + r * 16 + h * 8 + (lane >> 2), (int64_t)a.N - 1);
-        code[r][h] = a.codes + n * a.pitch + step * 64 + (lane & 3) * PIECE;
+        code[r][h] = a.codes + n * a.pitch + step * 64 + (lane & 3) * 16;
         scale[r][h] = static_cast<const uint16_t*>(a.scales) + n * a.scale_stride + step * GP;
         if (ZERO) zero[r][h] = static_cast<const uint16_t*>(a.zeros) + n * a.scale_stride + step * GP;
       }
@@ -123,16 +126,12 @@ struct NibbleWarp {
   // read its first ones.
   template <int S, bool TAIL>
   S1C_DEV void load(int step, uint32_t side) {
+    int off = S * 64;
+    if (TAIL && step * 64 + (lane & 3) * 16 >= a.width) off = (S - step) * 64 - (lane & 3) * 16;
 #pragma unroll
-    for (int q = 0; q < GP; ++q) {
-      int off = S * 64 + q * 4 * PIECE;
-      if (TAIL && step * 64 + q * 4 * PIECE + (lane & 3) * PIECE >= a.width) off = (S - step) * 64 - (lane & 3) * PIECE;
+    for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          copy_async<PIECE>(ring + side * (SPAN * STEP) + S * STEP + (r * 2 + h) * 512 + q * PIECE, code[r][h] + off);
-    }
+      for (int h = 0; h < 2; ++h) copy_async(copy_at + side * (SPAN * STEP) + S * STEP + (r * 2 + h) * 512, code[r][h] + off);
   }
   // A span's scales and zero points, spread over the four lanes of a row. Groups past the last read the last one.
   S1C_DEV void fetch(uint32_t (&v)[RT][2][NS], int step) {
@@ -170,13 +169,20 @@ struct NibbleWarp {
   template <int S>
   S1C_DEV void consume(int ahead, uint32_t side) {
     uint32_t words[RT][2][4];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 p = lds_v4<S * STEP>(ring + side * (SPAN * STEP) + (r * 2 + h) * 512);
-        words[r][h][0] = p.x, words[r][h][1] = p.y, words[r][h][2] = p.z, words[r][h][3] = p.w;
+    const uint32_t from = word_at + side * (SPAN * STEP);
+    static_for<RT * 2>([&](auto X) {
+      constexpr int r = decltype(X)::value / 2, h = decltype(X)::value % 2, OFF = S * STEP + decltype(X)::value * 512;
+      uint32_t(&w)[4] = words[r][h];
+      if constexpr (GROUP == 128) {
+        const uint4 p = lds_v4<OFF>(from);
+        w[0] = p.x, w[1] = p.y, w[2] = p.z, w[3] = p.w;
+      } else if constexpr (GROUP == 64) {
+        const uint2 p0 = lds_v2<OFF>(from), p1 = lds_v2<OFF>(from ^ 32);
+        w[0] = p0.x, w[1] = p0.y, w[2] = p1.x, w[3] = p1.y;
+      } else {
+        static_for<4>([&](auto I) { w[decltype(I)::value] = lds_u32<OFF>(from ^ (decltype(I)::value * 16)); });
       }
+    });
     static_for<GP>([&](auto Q) {
       constexpr int q = decltype(Q)::value, at = S * GP + q;
       float acc[RT][NT][4];
@@ -288,6 +294,7 @@ S1C_DEV void nibble_stage(const NibbleArgs& a, __half* xs, float* sums, float* r
   for (int p = w; p < a.M * parts; p += WARPS) {
     const int m = p / parts, s0 = p % parts * passes / parts, s1 = (p % parts + 1) * passes / parts;
     uint32_t top = 0;
+#pragma unroll 4
     for (int s = s0; s < s1; ++s) {
       const int k = first + s * 256 + lane * 8;
       uint32_t v[4] = {};
@@ -314,6 +321,7 @@ S1C_DEV void nibble_stage(const NibbleArgs& a, __half* xs, float* sums, float* r
     const int e = (int)(tops[m] >> 23) - 127, up = e == 128 ? 0 : min(14 - e, 100);
     const float by = __uint_as_float((uint32_t)(127 + up) << 23);
     if (lane == 0) row_scale[m] = __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll 2
     for (int s = s0; s < s1; ++s) {
       uint4* slot = reinterpret_cast<uint4*>(xs + m * pitch + s * 256 + place);
       const uint4 u = *slot;
@@ -334,7 +342,7 @@ S1C_DEV void nibble_stage(const NibbleArgs& a, __half* xs, float* sums, float* r
 template <typename T, int GROUP, int NT, int RT, int SPAN, int WARPS, bool ZERO>
 __global__ void __launch_bounds__(WARPS * 32) nibble_kernel(const NibbleArgs a) {
   using W = NibbleWarp<T, GROUP, NT, RT, SPAN, WARPS, ZERO>;
-  extern __shared__ __align__(16) uint8_t base[];
+  extern __shared__ __align__(128) uint8_t base[];
   const bool split = a.split;
   const NibbleSmem sm(a.M, a.block, GROUP, W::RING, WARPS * W::PART, split);
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -424,12 +432,25 @@ __global__ void __launch_bounds__(WARPS * 32) nibble_kernel(const NibbleArgs a) 
     const int have = a.steps - step;
     const uint32_t side = i & 1;
     if (left > 0) p.fetch(p.sz[1], next_step);
-    static_for<SPAN>([&](auto S) {
-      constexpr int s = decltype(S)::value;
-      load(S, side ^ 1);
-      copy_wait<SPAN>();
-      if (s < have) p.template consume<s>(at * 128, side);
-    });
+    if (left > 0 && have >= SPAN && next_step + SPAN < a.steps) {
+      // whole spans: no step to ask about
+      static_for<SPAN>([&](auto S) {
+        constexpr int s = decltype(S)::value;
+        p.template load<s, false>(0, side ^ 1);
+        copy_commit();
+        copy_wait<SPAN>();
+        __syncwarp();
+        p.template consume<s>(at * 128, side);
+      });
+    } else {
+      static_for<SPAN>([&](auto S) {
+        constexpr int s = decltype(S)::value;
+        load(S, side ^ 1);
+        copy_wait<SPAN>();
+        __syncwarp();
+        if (s < have) p.template consume<s>(at * 128, side);
+      });
+    }
     loaded();
 #pragma unroll
     for (int r = 0; r < RT; ++r)
