@@ -109,8 +109,8 @@ AttnPlan plan_attention(const CacheView& c, int heads, int n, int max_q, int max
   const int per = p.prompt ? CATP_ROWS : 16;
   p.tiles = (int)((rows + per - 1) / per);
   const int64_t units = (int64_t)n * c.heads * p.tiles;
-  // few rows: four rounds of two blocks on 148 SMs; many: one round, since their joining costs more
-  const int64_t want = (units * max_kv + (p.prompt ? 295 : 1183)) / (p.prompt ? 296 : 1184);
+  // one round of the blocks that 148 SMs hold, three each, or two of a prompt's
+  const int64_t round = p.prompt ? 296 : 444, want = (units * max_kv + round - 1) / round;
   const int64_t most = p.prompt ? (int64_t)CATP_PAGES * c.page - 128 : std::min<int64_t>(2048, (int64_t)CATT_PAGES * c.page);
   p.chunk = (int)std::max<int64_t>(128, std::min(most, (want + 127) / 128 * 128));
   if (p.prompt && units >= 148 && max_kv <= most) p.chunk = (int)most;
