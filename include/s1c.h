@@ -255,14 +255,14 @@ S1C_API s1c_status s1c_selftest_wait_timeout(int32_t device, int64_t budget_ns, 
 S1C_API int64_t s1c_last_launch_count(const s1c_backend* b);
 
 /* ---- Token-step operators (no counterpart in the reference) ---------------------------------
- * What a host that generates an answer token by token runs beside the encoder, on device pointers:
- * products of a few rows with 4-bit weights, a paged cache of keys and values held in 8 bits, causal
- * attention over that cache, and sampling. Every call checks its arguments (S1C_ERR_ARG, text in
- * s1c_create_error()), runs on the device that holds its output, enqueues its work on `stream` (a
- * cudaStream_t of that device, NULL = legacy default stream), allocates nothing, does not synchronise and can be
- * captured into a CUDA graph. Device-side integers (offsets, lengths, page tables) are read when the
- * kernels run, so a graph replays with other lengths below the same bounds. `dtype` is an
- * S1C_DT_ code; strides count elements. Results do not change from one call to the next. */
+ * What a host that generates an answer token by token runs beside the encoder, on device pointers: products
+ * of a few rows with 4-bit weights, a paged cache of keys and values held in 8 bits, causal attention over
+ * that cache, and sampling. Every call checks its arguments (S1C_ERR_ARG, text in s1c_create_error()), runs
+ * on the device that holds its output, enqueues its work on `stream` (a cudaStream_t of that device, NULL =
+ * legacy default stream), allocates nothing, does not synchronise and can be captured into a CUDA graph.
+ * Device-side integers (offsets, lengths, page tables) are read when the kernels run, so a graph replays
+ * with other lengths below the same bounds. `dtype` is an S1C_DT_ code; strides count elements. Results do
+ * not change from one call to the next. */
 
 /* out[m, n] = act( sum_g s[n, g] * sum_{k in g} (q[n, k] - z[n, g]) * x[m, k] + bias[n] ): M rows x
  * [M, K] (0 to 64) times a matrix [N, K] held as 4-bit codes q. Column k of row n is the low (even k) or
@@ -292,13 +292,14 @@ typedef struct s1c_cache {
 } s1c_cache;
 
 /* Append: rows d_cu[i] .. d_cu[i+1] of k and v (F16 or BF16, [rows, kv_heads, head_dim] with a row
- * stride) become positions d_start[i] .. of sequence i, for n sequences of at most max_new rows (what is longer is cut there).
- * For a page and head that new rows fall into, s = max(s_old, max |new| / 127), s_old being the page's scale if earlier rows of the sequence
- * stand in it and 0 otherwise. A new code is x / s rounded half to even, and where s grew, the earlier rows'
- * codes become code * s_old / s rounded half to even, both of the exact quotient. Infinities become +-127 and NaN 0, and
- * neither counts in the maximum. Rows behind the last new one are left as they were. Rows whose page is not in
- * [0, num_pages), or whose position is past the table, are dropped. A page written for two sequences in
- * one call ends with unspecified codes. */
+ * stride) become positions d_start[i] .. of sequence i, for n sequences of at most max_new rows (what is
+ * longer is cut there). For a page and head that new rows fall into, s = max(s_old, max |new| / 127), s_old
+ * being the page's scale if earlier rows of the sequence stand in it and 0 otherwise. A new code is x / s
+ * rounded half to even, and where s grew, the earlier rows' codes become code * s_old / s rounded half to
+ * even, both of the exact quotient. Infinities become +-127 and NaN 0, and neither counts in the maximum.
+ * Rows behind the last new one are left as they were. Rows whose page is not in [0, num_pages), or whose
+ * position is past the table, are dropped. A page written for two sequences in one call ends with
+ * unspecified codes. */
 S1C_API s1c_status s1c_cache_write(const s1c_cache* cache, int32_t dtype, const void* d_k, int64_t k_stride,
                                    const void* d_v, int64_t v_stride, const int32_t* d_cu, const int32_t* d_start,
                                    const int32_t* d_pages, int32_t max_pages, int32_t n, int32_t max_new, void* stream);
@@ -319,9 +320,10 @@ S1C_API size_t s1c_cache_attention_workspace(const s1c_cache* cache, int32_t hea
  * whose page is in [0, num_pages). q and out are [rows, heads, head_dim] (F16 or BF16, row
  * strides); query head h reads key head h / (heads / kv_heads). lse (nullable, [rows, heads]
  * fp32) is the natural log of the sum of exp(scale * q . k). A query that sees no key gets out 0 and lse
- * -inf. No sequence may have more than max_q query rows or max_kv positions: what is past them is not computed.
- * Scores, softmax statistics and sums are held in fp32. The workspace (16-byte aligned) is free for other use when the call's
- * work has run; calls that overlap on the GPU need one each. */
+ * -inf. No sequence may have more than max_q query rows or max_kv positions: what is past them is not
+ * computed. Scores, softmax statistics and sums are held in fp32; a key's weight times its value scale is
+ * rounded to 11 bits, or to 2^-38 of the row's largest where that is more. The workspace (16-byte aligned) is free
+ * for other use when the call's work has run; calls that overlap on the GPU need one each. */
 S1C_API s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, const void* d_q, int64_t q_stride,
                                        void* d_out, int64_t out_stride, float* d_lse, int32_t heads,
                                        const int32_t* d_cu, const int32_t* d_len, const int32_t* d_pages,
@@ -329,13 +331,14 @@ S1C_API s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, co
                                        float scale, void* d_workspace, size_t workspace_bytes, void* stream);
 
 /* One token for each row of logits [rows, vocab] (F32, F16 or BF16). With e_i = exp((l_i - max l) / T)
- * and the tokens ordered by descending logit (equal ones by index): top-k keeps the first k (k <= 0: all); top-p keeps, of these, the
- * first and every one before which less than p times their mass lies (p >= 1: all); min-p keeps those with
- * e_i >= min(min_p, 1). The token is the first index, in ascending order, at which the kept mass
- * summed so far exceeds u times the kept mass (u >= 1 or NaN: the last kept one); prob (nullable) is its share of the kept mass.
- * T <= 0 or NaN takes the largest logit, the lowest index among equals, with prob 1. temperature, top_k, top_p and min_p hold
- * a value for each row and are nullable (1, off, off, off). Logits of -inf are never chosen; a row with a
- * NaN or +inf, or with nothing above -inf, gets token -1 and prob 0. vocab is at most 2^18. */
+ * and the tokens ordered by descending logit (equal ones by index): top-k keeps the first k (k <= 0: all);
+ * top-p keeps, of these, the first and every one before which less than p times their mass lies (p >= 1:
+ * all); min-p keeps those with e_i >= min(min_p, 1). The token is the first index, in ascending order, at
+ * which the kept mass summed so far exceeds u times the kept mass (u >= 1 or NaN: the last kept one); prob
+ * (nullable) is its share of the kept mass. T <= 0 or NaN takes the largest logit, the lowest index among
+ * equals, with prob 1. temperature, top_k, top_p and min_p hold a value for each row and are nullable (1,
+ * off, off, off). Logits of -inf are never chosen; a row with a NaN or +inf, or with nothing above -inf,
+ * gets token -1 and prob 0. vocab is at most 2^18. */
 S1C_API s1c_status s1c_sample(int32_t dtype, const void* d_logits, int64_t row_stride, int32_t rows, int32_t vocab,
                               const float* d_temperature, const int32_t* d_top_k, const float* d_top_p,
                               const float* d_min_p, const float* d_uniform, int32_t* d_token, float* d_prob,

@@ -15,19 +15,20 @@
 //  - values: the sum runs over keys, so a register pairs two keys' codes of one dimension; words of two
 //    keys are interleaved by byte permutes, put under the exponent of 1024 and 1152 subtracted.
 //  - a page's value scale differs from its neighbours' inside one sum, so it goes into the weight: with t = log2(scale /
-//    largest scale of the block), the weight is exp2(s + t - m + 14.5), m a running maximum of s + t, and the sum of
-//    the softmax adds weight * 2^-t. m follows the true maximum only when that is 1.25 ahead, so outputs are
+//    largest scale of the block), the weight is exp2(s + t - m + 14), m a running maximum of s + t, and the sum of
+//    the softmax adds weight * 2^-t. m follows the true maximum only when that is 1.75 ahead, so outputs are
 //    seldom rescaled. Weights are held as f16: at most 2^15.75, with all 11 bits down to 2^-28 of the
 //    largest; scores, maxima, sums and outputs are fp32.
 //
-// Few query rows (bound by the cache's bytes): each warp has its own tiles of the block's keys and its own ring
-// of loads, so nothing waits inside the loop; the four warps' results are joined at the end. Long caches are split
-// over blocks, whose results a second kernel joins.
+// Few query rows (bound by the cache's bytes): each warp has its own tiles of the block's keys and its own
+// ring of loads, so nothing waits inside the loop; the four warps' results are joined at the end. Long
+// caches are split over blocks, whose results a second kernel joins.
 //
-// Many rows: a block of 128 rows on the 5th-generation tensor cores. Four warps convert a tile of 64 keys once for all
-// rows, to f16 in shared memory (whole codes, so no scale enters before the scores); one thread issues S = Q K^T into one of two
-// buffers of TMEM, a tile ahead, and O += P V; four warps have a row in each thread, and write the weights P over the scores
-// they come from, where the second product reads them as its first operand.
+// Many rows: a block of 128 rows on the 5th-generation tensor cores. Four warps convert a tile of 64 keys
+// once for all rows, to f16 in shared memory (whole codes, so no scale enters before the scores); one
+// thread issues S = Q K^T into one of two buffers of TMEM, a tile ahead, and O += P V; four warps have a
+// row in each thread, and write the weights P over the scores they come from, where the second product
+// reads them as its first operand.
 #pragma once
 #include <cuda.h>
 #include <limits.h>
@@ -84,8 +85,8 @@ S1C_DEV bool attn_unit(const CacheView& c, const CacheAttnArgs& a, AttnUnit& u) 
   return true;
 }
 
-// The chunk's pages: (key scale * 2^24, t, 2^-t, page), a few more than there are, without a page (-1) 0, -inf, 0. Returns the
-// largest value scale, which the outputs are multiplied by. All threads call.
+// The chunk's pages: (key scale * 2^24, t, 2^-t, page), a few more than there are, without a page (-1) 0,
+// -inf, 0. Returns the largest value scale, which the outputs are multiplied by. All threads call.
 template <int WARPS>
 S1C_DEV float attn_pages(const CacheView& c, const CacheAttnArgs& a, const AttnUnit& u, float4* list, float* tops) {
   const int tid = threadIdx.x, p0 = u.lo >> u.shift, pages = ((u.hi - 1) >> u.shift) - p0 + 1;  // and more behind them than a tile has
@@ -107,8 +108,9 @@ S1C_DEV float attn_pages(const CacheView& c, const CacheAttnArgs& a, const AttnU
   for (int i = 0; i < WARPS; ++i) top = fmaxf(top, tops[i]);
   for (int i = tid; i < pages + ATTN_BEYOND; i += WARPS * 32) {
     float4 e = list[i];
-    // scales below 2^-60 of the largest (and zero ones, whose codes are zero) count as that
-    const float l2 = top > 0.f ? fmaxf(log2f(e.y / top), -60.f) : 0.f;
+    // scales below 2^-90 of the largest (and zero ones, whose codes are zero) count as that: the sum then stays
+    // below 2^(15.75 + 90 + 14) for the 2^14 keys of a chunk
+    const float l2 = top > 0.f ? fmaxf(log2f(e.y / top), -90.f) : 0.f;
     const bool in = __float_as_int(e.w) >= 0;
     e.y = in ? l2 : -INFINITY, e.z = in ? exp2f(-l2) : 0.f;
     list[i] = e;
@@ -117,8 +119,8 @@ S1C_DEV float attn_pages(const CacheView& c, const CacheAttnArgs& a, const AttnU
   return top;
 }
 
-// TMA of one tile's keys and values to `dst`, by a whole warp: a lane for each page or 32 rows of one. Pages outside
-// the cache are not read.
+// TMA of one tile's keys and values to `dst`, by a whole warp: a lane for each page or 32 rows of one.
+// Pages outside the cache are not read.
 template <int D, int TK>
 S1C_DEV void attn_issue(const CacheView& c, const AttnUnit& u, const float4* list, const CUtensorMap& k_map, const CUtensorMap& v_map, int i,
                         uint8_t* dst, uint64_t* bar) {
@@ -157,8 +159,8 @@ struct AttnRows {
       m[e] = -INFINITY, l[e] = 0.f;
     }
   }
-  // The rows as f16 operands. The columns 2 cq, 2 cq + 1 (and those 8 on) of operand i are dimensions 16 i + 4 cq .. + 3, the order
-  // of a lane's word of codes.
+  // The rows as f16 operands. The columns 2 cq, 2 cq + 1 (and those 8 on) of operand i are dimensions 16 i
+  // + 4 cq .. + 3, the order of a lane's word of codes.
   template <typename T, int D>
   S1C_DEV void operands(const CacheAttnArgs& a, uint32_t (&qa)[D / 16][4]) {
     const int cq = threadIdx.x % 4;
@@ -188,8 +190,9 @@ struct AttnRows {
       start[e] = sum * -0x1p-17f;
     }
   }
-  // Scores (in units of the key scale * factor) of a tile that begins at `key` to weights times 2^14.5; the sums take them, and the
-  // outputs o are rescaled when the maximum has grown. kc0, kc1: where a lane's two columns stand among eight keys.
+  // Scores (in units of the key scale * factor) of a tile that begins at `key` to weights times 2^14; the
+  // sums take them, and the outputs o are rescaled when the maximum has grown. kc0, kc1: where a lane's two
+  // columns stand among eight keys.
   template <int N>
   S1C_DEV void weights(const CacheView& c, const AttnUnit& u, const float4* list, int key, int kc0, int kc1, float (&s)[4][4], float (&o)[N][4]) {
     const bool open = key + CATT_TK - 1 <= pos[0] && key >= pos[1] - u.window && key + CATT_TK <= u.hi;
@@ -224,7 +227,7 @@ struct AttnRows {
     for (int e = 0; e < 2; ++e) {
       top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
       top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-      grows |= top[e] > m[e] + 1.25f;
+      grows |= top[e] > m[e] + 1.75f;
     }
     if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
@@ -235,7 +238,7 @@ struct AttnRows {
         for (int i = 0; i < N; ++i) o[i][2 * e] *= keep, o[i][2 * e + 1] *= keep;
       }
     }
-    const float off[2] = {m[0] == -INFINITY ? 0.f : 14.5f - m[0], m[1] == -INFINITY ? 0.f : 14.5f - m[1]};
+    const float off[2] = {m[0] == -INFINITY ? 0.f : 14.f - m[0], m[1] == -INFINITY ? 0.f : 14.f - m[1]};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -262,11 +265,11 @@ S1C_DEV void attn_pack(const float (&s)[4][4], uint32_t (&pa)[2][4]) {
   }
 }
 
-// N neighbouring dimensions, from d on, of one row's result: v * v_top / sum, with log2 of the sum beside dimension 0. Without a
-// key the sum is 0: outputs 0 and -inf.
+// N neighbouring dimensions, from d on, of one row's result: v * v_top / sum, with log2 of the sum beside
+// dimension 0. Without a key the sum is 0: outputs 0 and -inf.
 template <typename T, int D, int N>
 S1C_DEV void attn_put(const CacheAttnArgs& a, const AttnUnit& u, int64_t row, int head, int d, const float (&v)[N], float v_top, float sum, float top) {
-  const float by = sum == 0.f ? 0.f : v_top / sum, log_sum = sum == 0.f ? -INFINITY : top - 14.5f + log2f(sum);
+  const float by = sum == 0.f ? 0.f : v_top / sum, log_sum = sum == 0.f ? -INFINITY : top - 14.f + log2f(sum);
   if (a.chunks > 1) {
     const int64_t at = ((u.seq * (int64_t)a.max_q + (row - u.first)) * a.heads + head) * a.chunks + u.chunk;
 #pragma unroll
@@ -335,7 +338,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   }
   const uint32_t q_at = smem_u32(&sm.q[0][lane]);
 
-  // shared offsets in a slot: the swizzle moves a row's 16-byte pieces by the row (128-byte rows) or by half of it
+  // shared offsets in a slot: the swizzle moves a row's 16-byte pieces by the row (128-byte rows) or by
+  // half of it
   const int kr = D == 128 ? g : (g & 4) | (g & 1) << 1 | (g >> 1 & 1);
   uint32_t k_at[QK], v_at[2][SEG];
 #pragma unroll
@@ -435,12 +439,14 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 
 // Many query rows: warps 0 to 3 softmax (thread = row = TMEM lane), 4 to 7 conversion, 8 products.
 constexpr int CATP_ROWS = 128, CATP_WARPS = 9, CATP_PAGES = 256;
-// TMEM columns: scores (then weights, f16 pairs, over the first 32 columns) of even tiles [0, 64), of odd tiles [64, 128); outputs from 128 on
+// TMEM columns: scores (then weights, f16 pairs, over the first 32 columns) of even tiles [0, 64), of odd
+// tiles [64, 128); outputs from 128 on
 constexpr uint32_t CATP_TMEM = 256, CATP_TMEM_O = 128;
 
 template <int D>
 struct CachePromptSmem {
-  // blocks of 64 dimensions, rows of 128 bytes, 16-byte pieces XORed with the row: the 128-byte swizzle of the products' operands
+  // blocks of 64 dimensions, rows of 128 bytes, 16-byte pieces XORed with the row: the 128-byte swizzle of
+  // the products' operands
   alignas(1024) uint8_t q[D / 64][CATP_ROWS * 128];
   alignas(1024) uint8_t k[D / 64][CATP_TK * 128];
   alignas(1024) uint8_t v[2][D / 64][CATP_TK * 128];
@@ -639,7 +645,7 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       for (int x = 0; x < 64; ++x) part[x & 3] = fmaxf(part[x & 3], s[x]);
       const float top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
       float keep = 1.f;
-      if (top > m + 1.25f) {
+      if (top > m + 1.75f) {
         keep = m == -INFINITY ? 0.f : exp2f(m - top);
         l *= keep;
         m = top;
@@ -660,7 +666,7 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
           tmem_st16(tmem + lanes + CATP_TMEM_O + x, t);
         }
       }
-      const float off = m == -INFINITY ? 0.f : 14.5f - m;
+      const float off = m == -INFINITY ? 0.f : 14.f - m;
       float pk[32];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {

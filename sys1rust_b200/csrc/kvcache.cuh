@@ -34,10 +34,10 @@ S1C_DEV int cache_page(const int* table, int64_t max_pages, int seq, int64_t at,
   return p >= 0 && p < num_pages ? p : -1;
 }
 
-// round-half-even(x / s) of the exact quotient, for |x| <= about 127 s and s >= 2^-100. The product
-// with the rounded reciprocal is within 1 of it. Where x / s is near a half, x is a multiple of s's last place
-// (a 16-bit type's x has at most 11 bits and is at least s / 2), so the remainder x - n s is exact in fp32 and its comparison with s / 2
-// decides; elsewhere its sign relative to s / 2 survives the rounding.
+// round-half-even(x / s) of the exact quotient, for |x| <= about 127 s and s >= 2^-100. The product with
+// the rounded reciprocal is within 1 of it. Where x / s is near a half, x is a multiple of s's last place
+// (a 16-bit type's x has at most 11 bits and is at least s / 2), so the remainder x - n s is exact in fp32
+// and its comparison with s / 2 decides; elsewhere its sign relative to s / 2 survives the rounding.
 S1C_DEV int quantise(float x, float s, float inv) {
   float n = rintf(x * inv);
   const float d = fmaf(-n, s, x), h = 0.5f * s;
@@ -52,8 +52,8 @@ S1C_DEV uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// Eight quotients x * by rounded to bytes by the place that adding 1.5 * 2^23 gives them; false where one is so near a half
-// that the product's error (below 3e-5) could decide, or is not finite.
+// Eight quotients x * by rounded to bytes by the place that adding 1.5 * 2^23 gives them; false where one
+// is so near a half that the product's error (below 3e-5) could decide, or is not finite.
 S1C_DEV bool quantise_fast(const float (&x)[8], float by, uint32_t (&q)[2]) {
   float worst = 0.f;
   uint32_t n[8];
@@ -180,9 +180,9 @@ __global__ void __launch_bounds__(128) cache_write_kernel(const CacheView c, con
   }
 }
 
-// Rows read back: value = code * scale, rounded once. A block has 128 rows (of 64 values: 256) of one head, a
-// thread 16 values (16 B of codes, 32 B of output) of four of them; rows on pages outside the cache are written as 0.
-// A byte code becomes fp32 under the exponent of 2^23.
+// Rows read back: value = code * scale, rounded once. A block has 128 rows (of 64 values: 256) of one head,
+// a thread 16 values (16 B of codes, 32 B of output) of four of them; rows on pages outside the cache are
+// written as 0. A byte code becomes fp32 under the exponent of 2^23.
 template <typename T>
 __global__ void __launch_bounds__(256) cache_read_kernel(const CacheView c, const CacheRows r) {
   const int seq = blockIdx.x / r.units, h = blockIdx.y, kv = blockIdx.z;

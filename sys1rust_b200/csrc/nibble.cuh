@@ -3,9 +3,9 @@
 // with codes q in 0..15 packed two to a byte (the even column in the low half), a scale s and,
 // where given, a zero point z for each group of 32, 64 or 128 columns of a row (z = 8 otherwise).
 //
-// Bound by the codes' bytes up to about 16 rows. A warp takes row tiles of 16 (or 2 x 16) rows in blocks of 128
-// columns; it copies its codes to its own place in shared memory (cp.async), a span of blocks ahead, so it waits
-// for no other warp, and little is spent on a code:
+// Bound by the codes' bytes up to about 16 rows. A warp takes row tiles of 16 (or 2 x 16) rows in blocks of
+// 128 columns; it copies its codes to its own place in shared memory (cp.async), a span of blocks ahead, so
+// it waits for no other warp, and little is spent on a code:
 //
 //  - Codes go to mma.m16n8k16 as f16 without arithmetic. The bits of a code at the bottom of a half are
 //    the subnormal q * 2^-24, four places up q * 2^-20, and the tensor cores take subnormals exactly. One
@@ -91,9 +91,9 @@ struct NibbleWarp {
   const uint8_t* code[RT][2];            // next codes of the tile being loaded; rows past N read the last one
   const uint16_t* scale[RT][2];
   const uint16_t* zero[ZERO ? RT : 1][2];
-  // In the first of the two spans' copies: where this lane's 16 bytes of a row go (chunk c of its row), and where its words of
-  // group 0 and (XORed) of the others are. Chunks of 16 bytes are moved by the row: all of 32 bytes for groups
-  // of 64, of 16 for 32.
+  // In the first of the two spans' copies: where this lane's 16 bytes of a row go (chunk c of its row), and
+  // where its words of group 0 and (XORed) of the others are. Chunks of 16 bytes are moved by the row: all
+  // of 32 bytes for groups of 64, of 16 for 32.
   uint32_t copy_at, word_at;
   uint32_t sz[2][RT][2][NS];             // (scale, zero point) of the span in use and of the next
   float total[RT][NT][4];
@@ -133,7 +133,8 @@ struct NibbleWarp {
 #pragma unroll
       for (int h = 0; h < 2; ++h) copy_async(copy_at + side * (SPAN * STEP) + S * STEP + (r * 2 + h) * 512, code[r][h] + off);
   }
-  // A span's scales and zero points, spread over the four lanes of a row. Groups past the last read the last one.
+  // A span's scales and zero points, spread over the four lanes of a row. Groups past the last read the
+  // last one.
   S1C_DEV void fetch(uint32_t (&v)[RT][2][NS], int step) {
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
@@ -281,7 +282,8 @@ struct NibbleWarp {
 };
 
 // Stages columns [first, first + passes * 256) of x: f16 by a power of two for each row, in the order of
-// the codes, and the groups' sums times -2^-24 (-8 * 2^-24 without zero points). A pair (row, part of its passes) belongs to one warp.
+// the codes, and the groups' sums times -2^-24 (-8 * 2^-24 without zero points). A pair (row, part of its
+// passes) belongs to one warp.
 template <typename T, int GROUP, int WARPS, bool ZERO>
 S1C_DEV void nibble_stage(const NibbleArgs& a, __half* xs, float* sums, float* row_scale, uint32_t* tops, int pitch, int sum_pitch,
                           int first, int passes, int groups) {
@@ -472,7 +474,8 @@ __global__ void __launch_bounds__(WARPS * 32) nibble_kernel(const NibbleArgs a) 
     if (!split && at == a.block) at = 0;
   }
   if (!split) return;
-  // Tiles split between warps: the warp with the first piece, which it still holds, adds the later ones in order.
+  // Tiles split between warps: the warp with the first piece, which it still holds, adds the later ones in
+  // order.
   __syncthreads();
   const int end = f0 + count, t0 = (end - 1) / spans * spans;
   if (count == 0 || end % spans == 0 || t0 < f0) return;

@@ -97,7 +97,8 @@ CacheRows check_rows(const CacheView& c, const void* k, int64_t k_stride, const 
   return r;
 }
 
-// How an attention call is laid out: blocks of 16 rows, or of many that share the keys' conversion; keys of a block.
+// How an attention call is laid out: blocks of 16 rows, or of many that share the keys' conversion; keys of
+// a block.
 struct AttnPlan {
   bool prompt;
   int tiles, chunk, chunks;
@@ -178,7 +179,7 @@ s1c_status s1c_nibble_gemm(int32_t dtype, const void* d_x, int64_t x_stride, con
   return enter([&] {
     check_half(dtype);
     need(d_x && d_codes && d_scales && d_out, "null argument");
-    need(M >= 0 && M <= 64 && N > 0 && K > 0, "M must be 0 to 64, N and K positive");
+    need(M >= 0 && M <= 64 && N > 0 && K > 0 && N <= (1 << 30) && K <= (1 << 30), "M must be 0 to 64, N and K 1 to 2^30");
     need(group == 32 || group == 64 || group == 128, "group must be 32, 64 or 128");
     const int64_t groups = ((int64_t)K + group - 1) / group;
     need(code_pitch % 16 == 0 && code_pitch >= ((int64_t)K + 31) / 32 * 16 && aligned(d_codes, 16),

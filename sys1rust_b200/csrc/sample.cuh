@@ -1,9 +1,9 @@
 // One token for each row of logits under temperature, top-k, top-p and min-p.
 //
-// With z_i = (max l - l_i) / T and e_i = exp(-z_i), tokens ordered by descending logit (the lowest index first
-// among equals): top-k keeps the first k; top-p keeps, of these, the first and every one whose
-// predecessors' mass is below p times the mass of the k; min-p keeps those with e_i >= min_p. The
-// token is the first index, in ascending order, at which the kept mass summed so far exceeds u times the kept mass.
+// With z_i = (max l - l_i) / T and e_i = exp(-z_i), tokens ordered by descending logit (the lowest index
+// first among equals): top-k keeps the first k; top-p keeps, of these, the first and every one whose
+// predecessors' mass is below p times the mass of the k; min-p keeps those with e_i >= min_p. The token is
+// the first index, in ascending order, at which the kept mass summed so far exceeds u times the kept mass.
 //
 // No sort is needed: both filters cut the order at one value, so each is a threshold (a logit, and how
 // many of its equals are kept, by index). A cluster of blocks shares a row:
@@ -17,9 +17,9 @@
 //     of the logit, 2048 ways at a time, until one value is left. What is kept is summed and walked. More
 //     than fit in the list are worked on in place.
 //
-// Masses are integers: e = m * 2^(n - 24), m an integer of 25 bits, and all e in one bin share n. So their sums are
-// exact and depend neither on the order of atomics nor on how a row is shared. Logits more than 45 powers of two
-// below the largest have no mass.
+// Masses are integers: e = m * 2^(n - 24), m an integer of 25 bits, and all e in one bin share n. So their
+// sums are exact and depend neither on the order of atomics nor on how a row is shared. Logits more than 45
+// powers of two below the largest have no mass.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -54,9 +54,10 @@ S1C_DEV float key_logit(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k
 
 S1C_DEV double pow2(int e) { return __hiloint2double((1023 + e) << 20, 0); }
 
-// exp as an integer: the bin of z and m with e = m * 2^(n - 24), n from the bin. The bin comes from the rounded product (it
-// only has to be monotonic); the mass adds what the difference and the product lost. 2^f by the Taylor series of
-// exp(f ln 2), |f| <= 0.52: its tenth term is below 1e-10, and rounding to fp32 leaves about 5e-8.
+// exp as an integer: the bin of z and m with e = m * 2^(n - 24), n from the bin. The bin comes from the
+// rounded product (it only has to be monotonic); the mass adds what the difference and the product lost.
+// 2^f by the Taylor series of exp(f ln 2), |f| <= 0.52: its tenth term is below 1e-10, and rounding to fp32
+// leaves about 5e-8.
 struct SampleMass {
   float top, rate, rate_lo;  // max l, log2(e) / T in two parts
   S1C_DEV SampleMass(float top_, float T) : top(top_) {
@@ -285,8 +286,8 @@ S1C_DEV unsigned long long sample_scan(SampleShared& s, unsigned long long v, un
   return v + __shfl_sync(0xffffffffu, sum - own, w);
 }
 
-// Step 3 for a list of up to 512, by one block: a bitonic sort of (key, place) with an element for each thread, then
-// ranks and masses are at hand.
+// Step 3 for a list of up to 512, by one block: a bitonic sort of (key, place) with an element for each
+// thread, then ranks and masses are at hand.
 S1C_DEV void sample_choose_sorted(SampleShared& s, const SampleArgs& a, int r, const SampleMass& f, int n, int k, float p, double least,
                                   unsigned long long total) {
   const int t = threadIdx.x;

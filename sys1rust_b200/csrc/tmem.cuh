@@ -1,5 +1,5 @@
-// tcgen05 helpers of the attention kernels: the MN-major operand of the values, wide TMEM loads and stores, and the
-// product with its first operand in TMEM.
+// tcgen05 helpers of the attention kernels: the MN-major operand of the values, wide TMEM loads and stores,
+// and the product with its first operand in TMEM.
 #pragma once
 #include "common.cuh"
 

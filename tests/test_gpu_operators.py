@@ -83,7 +83,8 @@ def _act(y, act):
 @pytest.mark.parametrize("M,N,K,group", [
     (1, 1, 1, 32), (1, 7, 31, 32), (2, 16, 32, 64), (1, 64, 33, 128), (1, 1024, 1024, 128), (3, 130, 257, 32),
     (5, 1000, 2624, 64), (8, 33, 4097, 128), (9, 300, 640, 32), (16, 257, 1100, 64), (17, 129, 129, 128), (33, 65, 2047, 32),
-    (64, 200, 1024, 128), (64, 31, 5000, 64), (1, 5000, 96, 32), (4, 20000, 160, 64), (2, 48, 20000, 128)])
+    (64, 200, 1024, 128), (64, 31, 5000, 64), (1, 5000, 96, 32), (4, 20000, 160, 64), (2, 48, 20000, 128),
+    (8, 100, 9000, 32), (16, 70, 6001, 64), (12, 300, 8192, 128), (6, 40, 30000, 64), (3, 2400, 12000, 128)])
 def test_nibble_gemm(ops, M, N, K, group, dt):
     """Every combination of zero points, bias, activation and output type at one or another size. The
     error is the sum's, the zero point's and bias's place in it, and one rounding; GELU's slope is at most 1.13."""
@@ -344,12 +345,16 @@ def _attention(ops, c, q, heads, lens, keys, scale, window=-1, most=None, max_kv
 def _check_attention(c, q, heads, lens, keys, scale, window, out, lse):
     """Bounds: a score is off by at most d = (D + 8) 2^-22 of the sum of its products' magnitudes (fp32
     sum; q's scaling and the key's scale are roundings within it), which moves its weight by the factor 1 + 2 d; a
-    weight is rounded to 11 bits, summed over the keys, once; sums over L keys add L 2^-22; one rounding of the result."""
+    weight is rounded to 11 bits, summed over the keys, once; sums over L keys add L 2^-22; one rounding of the result.
+    Weights (times their page's value scale) are f16 with the largest at 2^14 or above, whose smallest step is 2^-24: one far below
+    the largest is off by up to 2^-39 of it, so each of the L keys adds 2^-39 of the largest weight times 128 at most."""
     G, base = heads // c.H, 0
     for i, (n, L) in enumerate(zip(lens, keys)):
         K, ok = c.rows(0, i, L)
         V, _ = c.rows(1, i, L)
         K, V, ok = K.cuda(), V.cuda(), ok.cuda()
+        at = (torch.arange(L, device="cuda") // c.page).clamp(max=c.table.shape[1] - 1)
+        vs = c.scales[1].double()[c.table[i].long().clamp(0, c.count - 1)[at]].nan_to_num(0.0)  # [L, H]
         x = q[base: base + n, : heads * c.D].double().view(n, heads, c.D)
         pos = torch.arange(L - n, L, device="cuda")[:, None]
         j = torch.arange(L, device="cuda")[None]
@@ -364,6 +369,8 @@ def _check_attention(c, q, heads, lens, keys, scale, window, out, lse):
             want, mass = p @ V[:, h // G], p @ V[:, h // G].abs()
             have = out[base: base + n, h * c.D: (h + 1) * c.D].double()
             bound = _u(q.dtype) * want.abs() + mass * (2.0 ** -11 + 4 * d[:, None] + (L + 64) * 2.0 ** -22) + torch.finfo(q.dtype).tiny
+            if L:
+                bound += L * 2.0 ** -39 * 128 * (p * vs[:, h // G]).amax(1)[:, None]
             err = (have - want).abs()
             assert (err <= bound).all(), (i, h, (err / bound).max().item())
             assert (have[none] == 0).all() and (lse[base: base + n, h][none] == -math.inf).all()
@@ -426,8 +433,59 @@ def test_cache_attention_past_its_table(ops):
     _check_attention(c, q, 2, lens, keys, 0.125, -1, out, lse)
 
 
+def test_cache_attention_replayed_with_other_lengths(ops):
+    """A captured call over a cache long enough to be split (so two kernels), replayed with other lengths and
+    tables, one of them an empty sequence."""
+    H, D, page, heads = 2, 128, 32, 4
+    c = Paged(ops, 2, 3000, H, D, page, 55)
+    q = torch.randn(2, heads * D, generator=_gen(56), device="cuda").half()
+    out = torch.full((3, heads * D + 8), 5.0, dtype=torch.float16, device="cuda")
+    lse = torch.full((3, heads), 5.0, device="cuda")
+    cu, ln = _i32([0, 1, 2]), _i32([3000, 17])
+    ws = torch.empty(ops.cache_attention_workspace(c.handle, heads, 2, 1, 3000), dtype=torch.uint8, device="cuda")
+    assert ws.numel() > 0
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def call():
+        ops.cache_attention(c.handle, ops.DT_F16, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), heads,
+                            cu.data_ptr(), ln.data_ptr(), c.table.data_ptr(), c.table.shape[1], 2, 1, 3000, 0.088,
+                            lse_ptr=lse.data_ptr(), workspace_ptr=ws.data_ptr(), workspace_bytes=ws.numel(), stream=_stream())
+
+    with torch.cuda.stream(side):
+        call()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            call()
+    for keys in ([3000, 17], [1, 2999], [0, 1500], [2048, 2049]):
+        ln.copy_(_i32(keys))
+        c.table.copy_(c.table.flip(0).clone())
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_attention(c, q, heads, [1, 1], keys, 0.088, -1, out, lse)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
-def test_cache_attention_scores_and_scales_far_apart(ops, dt):
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("D,H,G,lens,keys,window", [
+    (64, 2, 4, [40, 300, 7], [40, 1000, 700], -1), (128, 1, 8, [129, 16, 1], [500, 16, 3000], -1),
+    (128, 2, 3, [200, 90, 64], [900, 2500, 64], 500), (64, 1, 33, [1, 1, 4], [5000, 0, 2], -1)])
+def test_cache_attention_prompts(ops, D, H, G, lens, keys, window, page, dt):
+    """Many query rows: tiles of 128 rows that end inside a sequence, windows, pages of every size, and a
+    group so wide that one token's rows make a tile."""
+    c = Paged(ops, 3, max(keys) + 1, H, D, page, 57)
+    c.scales[1][::5] *= 20
+    c.table[0, 2] = -1
+    q = torch.randn(sum(lens), H * G * D, generator=_gen(58), device="cuda").to(DT[dt])
+    scale = 1 / math.sqrt(D)
+    out, lse = _attention(ops, c, q, H * G, lens, keys, scale, window)
+    _check_attention(c, q, H * G, lens, keys, scale, window, out, lse)
+
+
+@pytest.mark.parametrize("many", [0, 1])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_cache_attention_scores_and_scales_far_apart(ops, dt, many):
     """Scores in the hundreds that grow along the keys, queries from 2^-12 to 2^12, pages whose values are all zero
     (scale 0), value scales 2^16 apart."""
     H, D, page, heads = 2, 128, 16, 8
@@ -441,7 +499,7 @@ def test_cache_attention_scores_and_scales_far_apart(ops, dt):
             if p % 9 == 4:
                 c.scales[1][pid] = 0
                 c.codes[1][pid] = 0
-    lens, keys = [1, 4, 1], [600, 555, 16 * 5]
+    lens, keys = [[1, 4, 1], [1, 30, 12]][many], [600, 555, 16 * 5]
     q = torch.randn(sum(lens), heads * D, generator=_gen(62), device="cuda")
     q = (q * torch.exp2(torch.linspace(-12, 5, q.shape[0], device="cuda"))[:, None]).to(DT[dt])
     q[:, D: 2 * D] *= 2.0 ** -9

@@ -30,7 +30,7 @@ def _nibble(**kw):
 
 @pytest.mark.parametrize("bad,text", [
     (dict(dtype=ops.DT_F32), "dtype"), (dict(dtype=7), "dtype"), (dict(x_ptr=0), "null"), (dict(codes_ptr=0), "null"),
-    (dict(scales_ptr=0), "null"), (dict(out_ptr=0), "null"), (dict(M=65), "M must"), (dict(M=-1), "M must"),
+    (dict(scales_ptr=0), "null"), (dict(out_ptr=0), "null"), (dict(M=65), "M must"), (dict(M=-1), "M must"), (dict(N=(1 << 30) + 1), "M must"),
     (dict(N=0), "M must"), (dict(K=0), "M must"), (dict(group=48), "group"), (dict(group=0), "group"),
     (dict(code_pitch=24), "pitch"), (dict(code_pitch=16), "pitch"), (dict(codes_ptr=PTR + 8), "aligned"),
     (dict(x_stride=63), "stride"), (dict(out_stride=7), "stride"), (dict(scale_stride=1), "stride"), (dict(act=3), "act"),
