@@ -515,6 +515,9 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     }
   };
 
+  // another block's shared memory, for eight lanes at a time (repeating the last block's where there are fewer)
+  const auto of_block = [&](int i) { return cluster.map_shared_rank(&s, min(i % SMP_CLUSTER, blocks - 1)); };
+
   // 1. The largest logit; a NaN (which the maximum keeps) or +inf leaves no distribution.
   float top = -INFINITY;
 #pragma unroll 4
@@ -533,7 +536,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   if (blocks > 1) {
     if (t == 0) s.top = top;
     cluster.sync();
-    for (int i = 0; i < blocks; ++i) top = max_nan(top, cluster.map_shared_rank(&s, i)->top);
+    top = of_block(lane)->top;  // each lane asks one block
+    for (int o = 4; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   }
   top += 0.f;  // -0 and 0 are equal
   const bool none = !(top < INFINITY) || top == -INFINITY;
@@ -552,7 +556,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
       if (t == 0) s.at = at;
       cluster.sync();
       if (me == 0)
-        for (int i = 0; i < blocks; ++i) at = min(at, cluster.map_shared_rank(&s, i)->at);
+        at = (int)__reduce_min_sync(0xffffffffu, (uint32_t)of_block(lane)->at);
       cluster.sync();  // nobody leaves while others read it
     }
     if (t == 0 && me == 0) {
@@ -604,20 +608,18 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     if (blocks > 1) {
       if (t == 0) s.sum = total;
       cluster.sync();
-      unsigned long long sums_[SMP_CLUSTER];
-      uint4 counts[SMP_CLUSTER];
-#pragma unroll
-      for (int i = 0; i < SMP_CLUSTER; ++i) {  // all in flight together
-        const SampleShared* o = cluster.map_shared_rank(&s, min(i, blocks - 1));
-        sums_[i] = o->sum;
-        counts[i] = have ? *reinterpret_cast<const uint4*>(&o->count[PER * t]) : make_uint4(0, 0, 0, 0);
-      }
-      total = 0;
+      total = sums && lane < blocks ? of_block(lane)->sum : 0ull;
       all4 = make_uint4(0, 0, 0, 0);
+      if (__any_sync(0xffffffffu, have)) {
+        uint4 counts[SMP_CLUSTER];
 #pragma unroll
-      for (int i = 0; i < SMP_CLUSTER; ++i)
-        if (i < blocks)
-          total += sums_[i], all4.x += counts[i].x, all4.y += counts[i].y, all4.z += counts[i].z, all4.w += counts[i].w;
+        for (int i = 0; i < SMP_CLUSTER; ++i)  // all in flight together
+          counts[i] = have && i < blocks ? *reinterpret_cast<const uint4*>(&of_block(i)->count[PER * t]) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < SMP_CLUSTER; ++i) all4.x += counts[i].x, all4.y += counts[i].y, all4.z += counts[i].z, all4.w += counts[i].w;
+      }
+      for (int o = 4; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      total = __shfl_sync(0xffffffffu, total, 0);
     }
     const uint32_t own[PER] = {own4.x, own4.y, own4.z, own4.w}, all[PER] = {all4.x, all4.y, all4.z, all4.w};
     if (by_k || by_p) {
@@ -663,7 +665,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     if (blocks > 1 && list) {
       if (t == 0) s.listed = mine;
       cluster.sync();
-      for (int i = 0; i < me; ++i) before += cluster.map_shared_rank(&s, i)->listed;
+      before = __reduce_add_sync(0xffffffffu, lane < me ? of_block(lane)->listed : 0u);
     }
   }
 
