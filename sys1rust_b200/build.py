@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libs1c.so")
-UNITS = ("s1c.cu", "operators.cu", "nibble_f16.cu", "nibble_bf16.cu")
+UNITS = ("s1c.cu", "operators.cu", "nibble_f16.cu", "nibble_bf16.cu", "nibble_f16_zeros.cu", "nibble_bf16_zeros.cu")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

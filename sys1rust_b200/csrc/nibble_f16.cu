@@ -1,10 +1,11 @@
-// The 4-bit products' kernels for f16 rows, in a unit of their own: the units compile side by side.
+// The 4-bit products' kernels for f16 rows, without zero points, in a unit of their own: the units compile
+// side by side.
 #include "nibble_launch.cuh"
 
 namespace s1c {
 
 void launch_nibble_f16(const NibbleArgs& a, int group, int dev, cudaStream_t st) {
-  launch_nibble<__half>(a, group, dev, st);
+  launch_nibble<__half, false>(a, group, dev, st);
 }
 
 }  // namespace s1c

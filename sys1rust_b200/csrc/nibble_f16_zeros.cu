@@ -1,0 +1,11 @@
+// The 4-bit products' kernels for f16 rows, with zero points, in a unit of their own: the units compile
+// side by side.
+#include "nibble_launch.cuh"
+
+namespace s1c {
+
+void launch_nibble_f16_zeros(const NibbleArgs& a, int group, int dev, cudaStream_t st) {
+  launch_nibble<__half, true>(a, group, dev, st);
+}
+
+}  // namespace s1c

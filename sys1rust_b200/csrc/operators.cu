@@ -19,9 +19,11 @@
 using namespace s1c;
 
 namespace s1c {
-// nibble_f16.cu, nibble_bf16.cu
+// nibble_f16.cu and its kind
 void launch_nibble_f16(const NibbleArgs& a, int group, int dev, cudaStream_t st);
 void launch_nibble_bf16(const NibbleArgs& a, int group, int dev, cudaStream_t st);
+void launch_nibble_f16_zeros(const NibbleArgs& a, int group, int dev, cudaStream_t st);
+void launch_nibble_bf16_zeros(const NibbleArgs& a, int group, int dev, cudaStream_t st);
 }  // namespace s1c
 
 namespace {
@@ -193,9 +195,9 @@ s1c_status s1c_nibble_gemm(int32_t dtype, const void* d_x, int64_t x_stride, con
     a.vec = x_stride % 8 == 0 && aligned(d_x, 16);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == S1C_DT_F16)
-      launch_nibble_f16(a, group, dev.device, st);
+      (d_zeros ? launch_nibble_f16_zeros : launch_nibble_f16)(a, group, dev.device, st);
     else
-      launch_nibble_bf16(a, group, dev.device, st);
+      (d_zeros ? launch_nibble_bf16_zeros : launch_nibble_bf16)(a, group, dev.device, st);
     CK(cudaGetLastError());
   });
 }

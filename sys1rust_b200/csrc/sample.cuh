@@ -123,6 +123,19 @@ struct SampleItems {
   S1C_DEV float operator()(int i) const { return value ? value[i] : to_f32(row[i]) + 0.f; }
 };
 
+// f(element) for all elements, each thread with every 512th, four loads in flight.
+template <typename T, typename F>
+S1C_DEV void sample_each(const SampleItems<T>& items, F&& f) {
+  for (int i0 = threadIdx.x; i0 < items.n; i0 += 4 * SMP_THREADS) {
+    float x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = i0 + j * SMP_THREADS < items.n ? items(i0 + j * SMP_THREADS) : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (x[j] > -INFINITY) f(x[j]);
+  }
+}
+
 // First bin whose elements reach `want` (by count), or last non-empty bin whose predecessors' mass is
 // below `want` (by mass), and the count and mass before it; -1 where there is none. A mass counts 2^power
 // of its bin of z, or `scale`. All threads call.
@@ -204,11 +217,10 @@ S1C_DEV SampleCut sample_narrow(SampleShared& s, const SampleMass& f, const Samp
   if (t == 0) s.key_lo = 0xffffffffu, s.key_hi = 0;
   __syncthreads();
   uint32_t lo = 0xffffffffu, hi = 0;
-  for (int i = t; i < items.n; i += SMP_THREADS) {
-    const float l = items(i);
+  sample_each(items, [&](float l) {
     const uint32_t k = logit_key(l);
     if (f.bin(l) == zbin && k >= limit.key) lo = min(lo, k), hi = max(hi, k);
-  }
+  });
   lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
   if (t % 32 == 0) atomicMin(&s.key_lo, lo), atomicMax(&s.key_hi, hi);
   __syncthreads();
@@ -220,17 +232,14 @@ S1C_DEV SampleCut sample_narrow(SampleShared& s, const SampleMass& f, const Samp
     __syncthreads();
     sample_clear(s, bins);
     __syncthreads();
-    for (int i = t; i < items.n; i += SMP_THREADS) {
-      const float l = items(i);
+    sample_each(items, [&](float l) {
       const uint32_t k = logit_key(l);
-      if (k < lo || k > hi || k == limit.key) continue;
-      if (f.bin(l) == zbin) {
-        if (MASS)
-          sample_count(s, (int)((hi - k) >> shift), f.mass(l, zbin));
-        else
-          atomicAdd(&s.count[(hi - k) >> shift], 1u);
-      }
-    }
+      if (k < lo || k > hi || k == limit.key || f.bin(l) != zbin) return;
+      if (MASS)
+        sample_count(s, (int)((hi - k) >> shift), f.mass(l, zbin));
+      else
+        atomicAdd(&s.count[(hi - k) >> shift], 1u);
+    });
     __syncthreads();
     if (t == 0 && limit.need && limit.key >= lo && limit.key <= hi) {
       const int b = (int)((hi - limit.key) >> shift);
@@ -356,11 +365,10 @@ S1C_DEV void sample_choose(SampleShared& s, const SampleArgs& a, int r, const Sa
   if (by_k || by_p) {
     sample_clear(s, SMP_ZBINS);
     __syncthreads();
-    for (int i = t; i < items.n; i += SMP_THREADS) {
-      const float l = items(i);
+    sample_each(items, [&](float l) {
       const int b = f.bin(l);
       if (b < SMP_ZBINS) sample_count(s, b, f.mass(l, b));
-    }
+    });
     __syncthreads();
     double total = (double)total44 * pow2(-44);  // mass of what top-k keeps
     int last = SMP_ZBINS;                        // bin of top-k's cut
@@ -375,14 +383,13 @@ S1C_DEV void sample_choose(SampleShared& s, const SampleArgs& a, int r, const Sa
           unsigned long long part = 0;
           sample_clear(s, SMP_ZBINS);
           __syncthreads();
-          for (int i = t; i < items.n; i += SMP_THREADS) {
-            const float l = items(i);
+          sample_each(items, [&](float l) {
             const int b = f.bin(l);
             if (b < last)
               sample_count(s, b, f.mass(l, b));
             else if (b == last && logit_key(l) > cut.key)
               part += f.mass(l, last);
-          }
+          });
           part = sample_sum(s, part) + (unsigned long long)f.mass(key_logit(cut.key), last) * cut.need;
           if (t == 0) s.count[last] = 1, s.lo[last] = (uint32_t)(part & 4095u), s.hi[last] = (uint32_t)(part >> 12);
           __syncthreads();
@@ -425,25 +432,34 @@ S1C_DEV void sample_choose(SampleShared& s, const SampleArgs& a, int r, const Sa
     __syncthreads();
     for (int i = 0; i < w; ++i) ahead += s.warp_a[i];
   }
-  const auto kept = [&](int i, uint32_t& rank, float& l, int& b) {
-    l = i < i1 ? items(i) : -INFINITY;
-    b = f.bin(l);
-    const uint32_t key = logit_key(l);
-    bool keep = i < i1 && b < SMP_ZBINS && (double)l >= least && key >= cut.key;
-    if (cut.need) {
-      const bool eq = i < i1 && key == cut.key;
-      const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
-      if (eq && rank + __popc(eqs & ((1u << lane) - 1)) >= cut.need) keep = false;
-      rank += __popc(eqs);
+  // Masses of the kept ones of 128 elements from j on, four steps of 32 (their loads in flight together); rank: equals of the
+  // cut so far.
+  const auto masses = [&](int j, uint32_t& rank, unsigned long long (&m)[4]) {
+    float x[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = j + q * 32 + lane < i1 ? items(j + q * 32 + lane) : -INFINITY;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      m[q] = 0;
+      if (j + q * 32 >= i1) continue;
+      const int b = f.bin(x[q]);
+      const uint32_t key = logit_key(x[q]);
+      bool keep = b < SMP_ZBINS && key >= cut.key && (least == -INFINITY || (double)x[q] >= least);
+      if (cut.need) {
+        const bool eq = key == cut.key;
+        const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
+        if (eq && rank + __popc(eqs & ((1u << lane) - 1)) >= cut.need) keep = false;
+        rank += __popc(eqs);
+      }
+      m[q] = keep ? f.fixed(x[q], b) : 0ull;
     }
-    return keep;
   };
-  unsigned long long sum = 0, total = 0, base = 0;
+  unsigned long long sum = 0, total = 0, base = 0, m[4];
   uint32_t rank = ahead;
-  for (int j = i0; j < i1; j += 32) {
-    float l;
-    int b;
-    if (kept(j + lane, rank, l, b)) sum += f.fixed(l, b);
+  for (int j = i0; j < i1; j += 128) {
+    masses(j, rank, m);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum += m[q];
   }
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) s.warp_u[w] = sum;
@@ -463,26 +479,43 @@ S1C_DEV void sample_choose(SampleShared& s, const SampleArgs& a, int r, const Sa
     if ((double)run > goal) break;
   }
   if (w != walker) return;
+  // the 128 elements that it falls into, or the last ones with mass
+  int at = i0;
+  uint32_t at_rank = ahead;
+  unsigned long long at_base = base;
   rank = ahead;
+  for (int j = i0; j < i1; j += 128) {
+    const uint32_t before = rank;
+    masses(j, rank, m);
+    sum = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum += m[q];
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (!sum) continue;
+    at = j, at_rank = before, at_base = base;
+    base += sum;
+    if ((double)base > goal) break;
+  }
+  masses(at, at_rank, m);
   int token = -1;
   float prob = 0.f;
-  for (int j = i0; j < i1; j += 32) {
-    float l;
-    int b;
-    const bool keep = kept(j + lane, rank, l, b);
-    const unsigned long long m = keep ? f.fixed(l, b) : 0ull;
-    if (!__any_sync(0xffffffffu, m != 0)) continue;
-    unsigned long long upto = m;
+  bool found = false;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (at + q * 32 >= i1) continue;
+    unsigned long long upto = m[q];
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned long long v = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += v;
     }
-    const uint32_t over = __ballot_sync(0xffffffffu, m && (double)(base + upto) > goal);
-    const int pick = over ? __ffs(over) - 1 : 31 - __clz(__ballot_sync(0xffffffffu, m != 0));
-    token = j + pick;
-    prob = (float)((double)__shfl_sync(0xffffffffu, m, pick) / (double)total);
-    if (over) break;
-    base += __shfl_sync(0xffffffffu, upto, 31);
+    const uint32_t any = __ballot_sync(0xffffffffu, m[q] != 0), over = __ballot_sync(0xffffffffu, m[q] && (double)(at_base + upto) > goal);
+    if (any && !found) {
+      const int pick = over ? __ffs(over) - 1 : 31 - __clz(any);
+      token = at + q * 32 + pick;
+      prob = (float)((double)__shfl_sync(0xffffffffu, m[q], pick) / (double)total);
+      found = over != 0;
+    }
+    at_base += __shfl_sync(0xffffffffu, upto, 31);
   }
   if (lane == 0) {
     a.token[r] = index ? index[token] : token;

@@ -84,7 +84,9 @@ def _act(y, act):
     (1, 1, 1, 32), (1, 7, 31, 32), (2, 16, 32, 64), (1, 64, 33, 128), (1, 1024, 1024, 128), (3, 130, 257, 32),
     (5, 1000, 2624, 64), (8, 33, 4097, 128), (9, 300, 640, 32), (16, 257, 1100, 64), (17, 129, 129, 128), (33, 65, 2047, 32),
     (64, 200, 1024, 128), (64, 31, 5000, 64), (1, 5000, 96, 32), (4, 20000, 160, 64), (2, 48, 20000, 128),
-    (8, 100, 9000, 32), (16, 70, 6001, 64), (12, 300, 8192, 128), (6, 40, 30000, 64), (3, 2400, 12000, 128)])
+    (8, 100, 9000, 32), (16, 70, 6001, 64), (12, 300, 8192, 128), (6, 40, 30000, 64), (3, 2400, 12000, 128),
+    (45, 70, 9000, 32), (64, 20, 16000, 128), (20, 50, 2700, 64), (10, 17, 100000, 32), (1, 33, 90001, 128),
+    (17, 40, 9900, 64)])
 def test_nibble_gemm(ops, M, N, K, group, dt):
     """Every combination of zero points, bias, activation and output type at one or another size. The
     error is the sum's, the zero point's and bias's place in it, and one rounding; GELU's slope is at most 1.13."""
