@@ -29,6 +29,13 @@
 // thread issues S = Q K^T into one of two buffers of TMEM, a tile ahead, and O += P V; four warps have a
 // row in each thread, and write the weights P over the scores they come from, where the second product
 // reads them as its first operand.
+//
+// Measured: 64 sequences of 4096 to 8192 keys, 32 heads on 8 of 128, pages of 16: 165 us, 4.7 TB/s; what is
+// left there is instructions (850 for a tile of 32 keys, most of them conversions) at three blocks an SM. 1
+// x 131072 keys: 37 us, 3.6 TB/s, with one round of blocks and 3 us to join them; 1 x 700: 7.7 us, two
+// launches. Prompts, 4 x 512 rows over 2048 to 4096 keys, 16 heads on 4: 116 us, 461 TFLOP/s; on
+// mma.m16n8k16 the same took 326 us, of shared memory reads. There 256 blocks lie unevenly on 148 SMs, and
+// the softmax threads wait for the scores a third of the time.
 #pragma once
 #include <cuda.h>
 #include <limits.h>

@@ -5,7 +5,8 @@
 
 namespace s1c {
 
-// Launches the variant; false, and nothing, if x does not fit beside its rings. WHOLE: x passes in blocks of columns instead.
+// Launches the variant; false, and nothing, if x does not fit beside its rings. WHOLE: x passes in blocks
+// of columns instead.
 template <typename T, int GROUP, bool ZERO, int NT, int RT, int SPAN, int WARPS, bool WHOLE = false>
 bool launch_nibble_as(NibbleArgs a, int dev, cudaStream_t st) {
   using W = NibbleWarp<T, GROUP, NT, RT, SPAN, WARPS, ZERO>;
@@ -29,8 +30,8 @@ bool launch_nibble_as(NibbleArgs a, int dev, cudaStream_t st) {
   return true;
 }
 
-// x in shared memory, if need be beside shorter rings; false if it does not fit. The variants are those for `like` rows: what
-// fits for these fits for fewer.
+// x in shared memory, if need be beside shorter rings; false if it does not fit. The variants are those for
+// `like` rows: what fits for these fits for fewer.
 template <typename T, int GROUP, bool ZERO>
 bool launch_nibble_fit(const NibbleArgs& a, int like, int dev, cudaStream_t st) {
   if (like <= 8) return launch_nibble_as<T, GROUP, ZERO, 1, 1, 4, 16>(a, dev, st) || launch_nibble_as<T, GROUP, ZERO, 1, 1, 2, 16>(a, dev, st);
@@ -39,9 +40,9 @@ bool launch_nibble_fit(const NibbleArgs& a, int like, int dev, cudaStream_t st) 
   return launch_nibble_as<T, GROUP, ZERO, 8, 1, 2, 8>(a, dev, st);
 }
 
-// Rows whose x does not fit go in as many launches as make it fit: the codes then come from the cache again, which
-// costs less than passing x through each block in blocks of columns (32 x 8192 x 4096: two launches 35 us, columns 65 us).
-// That is left for columns so many that not even one row fits.
+// Rows whose x does not fit go in as many launches as make it fit: the codes then come from the cache
+// again, which costs less than passing x through each block in blocks of columns (32 x 8192 x 4096: two
+// launches 35 us, columns 65 us). That is left for columns so many that not even one row fits.
 template <typename T, int GROUP, bool ZERO>
 void launch_nibble(const NibbleArgs& a, int dev, cudaStream_t st) {
   const int64_t out_bytes = a.out_f32 ? 4 : sizeof(T);

@@ -20,6 +20,11 @@
 // Masses are integers: e = m * 2^(n - 24), m an integer of 25 bits, and all e in one bin share n. So their
 // sums are exact and depend neither on the order of atomics nor on how a row is shared. Logits more than 45
 // powers of two below the largest have no mass.
+//
+// Measured: 1 x 50368 fp32, top-k 50 and top-p: 17.6 us, of which the exchanges of the eight blocks are
+// about half; 256 x 50368 bf16, top-p and min-p: 49 us, where the pass that counts and sums (25 instructions
+// a logit) is a third. Without a list (64 x 131072, no filter) 124 us. Not kept: a row in shared memory and
+// one block of 1024 threads an SM (65 us for the 256 rows).
 #pragma once
 #include <cooperative_groups.h>
 
@@ -432,8 +437,8 @@ S1C_DEV void sample_choose(SampleShared& s, const SampleArgs& a, int r, const Sa
     __syncthreads();
     for (int i = 0; i < w; ++i) ahead += s.warp_a[i];
   }
-  // Masses of the kept ones of 128 elements from j on, four steps of 32 (their loads in flight together); rank: equals of the
-  // cut so far.
+  // Masses of the kept ones of 128 elements from j on, four steps of 32 (their loads in flight together);
+  // rank: equals of the cut so far.
   const auto masses = [&](int j, uint32_t& rank, unsigned long long (&m)[4]) {
     float x[4];
 #pragma unroll
