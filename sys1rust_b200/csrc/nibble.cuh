@@ -274,7 +274,7 @@ struct NibbleWarp {
         for (int j = 0; j < NT; ++j) {
           const int m = 8 * j + 2 * c + e % 2;
           if (m >= a.M) continue;
-          float y = total[r][j][e] * 0x1p24f * row_scale[m];
+          float y = total[r][j][e] * (fminf(row_scale[m], 1.f) * 0x1p24f) * fmaxf(row_scale[m], 1.f);  // nothing in between underflows
           if (a.bias) y += b;
           if (a.act == 1) y = y < 0.f ? 0.f : y;  // keeps NaN
           if (a.act == 2) y = 0.5f * y * (1.f + erff(y * 0.70710678118654752f));
@@ -327,7 +327,7 @@ S1C_DEV void nibble_stage(const NibbleArgs& a, __half* xs, float* sums, float* r
   for (int p = w; p < a.M * parts; p += WARPS) {
     const int m = p / parts, s0 = p % parts * passes / parts, s1 = (p % parts + 1) * passes / parts;
     // 2^up brings the largest value to [2^14, 2^15); rows with an infinity or NaN keep theirs
-    const int e = (int)(tops[m] >> 23) - 127, up = e == 128 ? 0 : min(14 - e, 100);
+    const int e = (int)(tops[m] >> 23) - 127, up = e == 128 ? 0 : min(14 - e, 126);
     const float by = __uint_as_float((uint32_t)(127 + up) << 23);
     if (lane == 0) row_scale[m] = __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll 2

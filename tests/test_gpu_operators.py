@@ -137,6 +137,23 @@ def test_nibble_gemm_extreme_codes_and_values(ops):
     assert torch.isnan(out2[1][keep]).all() and not torch.isfinite(out2[2][keep]).any()
 
 
+def test_nibble_gemm_rows_far_from_one(ops):
+    """bf16 rows from 2^-124 (subnormal values among them) to 2^120 keep the bound of the sum: the rows' scaling and
+    its undoing leave the range of fp32 nowhere; with few columns, in several launches, and in pieces."""
+    for K, rows in [(256, 7), (9000, 7), (100000, 7)]:
+        x, codes, scales, _ = _nibble_inputs(rows, 40, K, 128, torch.bfloat16, False, 9)
+        for m, p in enumerate([-124, -120, -112, -90, -40, 40, 110]):
+            x[m] = (x[m].double() * 2.0 ** p).to(torch.bfloat16)
+        out = torch.empty(rows, 40, device="cuda")
+        _nibble(ops, x, codes, scales, None, out, K, 128)
+        ref = x.double() @ _nibble_weights(codes, scales, None, K, 128).t()
+        mag = x.double().abs() @ (scales.double()[:, torch.arange(K, device="cuda") // 128] * 30).t()
+        # as in test_nibble_gemm; results below the normal range are stored to 2^-149
+        bound = (K + 64) * 2.0 ** -22 * mag + _u(torch.float32) * ref.abs() + 2.0 ** -149
+        err = (out.double() - ref).abs()
+        assert (err <= bound).all(), (K, (err / bound).max(1).values)
+
+
 def test_nibble_gemm_is_bitwise_repeatable_and_row_independent(ops):
     """The same call gives the same bits; the packer's codes give its weights' products."""
     x, codes, scales, z = _nibble_inputs(7, 515, 3001, 64, torch.bfloat16, True, 9)
@@ -845,3 +862,66 @@ def test_host_memory_is_refused(ops):
     out = torch.zeros(1, 8, dtype=torch.float16)
     with pytest.raises(BackendError, match="device memory"):
         _nibble(ops, x, codes, scales, None, out, 64, 32)
+
+
+_FIRST_CALLS = """
+import sys, torch
+from sys1rust_b200 import operators as ops
+g = torch.Generator(device="cuda").manual_seed(1)
+dev = dict(device="cuda")
+x = torch.randn(3, 256, generator=g, **dev).half()
+codes = torch.randint(0, 256, (64, 128), generator=g, dtype=torch.uint8, **dev)
+scales = torch.rand(64, 2, generator=g, **dev).half()
+y = torch.zeros(3, 64, dtype=torch.half, **dev)
+page, heads, dim, count = 16, 2, 64, 300
+kc, vc = torch.zeros(count, heads, page, dim, dtype=torch.int8, **dev), torch.zeros(count, heads, page, dim, dtype=torch.int8, **dev)
+ks, vs = torch.zeros(count, heads, **dev), torch.zeros(count, heads, **dev)
+cache = ops.Cache(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), count, page, heads, dim)
+L = 4000
+k, v = (torch.randn(L, heads * dim, generator=g, **dev).half() for _ in range(2))
+rk, rv = torch.zeros_like(k), torch.zeros_like(v)
+cu, zero, last = (torch.tensor(t, dtype=torch.int32, **dev) for t in ([0, L], [0], [L]))
+table = torch.randperm(count, generator=g, **dev)[:250].int()
+qs = {n: (torch.randn(n, 8 * dim, generator=g, **dev).half(), torch.zeros(n, 8 * dim, dtype=torch.half, **dev),
+          torch.tensor([0, n], dtype=torch.int32, **dev)) for n in (1, 40)}
+space = torch.zeros(max(ops.cache_attention_workspace(cache, 8, 1, n, L) for n in qs) + 16, dtype=torch.uint8, **dev)
+logits = torch.randn(2, 5000, generator=g, **dev)
+u = torch.rand(2, generator=g, **dev)
+token = torch.zeros(2, dtype=torch.int32, **dev)
+
+def run():
+    st = torch.cuda.current_stream().cuda_stream
+    ops.nibble_gemm(ops.DT_F16, x.data_ptr(), 256, codes.data_ptr(), 128, scales.data_ptr(), 2, y.data_ptr(), 64, 3, 64, 256, 128, stream=st)
+    rows = (heads * dim, v.data_ptr(), heads * dim, cu.data_ptr(), zero.data_ptr(), table.data_ptr(), 250, 1, L)
+    ops.cache_write(cache, ops.DT_F16, k.data_ptr(), *rows, stream=st)
+    ops.cache_read(cache, ops.DT_F16, rk.data_ptr(), heads * dim, rv.data_ptr(), *rows[2:], stream=st)
+    for n, (q, o, at) in qs.items():
+        ops.cache_attention(cache, ops.DT_F16, q.data_ptr(), 8 * dim, o.data_ptr(), 8 * dim, 8, at.data_ptr(), last.data_ptr(),
+                            table.data_ptr(), 250, 1, n, L, 0.125, workspace_ptr=space.data_ptr(), workspace_bytes=space.numel(), stream=st)
+    ops.sample(ops.DT_F32, logits.data_ptr(), 5000, 2, 5000, token.data_ptr(), u.data_ptr(), stream=st)
+
+outs = [y, kc, vc, ks, vs, rk, rv, token] + [o for _, o, _ in qs.values()]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    run()
+graph.replay()
+torch.cuda.synchronize()
+captured = [t.clone() for t in outs]
+for t in outs:
+    t.zero_()
+run()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(captured, outs))
+assert all(t.any() for t in outs)
+"""
+
+
+def test_first_calls_of_a_process_can_be_captured(ops):
+    """Each operator's first call, which sets its kernels up, inside a stream capture; the replayed graph
+    computes what the calls do."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", _FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stderr[-2000:]
