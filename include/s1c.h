@@ -261,8 +261,8 @@ S1C_API int64_t s1c_last_launch_count(const s1c_backend* b);
  * on the device that holds its output, enqueues its work on `stream` (a cudaStream_t of that device, NULL =
  * legacy default stream), allocates nothing, does not synchronise and can be captured into a CUDA graph.
  * Device-side integers (offsets, lengths, page tables) are read when the kernels run, so a graph replays
- * with other lengths below the same bounds. `dtype` is an S1C_DT_ code; strides count elements. Results do
- * not change from one call to the next. */
+ * with other lengths below the same bounds. `dtype` is an S1C_DT_ code; strides count elements; pointers are
+ * aligned to their element type at least. Results do not change from one call to the next. */
 
 /* out[m, n] = act( sum_g s[n, g] * sum_{k in g} (q[n, k] - z[n, g]) * x[m, k] + bias[n] ): M rows x
  * [M, K] (0 to 64) times a matrix [N, K] held as 4-bit codes q. Column k of row n is the low (even k) or
@@ -270,7 +270,8 @@ S1C_API int64_t s1c_last_launch_count(const s1c_backend* b);
  * codes, whose padding is read and ignored. Each group of 32, 64 or 128 columns of a row has a scale s
  * and, where d_zeros is given, a zero point z (8 otherwise), in [N, ceil(K / group)] arrays of row
  * stride scale_stride. x, scales, zeros and out are F16 or BF16 (dtype); out_f32 = 1 makes out fp32.
- * bias (fp32) is nullable; act 0 none, 1 ReLU, 2 GELU. Sums are held in fp32. */
+ * bias (fp32) is nullable; act 0 none, 1 ReLU, 2 GELU. Sums are held in fp32. A row of x with an infinity or
+ * NaN gives NaN or infinities, in that row only. */
 S1C_API s1c_status s1c_nibble_gemm(int32_t dtype, const void* d_x, int64_t x_stride, const void* d_codes,
                                    int64_t code_pitch, const void* d_scales, const void* d_zeros, int64_t scale_stride,
                                    int32_t group, void* d_out, int64_t out_stride, int32_t M, int32_t N, int32_t K,
@@ -298,8 +299,8 @@ typedef struct s1c_cache {
  * rounded half to even, and where s grew, the earlier rows' codes become code * s_old / s rounded half to
  * even, both of the exact quotient. Infinities become +-127 and NaN 0, and neither counts in the maximum.
  * Rows behind the last new one are left as they were. Rows whose page is not in [0, num_pages), or whose
- * position is past the table, are dropped. A page written for two sequences in one call ends with
- * unspecified codes. */
+ * position is past the table, are dropped. A page that one call writes
+ * for two sequences, or at two places of one table row, ends with unspecified codes and scale. */
 S1C_API s1c_status s1c_cache_write(const s1c_cache* cache, int32_t dtype, const void* d_k, int64_t k_stride,
                                    const void* d_v, int64_t v_stride, const int32_t* d_cu, const int32_t* d_start,
                                    const int32_t* d_pages, int32_t max_pages, int32_t n, int32_t max_new, void* stream);

@@ -34,6 +34,12 @@ void need(bool ok, const char* what) {
 
 bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
+// Pointers (null ones are) to elements of `bytes` that lie where such elements may.
+template <typename... P>
+void need_elements(size_t bytes, const P*... p) {
+  need(((reinterpret_cast<uintptr_t>(p) % bytes == 0) && ...), "a pointer is not aligned to its element type");
+}
+
 // Makes the device that holds `p` current for the call, so that a caller with several devices needs no
 // cudaSetDevice; put back at the end. Host memory that the device cannot be shown to reach is refused.
 struct OnDeviceOf {
@@ -80,6 +86,7 @@ CacheView check_cache(const s1c_cache* c) {
   need(c->page == 16 || c->page == 32 || c->page == 64, "page must be 16, 32 or 64");
   need(c->head_dim == 64 || c->head_dim == 128, "head_dim must be 64 or 128");
   need(aligned(c->k_codes, 16) && aligned(c->v_codes, 16), "cache codes must be 16-byte aligned");
+  need_elements(4, c->k_scales, c->v_scales);
   need((int64_t)c->num_pages * c->kv_heads * c->page <= INT_MAX, "num_pages * kv_heads * page must stay below 2^31");
   return CacheView{{static_cast<int8_t*>(c->k_codes), static_cast<int8_t*>(c->v_codes)}, {c->k_scales, c->v_scales},
                    c->num_pages, c->page, c->kv_heads, c->head_dim};
@@ -92,6 +99,7 @@ CacheRows check_rows(const CacheView& c, const void* k, int64_t k_stride, const 
   need(k_stride >= (int64_t)c.heads * c.dim && v_stride >= (int64_t)c.heads * c.dim && k_stride % 8 == 0 && v_stride % 8 == 0,
        "row strides must hold kv_heads * head_dim values and be multiples of 8");
   need(aligned(k, 16) && aligned(v, 16), "rows must be 16-byte aligned");
+  need_elements(4, cu, start, table);
   CacheRows r{};
   r.rows[0] = const_cast<void*>(k), r.rows[1] = const_cast<void*>(v);
   r.stride[0] = k_stride, r.stride[1] = v_stride;
@@ -187,6 +195,9 @@ s1c_status s1c_nibble_gemm(int32_t dtype, const void* d_x, int64_t x_stride, con
     need(code_pitch % 16 == 0 && code_pitch >= ((int64_t)K + 31) / 32 * 16 && aligned(d_codes, 16),
          "codes must be 16-byte aligned, their row pitch a multiple of 16 bytes that holds K rounded up to 32 codes");
     need(x_stride >= K && out_stride >= N && scale_stride >= groups, "a row stride is shorter than its row");
+    need_elements(2, d_x, d_scales, d_zeros);
+    need_elements(4, d_bias);
+    need_elements(out_f32 ? 4 : 2, d_out);
     need(act >= 0 && act <= 2, "act must be 0 (none), 1 (ReLU) or 2 (GELU)");
     if (M == 0) return;
     OnDeviceOf dev(d_out);
@@ -271,6 +282,7 @@ s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, const void
     need(q_stride >= width && out_stride >= width && q_stride % 8 == 0 && out_stride % 8 == 0 && aligned(d_q, 16) && aligned(d_out, 16),
          "q and out must be 16-byte aligned, their row strides multiples of 8 that hold heads * head_dim values");
     need(std::isfinite(scale), "scale must be finite");
+    need_elements(4, d_lse, d_cu, d_len, d_pages);
     if (n == 0 || max_q == 0) return;
     need((int64_t)n * max_q <= INT_MAX / heads, "n * max_q * heads must stay below 2^31");
     const AttnPlan p = plan_attention(c, heads, n, max_q, max_kv);
@@ -301,6 +313,8 @@ s1c_status s1c_sample(int32_t dtype, const void* d_logits, int64_t row_stride, i
     need(rows >= 0 && vocab > 0 && vocab <= (1 << 18), "rows must not be negative, vocab 1 to 2^18");
     need(rows <= INT_MAX / SMP_CLUSTER, "too many rows");
     need(row_stride >= vocab, "a row stride is shorter than its row");
+    need_elements(dtype == S1C_DT_F32 ? 4 : 2, d_logits);
+    need_elements(4, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_token, d_prob);
     if (rows == 0) return;
     OnDeviceOf dev(d_token);
     SampleArgs a{d_logits, row_stride, vocab, d_temperature, d_top_k, d_top_p, d_min_p, d_uniform, d_token, d_prob};

@@ -41,7 +41,10 @@ def nibble_pack(w: np.ndarray, group: int, scale_dtype=np.float32):
     padded = np.zeros((N, groups * group), dtype=np.float32)
     padded[:, :K] = w
     parts = padded.reshape(N, groups, group)
-    scales = (np.abs(parts).max(2) / 7).astype(scale_dtype)
+    with np.errstate(over="ignore"):
+        scales = (np.abs(parts).max(2) / 7).astype(scale_dtype)
+    if not np.isfinite(scales).all():
+        raise BackendError(S1C_ERR_ARG, "nibble_pack: a group's scale does not fit scale_dtype")
     div = np.where(scales > 0, scales, 1).astype(np.float64)
     codes = np.clip(np.rint(parts / div[:, :, None]), -7, 7).astype(np.int8).reshape(N, -1) + 8
     pitch = -(-K // 32) * 16

@@ -122,6 +122,33 @@ def test_sample_refuses(bad, text):
     _refused(ops.sample, text=text, **a)
 
 
+def test_pointers_off_their_element_type_are_refused():
+    """An odd address of 16-bit elements, or one off by two of 32-bit ones, would fault on the GPU."""
+    bad = dict(text="element type")
+    for name, by in [("x_ptr", 1), ("scales_ptr", 1), ("zeros_ptr", 1), ("bias_ptr", 2), ("out_ptr", 1)]:
+        _refused(ops.nibble_gemm, **bad, **_nibble(**{name: PTR + by}))
+    _refused(ops.nibble_gemm, **bad, **_nibble(out_ptr=PTR + 2, out_f32=True))
+    for name in ("k_scales_ptr", "v_scales_ptr"):
+        c = _cache(**{name: PTR + 2})
+        _refused(ops.cache_write, max_new=1, **bad, **_rows(cache=c))
+        _refused(ops.cache_read, max_rows=1, **bad, **_rows(cache=c))
+        _refused(ops.cache_attention, **bad, **_attend(cache=c))
+    for name in ("cu_ptr", "start_ptr", "pages_ptr"):
+        _refused(ops.cache_write, max_new=1, **bad, **_rows(**{name: PTR + 2}))
+        _refused(ops.cache_read, max_rows=1, **bad, **_rows(**{name: PTR + 2}))
+    for name in ("lse_ptr", "cu_ptr", "len_ptr", "pages_ptr"):
+        _refused(ops.cache_attention, **bad, **_attend(**{name: PTR + 2}))
+    a = dict(dtype=ops.DT_F32, logits_ptr=PTR, row_stride=10, rows=1, vocab=10, token_ptr=PTR, uniform_ptr=PTR)
+    for name in ("logits_ptr", "token_ptr", "uniform_ptr", "temperature_ptr", "top_k_ptr", "top_p_ptr", "min_p_ptr", "prob_ptr"):
+        _refused(ops.sample, **bad, **{**a, name: PTR + 2})
+    _refused(ops.sample, **bad, **{**a, "dtype": ops.DT_BF16, "logits_ptr": PTR + 1})
+
+
+def test_nibble_pack_refuses_scales_that_do_not_fit():
+    with pytest.raises(BackendError):
+        ops.nibble_pack(np.full((1, 32), 1e6), 32, scale_dtype=np.float16)  # 142857 is past f16
+
+
 def test_calls_without_rows_do_nothing():
     """No rows: accepted without touching the GPU."""
     ops.nibble_gemm(**_nibble(M=0))
