@@ -13,13 +13,15 @@
 //  2. the counts of the logits in bins of z, 1/32 of a power of two wide, and where top-p needs it the exact
 //     mass of all, give a bin below which nothing can be kept;
 //  3. what stands above is gathered in the order of the indexes in the first block. Up to 512 of them are
-//     sorted, one by each thread. More have their thresholds found by histograms over bins of z and, inside the bin that holds the cut, over the order-preserving integer
-//     of the logit, 2048 ways at a time, until one value is left. What is kept is summed and walked. More
-//     than fit in the list are worked on in place.
+//     sorted, one by each thread. More have their thresholds found by histograms over bins of z and, inside
+//     the bin that holds the cut, over the order-preserving integer of the logit, 2048 ways at a time, until
+//     one value is left. What is kept is summed and walked. More than fit in the list are worked on in place.
 //
 // Masses are integers: e = m * 2^(n - 24), m an integer of 25 bits, and all e in one bin share n. So their
-// sums are exact and depend neither on the order of atomics nor on how a row is shared. Logits more than 45
-// powers of two below the largest have no mass.
+// sums are exact and depend neither on the order of atomics nor on how a row is shared. One sum is not of
+// this kind: where top-p counts the mass of a whole row, what lies below 1/16 of the largest is summed in
+// fp32 by each thread first, in a fixed order. Logits more than 45 powers of two below the largest have no
+// mass.
 //
 // Measured: 1 x 50368 fp32, top-k 50 and top-p: 17.6 us, of which the exchanges of the eight blocks are
 // about half; 256 x 50368 bf16, top-p and min-p: 49 us, where the pass that counts and sums (25 instructions
