@@ -32,7 +32,7 @@
 //
 // Measured: 64 sequences of 4096 to 8192 keys, 32 heads on 8 of 128, pages of 16: 165 us, 4.7 TB/s; what is
 // left there is instructions (850 for a tile of 32 keys, most of them conversions) at three blocks an SM. 1
-// x 131072 keys: 37 us, 3.6 TB/s, with one round of blocks and 3 us to join them; 1 x 700: 7.7 us, two
+// x 131072 keys: 36 us, 3.7 TB/s, with one round of blocks and 3 us to join them; 1 x 700: 7.9 us, two
 // launches. Prompts, 4 x 512 rows over 2048 to 4096 keys, 16 heads on 4: 116 us, 461 TFLOP/s; on
 // mma.m16n8k16 the same took 326 us, of shared memory reads. There 256 blocks lie unevenly on 148 SMs, and
 // the softmax threads wait for the scores a third of the time.
@@ -316,6 +316,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   constexpr int QK = D / 16, SEG = D / 32;
   const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, g = lane >> 2, cq = lane & 3;
   pdl_trigger();
+  pdl_wait();
   AttnUnit u;
   if (!attn_unit<16, CATT_TK>(c, a, u)) return;
   float v_top = 0.f;
@@ -474,6 +475,7 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   S& sm = *reinterpret_cast<S*>(raw + (1024 - smem_u32(raw) % 1024) % 1024);
   const int tid = threadIdx.x, w = tid / 32, lane = tid % 32;
   pdl_trigger();
+  pdl_wait();
   AttnUnit u;
   if (!attn_unit<CATP_ROWS, CATP_TK>(c, a, u)) return;
   // the softmax threads' rows; those past the last repeat it
@@ -719,6 +721,7 @@ __global__ void __launch_bounds__(WARPS * 32) cache_attention_join_kernel(const 
   __shared__ float tops[WARPS], sums[WARPS], outs[WARPS][D];
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t item = blockIdx.x;  // (sequence, row, head)
+  pdl_trigger();
   const int head = (int)(item % a.heads), i = (int)(item / a.heads % a.max_q);
   const int64_t seq = item / a.heads / a.max_q;
   pdl_wait();

@@ -84,6 +84,8 @@ S1C_DEV void unpack8(const uint4& v, float (&x)[8]) {
 // thread at the largest page), and a value costs about nine instructions.
 template <typename T>
 __global__ void __launch_bounds__(128) cache_write_kernel(const CacheView c, const CacheRows r) {
+  pdl_trigger();
+  pdl_wait();
   const int seq = blockIdx.x / r.units, h = blockIdx.y, kv = blockIdx.z;
   const int first = r.cu[seq], start = r.start[seq];
   const int count = min(r.cu[seq + 1] - first, r.most);
@@ -190,6 +192,8 @@ __global__ void __launch_bounds__(128) cache_write_kernel(const CacheView c, con
 // written as 0. A byte code becomes fp32 under the exponent of 2^23.
 template <typename T>
 __global__ void __launch_bounds__(256) cache_read_kernel(const CacheView c, const CacheRows r) {
+  pdl_trigger();
+  pdl_wait();
   const int seq = blockIdx.x / r.units, h = blockIdx.y, kv = blockIdx.z;
   const int first = r.cu[seq], count = min(r.cu[seq + 1] - first, r.most), start = r.start[seq];
   const int shift = 31 - __clz(c.page), vshift = c.dim == 128 ? 3 : 2;

@@ -26,9 +26,9 @@
 //    tiles are summed in the warps' order, hence the same bits in each call;
 //  - where not even one row of x fits, each warp has whole tiles, and x passes through in blocks of columns.
 //
-// Measured: 1 x 28672 x 8192, groups of 128: 27.7 us, 4.4 TB/s; 28672 rows more take 19.6 us more (6.2
+// Measured: 1 x 28672 x 8192, groups of 128: 27.2 us, 4.5 TB/s; 28672 rows more take 19.6 us more (6.2
 // TB/s), so what is left is fixed: the launch, staging x (3 us), the last tiles. 16 x 50368 x 2624 with
-// zero points, groups of 64: 36.9 us (2.1 TB/s), of which 5.5 us stage x; the warps, four on a scheduler,
+// zero points, groups of 64: 36.3 us (2.1 TB/s), of which 5.5 us stage x; the warps, four on a scheduler,
 // wait for one another's products and shared memory there. 16 warps were better than 12, 20 or 24
 // (registers). Not kept: TMA rings with a barrier for each step (38 us for the first case), codes loaded
 // ahead into registers (42 us: loads share a few scoreboards, so the oldest waits for the newest).
@@ -352,6 +352,8 @@ template <typename T, int GROUP, int NT, int RT, int SPAN, int WARPS, bool ZERO>
 __global__ void __launch_bounds__(WARPS * 32) nibble_kernel(const NibbleArgs a) {
   using W = NibbleWarp<T, GROUP, NT, RT, SPAN, WARPS, ZERO>;
   extern __shared__ __align__(128) uint8_t base[];
+  pdl_trigger();
+  pdl_wait();
   const bool split = a.split;
   const NibbleSmem sm(a.M, a.block, GROUP, W::RING, WARPS * W::PART, split);
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;

@@ -26,7 +26,7 @@ bool launch_nibble_as(NibbleArgs a, int dev, cudaStream_t st) {
   }
   const int units = a.split ? a.tiles : (a.tiles + WARPS - 1) / WARPS;
   allow_smem<KERNEL>(dev);
-  KERNEL<<<std::min(units, sm_count(dev)), WARPS * 32, smem(), st>>>(a);
+  launch_after(KERNEL, (unsigned)std::min(units, sm_count(dev)), WARPS * 32, smem(), 1, st, a);
   return true;
 }
 

@@ -140,18 +140,17 @@ void launch_attention(const CacheView& c, const CacheAttnArgs& a, bool prompt, i
   const dim3 grid((unsigned)(a.n * c.heads * a.tiles), a.chunks);
   if (prompt) {
     allow_smem<cache_prompt_kernel<T, D>>(dev);
-    cache_prompt_kernel<T, D><<<grid, CATP_WARPS * 32, sizeof(CachePromptSmem<D>) + 1024, st>>>(k, v, c, a);
+    launch_after(cache_prompt_kernel<T, D>, grid, CATP_WARPS * 32, sizeof(CachePromptSmem<D>) + 1024, 1, st, k, v, c, a);
   } else {
     allow_smem<cache_attention_kernel<T, D>>(dev);
-    cache_attention_kernel<T, D><<<grid, CATT_WARPS * 32, sizeof(CacheAttnSmem<D>) + 1024, st>>>(k, v, c, a);
+    launch_after(cache_attention_kernel<T, D>, grid, CATT_WARPS * 32, sizeof(CacheAttnSmem<D>) + 1024, 1, st, k, v, c, a);
   }
-  CK(cudaGetLastError());
   if (a.chunks > 1) {
     const unsigned items = (unsigned)((int64_t)a.n * a.max_q * a.heads);
     if (a.chunks > 16)
-      launch_after(cache_attention_join_kernel<T, D, 16>, items, 512, st, a);
+      launch_after(cache_attention_join_kernel<T, D, 16>, items, 512, 0, 1, st, a);
     else
-      launch_after(cache_attention_join_kernel<T, D, 4>, items, 128, st, a);
+      launch_after(cache_attention_join_kernel<T, D, 4>, items, 128, 0, 1, st, a);
   }
 }
 template <typename T>
@@ -168,14 +167,7 @@ void launch_sample(SampleArgs a, int rows, int dev, cudaStream_t st) {
   a.slice = ((a.vocab + blocks - 1) / blocks + 7) / 8 * 8;
   a.vec = aligned(a.logits, 16) && a.stride * (int64_t)sizeof(T) % 16 == 0;
   allow_smem<sample_kernel<T>>(dev);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(rows * blocks)), cfg.blockDim = dim3(SMP_THREADS), cfg.stream = st;
-  cfg.dynamicSmemBytes = sizeof(SampleShared);
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = blocks, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr, cfg.numAttrs = 1;
-  CK(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a));
+  launch_after(sample_kernel<T>, (unsigned)(rows * blocks), SMP_THREADS, sizeof(SampleShared), blocks, st, a);
 }
 
 }  // namespace
@@ -209,7 +201,6 @@ s1c_status s1c_nibble_gemm(int32_t dtype, const void* d_x, int64_t x_stride, con
       (d_zeros ? launch_nibble_f16_zeros : launch_nibble_f16)(a, group, dev.device, st);
     else
       (d_zeros ? launch_nibble_bf16_zeros : launch_nibble_bf16)(a, group, dev.device, st);
-    CK(cudaGetLastError());
   });
 }
 
@@ -227,10 +218,9 @@ s1c_status s1c_cache_write(const s1c_cache* cache, int32_t dtype, const void* d_
     const dim3 grid((unsigned)(n * r.units), (unsigned)c.heads, 2);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == S1C_DT_F16)
-      cache_write_kernel<__half><<<grid, 128, 0, st>>>(c, r);
+      launch_after(cache_write_kernel<__half>, grid, 128, 0, 1, st, c, r);
     else
-      cache_write_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(c, r);
-    CK(cudaGetLastError());
+      launch_after(cache_write_kernel<__nv_bfloat16>, grid, 128, 0, 1, st, c, r);
   });
 }
 
@@ -250,10 +240,9 @@ s1c_status s1c_cache_read(const s1c_cache* cache, int32_t dtype, void* d_k, int6
     const dim3 grid((unsigned)(n * units), (unsigned)c.heads, 2);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == S1C_DT_F16)
-      cache_read_kernel<__half><<<grid, 256, 0, st>>>(c, r);
+      launch_after(cache_read_kernel<__half>, grid, 256, 0, 1, st, c, r);
     else
-      cache_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(c, r);
-    CK(cudaGetLastError());
+      launch_after(cache_read_kernel<__nv_bfloat16>, grid, 256, 0, 1, st, c, r);
   });
 }
 
@@ -300,7 +289,6 @@ s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, const void
       launch_attention<__half>(c, a, p.prompt, dev.device, st);
     else
       launch_attention<__nv_bfloat16>(c, a, p.prompt, dev.device, st);
-    CK(cudaGetLastError());
   });
 }
 
@@ -325,7 +313,6 @@ s1c_status s1c_sample(int32_t dtype, const void* d_logits, int64_t row_stride, i
       launch_sample<__half>(a, rows, dev.device, st);
     else
       launch_sample<__nv_bfloat16>(a, rows, dev.device, st);
-    CK(cudaGetLastError());
   });
 }
 

@@ -23,7 +23,7 @@
 // fp32 by each thread first, in a fixed order. Logits more than 45 powers of two below the largest have no
 // mass.
 //
-// Measured: 1 x 50368 fp32, top-k 50 and top-p: 17.6 us, of which the exchanges of the eight blocks are
+// Measured: 1 x 50368 fp32, top-k 50 and top-p: 17.0 us, of which the exchanges of the eight blocks are
 // about half; 256 x 50368 bf16, top-p and min-p: 49 us, where the pass that counts and sums (25 instructions
 // a logit) is a third. Without a list (64 x 131072, no filter) 124 us. Not kept: a row in shared memory and
 // one block of 1024 threads an SM (65 us for the 256 rows).
@@ -534,6 +534,8 @@ template <typename T>
 __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   SampleShared& s = *reinterpret_cast<SampleShared*>(raw);
+  pdl_trigger();
+  pdl_wait();
   auto cluster = cooperative_groups::this_cluster();
   const int blocks = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
   const int r = blockIdx.x / blocks, t = threadIdx.x, lane = t & 31, w = t >> 5;

@@ -925,3 +925,60 @@ def test_first_calls_of_a_process_can_be_captured(ops):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     out = subprocess.run([sys.executable, "-c", _FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0, out.stderr[-2000:]
+
+
+@pytest.mark.parametrize("eager", [True, False])
+def test_calls_behind_copies_fills_and_other_streams(ops, eager):
+    """Inputs that a copy, a fill, a kernel of another stream and an operator made, one right before each
+    call: a kernel that is scheduled early must still see all of them. Eagerly and as a replayed graph."""
+    g = _gen(3)
+    M, K = 4, 512
+    _, codes, scales, _ = _nibble_inputs(M, K, K, 128, torch.float16, False, 4)
+    src = [torch.randn(M, K, generator=g, device="cuda").half() * 0.1 for _ in range(20)]
+    a, b, c = (torch.zeros(M, K, dtype=torch.float16, device="cuda") for _ in range(3))
+    logits = torch.zeros(M, K, device="cuda")
+    tokens = torch.zeros(20, M, dtype=torch.int32, device="cuda")
+    sums = torch.zeros(20, M, K, device="cuda")
+    u = torch.rand(M, generator=g, device="cuda")
+    side = torch.cuda.Stream()
+
+    def run():
+        main = torch.cuda.current_stream()
+        for i in range(20):
+            a.copy_(src[i])                                      # a copy, then the operator
+            _nibble(ops, a, codes, scales, None, b, K, 128)
+            _nibble(ops, b, codes, scales, None, c, K, 128)      # an operator behind an operator
+            a.fill_(float("nan"))                                # overwritten right behind
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                logits.copy_(c)
+                b.zero_()
+            main.wait_stream(side)
+            _nibble(ops, b, codes, scales, None, c, K, 128)      # behind another stream: zeros
+            logits.add_(c)
+            ops.sample(ops.DT_F32, logits.data_ptr(), K, M, K, tokens[i].data_ptr(), u.data_ptr(), stream=main.cuda_stream)
+            sums[i].copy_(logits)
+            logits.fill_(float("nan"))
+
+    if eager:
+        run()
+    else:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        graph.replay()
+        tokens.zero_(), sums.zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    for i in range(20):
+        b2, c2 = torch.empty_like(b), torch.empty_like(c)
+        _nibble(ops, src[i], codes, scales, None, b2, K, 128)
+        torch.cuda.synchronize()
+        _nibble(ops, b2, codes, scales, None, c2, K, 128)
+        torch.cuda.synchronize()
+        want = c2.float()
+        assert torch.equal(sums[i], want), i
+        one = torch.zeros(M, dtype=torch.int32, device="cuda")
+        ops.sample(ops.DT_F32, want.data_ptr(), K, M, K, one.data_ptr(), u.data_ptr(), stream=_stream())
+        torch.cuda.synchronize()
+        assert torch.equal(tokens[i], one), i
