@@ -28,10 +28,11 @@
 //
 // Measured: 1 x 28672 x 8192, groups of 128: 27.2 us, 4.5 TB/s; 28672 rows more take 19.6 us more (6.2
 // TB/s), so what is left is fixed: the launch, staging x (3 us), the last tiles. 16 x 50368 x 2624 with
-// zero points, groups of 64: 36.3 us (2.1 TB/s), of which 5.5 us stage x; the warps, four on a scheduler,
-// wait for one another's products and shared memory there. 16 warps were better than 12, 20 or 24
-// (registers). Not kept: TMA rings with a barrier for each step (38 us for the first case), codes loaded
-// ahead into registers (42 us: loads share a few scoreboards, so the oldest waits for the newest).
+// zero points, groups of 64: 35.7 us (2.2 TB/s), of which about 5 us stage x (two blocks together, from nine rows
+// on); the warps, four on a scheduler, wait for one another's products and shared memory there. 16 warps
+// were better than 12, 20 or 24 (registers). Not kept: TMA rings with a barrier for each step (38 us for
+// the first case), codes loaded ahead into registers (42 us: loads share a few scoreboards, so the oldest
+// waits for the newest).
 #pragma once
 #include "mma.cuh"
 
@@ -64,6 +65,29 @@ template <int N>
 S1C_DEV void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+
+// The block's place in its cluster, the cluster's blocks, its barrier, and an address in another block.
+S1C_DEV int cluster_rank() {
+  int r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+S1C_DEV int cluster_blocks() {
+  int r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+S1C_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+S1C_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+S1C_DEV uint32_t cluster_address(const void* p, int block) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(block));
+  return r;
+}
+S1C_DEV void cluster_put(uint32_t at, uint4 v) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+S1C_DEV void cluster_put(uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
 
 // Shared memory of one block, in bytes.
 struct NibbleSmem {
@@ -290,18 +314,22 @@ struct NibbleWarp {
 
 // Stages columns [first, first + passes * 256) of x: f16 by a power of two for each row, in the order of
 // the codes, and the groups' sums times -2^-24 (-8 * 2^-24 without zero points). A pair (row, part of its
-// passes) belongs to one warp.
-template <typename T, int GROUP, int WARPS, bool ZERO>
+// passes) belongs to one warp. PAIR: a block that is one of two in its cluster takes every second row, from
+// `rank` on, and writes what it has staged to the other block too.
+template <typename T, int GROUP, int WARPS, bool ZERO, bool PAIR>
 S1C_DEV void nibble_stage(const NibbleArgs& a, __half* xs, float* sums, float* row_scale, uint32_t* tops, int pitch, int sum_pitch,
-                          int first, int passes, int groups) {
+                          int first, int passes, int groups, int rank = 0, int blocks = 1) {
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int parts = a.M >= WARPS ? 1 : WARPS / a.M;
+  int rows = a.M;
+  if constexpr (PAIR) rows = (a.M - rank + blocks - 1) / blocks;  // none for the second block of a single row
+  const int parts = rows >= WARPS ? 1 : WARPS / (PAIR ? max(rows, 1) : rows);
   // where the lane's eight columns go among the 16 pieces of their 128: word j of lane c
   const int i = lane % 16;
   const int j = GROUP == 128 ? i % 4 : GROUP == 64 ? i / 8 * 2 + i % 2 : i / 4, c = GROUP == 128 ? i / 4 : GROUP == 64 ? i % 8 / 2 : i % 4;
   const int place = lane / 16 * 128 + (j * 4 + c) * 8;
-  for (int p = w; p < a.M * parts; p += WARPS) {
-    const int m = p / parts, s0 = p % parts * passes / parts, s1 = (p % parts + 1) * passes / parts;
+  for (int p = w; p < rows * parts; p += WARPS) {
+    const int m = PAIR ? rank + p / parts * blocks : p / parts;
+    const int s0 = p % parts * passes / parts, s1 = (p % parts + 1) * passes / parts;
     uint32_t top = 0;
 #pragma unroll 4
     for (int s = s0; s < s1; ++s) {
@@ -324,12 +352,16 @@ S1C_DEV void nibble_stage(const NibbleArgs& a, __half* xs, float* sums, float* r
     if (lane == 0) atomicMax(&tops[m], top);
   }
   __syncthreads();
-  for (int p = w; p < a.M * parts; p += WARPS) {
-    const int m = p / parts, s0 = p % parts * passes / parts, s1 = (p % parts + 1) * passes / parts;
+  if (PAIR && blocks > 1) cluster_wait();
+  for (int p = w; p < rows * parts; p += WARPS) {
+    const int m = PAIR ? rank + p / parts * blocks : p / parts;
+    const int s0 = p % parts * passes / parts, s1 = (p % parts + 1) * passes / parts;
     // 2^up brings the largest value to [2^14, 2^15); rows with an infinity or NaN keep theirs
     const int e = (int)(tops[m] >> 23) - 127, up = e == 128 ? 0 : min(14 - e, 126);
     const float by = __uint_as_float((uint32_t)(127 + up) << 23);
     if (lane == 0) row_scale[m] = __uint_as_float((uint32_t)(127 - up) << 23);
+    if (PAIR && blocks > 1 && lane == 0)
+      cluster_put(cluster_address(row_scale + m, rank ^ 1), __uint_as_float((uint32_t)(127 - up) << 23));
 #pragma unroll 2
     for (int s = s0; s < s1; ++s) {
       uint4* slot = reinterpret_cast<uint4*>(xs + m * pitch + s * 256 + place);
@@ -338,12 +370,18 @@ S1C_DEV void nibble_stage(const NibbleArgs& a, __half* xs, float* sums, float* r
       float f[8], sum = 0.f;
 #pragma unroll
       for (int e2 = 0; e2 < 8; ++e2) f[e2] = bits_f32<T>((uint16_t)(v[e2 / 2] >> (16 * (e2 % 2)))) * by, sum += f[e2];
-      *slot = make_uint4(pack_f16x2(f[0], f[4]), pack_f16x2(f[1] * 0.0625f, f[5] * 0.0625f), pack_f16x2(f[2], f[6]),
-                         pack_f16x2(f[3] * 0.0625f, f[7] * 0.0625f));
+      const uint4 staged = make_uint4(pack_f16x2(f[0], f[4]), pack_f16x2(f[1] * 0.0625f, f[5] * 0.0625f), pack_f16x2(f[2], f[6]),
+                                      pack_f16x2(f[3] * 0.0625f, f[7] * 0.0625f));
+      *slot = staged;
+      if (PAIR && blocks > 1) cluster_put(cluster_address(slot, rank ^ 1), staged);
 #pragma unroll
       for (int o = 1; o < GROUP / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       const int g = (s * 256 + lane * 8) / GROUP;
-      if (lane % (GROUP / 8) == 0 && g < groups) sums[m * sum_pitch + g] = sum * (ZERO ? -0x1p-24f : -0x1p-21f);
+      if (lane % (GROUP / 8) == 0 && g < groups) {
+        const float start = sum * (ZERO ? -0x1p-24f : -0x1p-21f);
+        sums[m * sum_pitch + g] = start;
+        if (PAIR && blocks > 1) cluster_put(cluster_address(sums + m * sum_pitch + g, rank ^ 1), start);
+      }
     }
   }
 }
@@ -353,6 +391,8 @@ __global__ void __launch_bounds__(WARPS * 32) nibble_kernel(const NibbleArgs a) 
   using W = NibbleWarp<T, GROUP, NT, RT, SPAN, WARPS, ZERO>;
   extern __shared__ __align__(128) uint8_t base[];
   pdl_trigger();
+  const int rank = NT > 1 ? cluster_rank() : 0, blocks = NT > 1 ? cluster_blocks() : 1;
+  if (blocks > 1) cluster_arrive();  // nibble_stage waits: the other block has begun
   pdl_wait();
   const bool split = a.split;
   const NibbleSmem sm(a.M, a.block, GROUP, W::RING, WARPS * W::PART, split);
@@ -409,7 +449,8 @@ __global__ void __launch_bounds__(WARPS * 32) nibble_kernel(const NibbleArgs a) 
   loaded();
   __syncthreads();
   if (split) {
-    nibble_stage<T, GROUP, WARPS, ZERO>(a, xs, sums, row_scale, tops, sm.pitch, sm.sum_pitch, 0, (a.steps + 1) / 2, a.steps * W::GP);
+    nibble_stage<T, GROUP, WARPS, ZERO, (NT > 1)>(a, xs, sums, row_scale, tops, sm.pitch, sm.sum_pitch, 0, (a.steps + 1) / 2, a.steps * W::GP, rank, blocks);
+    if (blocks > 1) cluster_arrive(), cluster_wait();  // the other block's rows have landed
     __syncthreads();
   }
   p.clear();
@@ -427,7 +468,7 @@ __global__ void __launch_bounds__(WARPS * 32) nibble_kernel(const NibbleArgs a) 
       if (step == 0 && threadIdx.x < 64) tops[threadIdx.x] = 0;
       __syncthreads();
       const int steps = min(a.block, a.steps - step);
-      nibble_stage<T, GROUP, WARPS, ZERO>(a, xs, sums, row_scale, tops, sm.pitch, sm.sum_pitch, step * 128, (steps + 1) / 2, steps * W::GP);
+      nibble_stage<T, GROUP, WARPS, ZERO, (NT > 1)>(a, xs, sums, row_scale, tops, sm.pitch, sm.sum_pitch, step * 128, (steps + 1) / 2, steps * W::GP);
       __syncthreads();
       if (step) {
 #pragma unroll

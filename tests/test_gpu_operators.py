@@ -110,6 +110,14 @@ def test_nibble_gemm(ops, M, N, K, group, dt):
         assert (full[:, N:] == 7).all()
 
 
+@pytest.mark.parametrize("M,N,K,group", [(64, 33, 9000, 128), (9, 16, 300, 32), (9, 33, 300, 64), (11, 17, 1000, 128),
+                                         (64, 50, 300, 128), (55, 2400, 8000, 32), (17, 3000, 700, 64)])
+def test_nibble_gemm_staged_by_two_blocks(ops, M, N, K, group):
+    """From nine rows on two blocks stage x together: one row tile (a block alone), odd numbers of rows and
+    tiles, several launches whose last has few rows. Bounds as in test_nibble_gemm."""
+    test_nibble_gemm(ops, M, N, K, group, "bf16")
+
+
 def test_nibble_gemm_extreme_codes_and_values(ops):
     """All codes 0 or 15 with the largest finite x of f16 in fp32 output; zero scales give zero; a NaN or
     infinite row of x stays in its own row; bytes behind the last column do not count."""
