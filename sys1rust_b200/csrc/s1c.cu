@@ -235,6 +235,9 @@ struct SplitCtx {
   size_t ws_bytes;
   void* out;
   int ldo;
+  // B is not written on the stream (a handle's weights): the cluster kernel loads it before it waits for the
+  // kernel before it. Where B is the caller's, that kernel may be what writes it.
+  bool fixed_b = true;
 };
 
 // Split-K factor for a GEMM with few output tiles: enough splits to cover the SMs, at least one
@@ -274,7 +277,7 @@ CskPlan plan_csk(int M, int N, int K, int num_sms, bool geglu) {
 }
 
 template <int BN, int EPI>
-void launch_csk_bn(const CUtensorMap& ta, const CUtensorMap& tb, const CskArgs& a, int tiles, cudaStream_t st) {
+void launch_csk_bn(const CUtensorMap& ta, const CUtensorMap& tb, const CskArgs& a, int tiles, bool fixed_b, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * a.C));
   cfg.blockDim = dim3(GEMM_THREADS);
@@ -288,7 +291,7 @@ void launch_csk_bn(const CUtensorMap& ta, const CUtensorMap& tb, const CskArgs& 
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = t_pdl ? 2 : 1;
+  cfg.numAttrs = t_pdl && fixed_b ? 2 : 1;
   CK(cudaLaunchKernelEx(&cfg, gemm_csk_sm100<BN, EPI>, ta, tb, a));
 }
 
@@ -304,10 +307,10 @@ void launch_csk(const CUtensorMap& ta, const WeightMap& tb, const GemmArgs& g, c
   a.status = g.status;
   a.pf = g.pf; a.pf_bytes = g.pf_bytes;
   if constexpr (EPI == EPI_GEGLU) {
-    launch_csk_bn<128, EPI>(ta, tb.quarter, a, p.tiles, st);
+    launch_csk_bn<128, EPI>(ta, tb.quarter, a, p.tiles, sk.fixed_b, st);
   } else {
-    if (p.bn == 128) launch_csk_bn<128, EPI>(ta, tb.half, a, p.tiles, st);
-    else launch_csk_bn<64, EPI>(ta, tb.quarter, a, p.tiles, st);
+    if (p.bn == 128) launch_csk_bn<128, EPI>(ta, tb.half, a, p.tiles, sk.fixed_b, st);
+    else launch_csk_bn<64, EPI>(ta, tb.quarter, a, p.tiles, sk.fixed_b, st);
   }
 }
 
@@ -2444,7 +2447,7 @@ s1c_status s1c_gemm(int32_t epi, const void* d_A, const void* d_B, void* d_out, 
       std::lock_guard<std::mutex> g(mu);
       if (!ws_dev[dev]) CK(cudaMalloc(&ws_dev[dev], (size_t)32 << 20));
     }
-    const SplitCtx sk{ws_dev[dev], (size_t)32 << 20, d_out, out_w};
+    const SplitCtx sk{ws_dev[dev], (size_t)32 << 20, d_out, out_w, false};
     switch (epi) {
       case EPI_STORE: launch_gemm<EPI_STORE>(ta, tb, tc, a, n_sms, st, variant, &sk); break;
       case EPI_ROPE: launch_gemm<EPI_ROPE>(ta, tb, tc, a, n_sms, st, variant, &sk); break;
@@ -2636,7 +2639,7 @@ s1c_status s1c_gemm_splitk_noalloc(int32_t epi, const void* d_A, const void* d_B
     const CUtensorMap ta = make_tmap(d_A, (uint64_t)M, K, K, GEMM_BM);
     const WeightMap tb = make_wmap(d_B, N, K, K);
     const CUtensorMap tc = make_out_tmap(d_out, f32, (uint64_t)M, out_w, out_w);
-    const SplitCtx sk{nd.scratch, scratch_bytes, d_out, out_w};
+    const SplitCtx sk{nd.scratch, scratch_bytes, d_out, out_w, false};
     t_pdl = false;
     switch (epi) {
       case EPI_STORE: launch_gemm<EPI_STORE>(ta, tb, tc, a, nd.n_sms, st, 3, &sk); break;

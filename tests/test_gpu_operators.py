@@ -990,3 +990,37 @@ def test_calls_behind_copies_fills_and_other_streams(ops, eager):
         ops.sample(ops.DT_F32, want.data_ptr(), K, M, K, one.data_ptr(), u.data_ptr(), stream=_stream())
         torch.cuda.synchronize()
         assert torch.equal(tokens[i], one), i
+
+
+@pytest.mark.parametrize("eager", [True, False])
+def test_gemm_whose_second_matrix_an_operator_wrote(ops, eager):
+    """``s1c_gemm`` with few rows right behind the operator that writes its B: B is complete before it is
+    loaded, eagerly and in a replayed graph. Bound: a rounded result and K products summed in fp32."""
+    from sys1rust_b200 import backend
+    M, N, K, inner, rounds = 16, 64, 2048, 8192, 20
+    _, codes, scales, _ = _nibble_inputs(1, K, inner, 128, torch.bfloat16, False, 5)
+    g = _gen(6)
+    x = [(torch.randn(N, inner, generator=g, device="cuda") * 0.01).bfloat16() for _ in range(rounds)]
+    a = torch.randn(M, K, generator=g, device="cuda").bfloat16()
+    b = torch.zeros(N, K, dtype=torch.bfloat16, device="cuda")
+    out = torch.zeros(rounds, M, N, dtype=torch.bfloat16, device="cuda")
+    seen = torch.zeros(rounds, N, K, dtype=torch.bfloat16, device="cuda")
+
+    def run():
+        for i in range(rounds):
+            _nibble(ops, x[i], codes, scales, None, b, inner, 128)
+            backend.gemm(backend.EPI_STORE, a.data_ptr(), b.data_ptr(), out[i].data_ptr(), M, N, K, stream=_stream())
+            seen[i].copy_(b)
+
+    run()
+    if not eager:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        out.zero_(), seen.zero_(), b.zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    want = a.double() @ seen.double().transpose(1, 2)
+    most = a.double().abs() @ seen.double().abs().transpose(1, 2)
+    assert ((out.double() - want).abs() <= _u(torch.bfloat16) * want.abs() + (1 + 2.0 ** -8) * K * 2.0 ** -22 * most).all()
