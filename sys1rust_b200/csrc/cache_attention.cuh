@@ -474,7 +474,6 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   extern __shared__ uint8_t raw[];
   S& sm = *reinterpret_cast<S*>(raw + (1024 - smem_u32(raw) % 1024) % 1024);
   const int tid = threadIdx.x, w = tid / 32, lane = tid % 32;
-  pdl_trigger();
   pdl_wait();
   AttnUnit u;
   if (!attn_unit<CATP_ROWS, CATP_TK>(c, a, u)) return;
@@ -502,6 +501,9 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   }
   tc_fence_before();
   const float v_top = attn_pages<CATP_WARPS>(c, a, u, sm.page, sm.top);  // with barriers of the block
+  // Only now: a kernel that is scheduled early may hold TMEM while it waits for this one, so each block has
+  // its own first.
+  pdl_trigger();
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
   volatile int* abort = &sm.abort;

@@ -52,9 +52,10 @@ inline int sm_count(int dev) {
 }
 
 // Launches a kernel, in clusters of `cluster` blocks, that may be scheduled while the one before it on the
-// stream ends: each operator's kernel starts with pdl_trigger and, before it touches global memory,
-// pdl_wait. Measured in a row of calls: 0.4 to 0.9 us less for each kernel (1 x 1024 x 1024 products 6.3 ->
-// 5.9 us; a cache's write and read of 64 tokens 16.9 -> 15.6 us, 20.4 -> 15.5 us one call at a time).
+// stream ends: each operator's kernel calls pdl_trigger as soon as it may (where it has TMEM: when it has
+// that) and, before it touches global memory, pdl_wait. Measured in a row of calls: 0.4 to 0.9 us less for each
+// kernel (1 x 1024 x 1024 products 6.3 -> 5.9 us; a cache's write and read of 64 tokens 16.9 -> 15.6 us, 20.4 ->
+// 15.5 us one call at a time).
 template <typename... P, typename... A>
 void launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, int cluster, cudaStream_t st, const A&... args) {
   cudaLaunchConfig_t cfg{};

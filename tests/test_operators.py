@@ -194,3 +194,23 @@ def test_cache_struct_matches_the_header(tmp_path):
     subprocess.run([cc, "-std=c11", "-I", os.path.join(root, "include"), str(src), "-o", str(tmp_path / "probe")], check=True)
     got = [int(v) for v in subprocess.run([str(tmp_path / "probe")], check=True, capture_output=True, text=True).stdout.split()]
     assert got == [C.sizeof(bk.CCache)] + [getattr(bk.CCache, n).offset for n in names]
+
+
+def test_kernels_hold_their_tmem_before_a_successor_may_start():
+    """A kernel that is scheduled early can hold tensor memory while it waits for its predecessor. If a block of the
+    predecessor had still to allocate its own, neither would end: so each kernel calls pdl_trigger after its
+    allocation and a barrier of the block (attn_pages has some)."""
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.abspath(bk.__file__)), "csrc")
+    checked = []
+    for name in sorted(os.listdir(csrc)):
+        with open(os.path.join(csrc, name)) as f:
+            text = re.sub(r"//[^\n]*", "", f.read())
+        for body in re.split(r"__global__", text)[1:]:
+            alloc = re.search(r"\btmem_alloc2?\(", body)
+            if alloc:
+                trigger = re.search(r"\bpdl_trigger\(\)", body)
+                assert trigger is None or alloc.start() < trigger.start(), name
+                assert trigger is None or re.search("__syncthreads|cluster_sync_all|attn_pages", body[alloc.end(): trigger.start()]), name
+                checked.append(name)
+    assert "cache_attention.cuh" in checked and "gemm_sm100_csk.cuh" in checked
