@@ -239,7 +239,8 @@ struct AttnRows {
     if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float n = fmaxf(m[e], top[e]), keep = m[e] == -INFINITY ? 0.f : exp2f(m[e] - n);
+        // each row by its own scores alone, so that its bits do not depend on the rows beside it
+        const float n = top[e] > m[e] + 1.75f ? top[e] : m[e], keep = m[e] == -INFINITY ? 0.f : exp2f(m[e] - n);
         m[e] = n, l[e] *= keep;
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i][2 * e] *= keep, o[i][2 * e + 1] *= keep;

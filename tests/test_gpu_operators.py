@@ -543,6 +543,25 @@ def test_cache_attention_all_values_zero(ops):
     _check_attention(c, q, 1, [1], [50], 0.125, -1, out, lse)
 
 
+@pytest.mark.parametrize("D,H,G,rows,L", [(64, 32, 2, 4, 8000), (128, 32, 4, 3, 4000), (128, 2, 8, 20, 3000), (64, 40, 8, 1, 6000)])
+def test_cache_attention_rows_do_not_depend_on_each_other(ops, D, H, G, rows, L):
+    """A row and head's bits are the same whatever the other rows and heads of the call hold: queries of zeros, whose
+    scores never grow along the keys, or large ones, whose scores do."""
+    heads = H * G
+    for seed in range(3):
+        c = Paged(ops, 1, L, H, D, 16, 73 + seed)
+        q = torch.randn(rows, heads, D, generator=_gen(74 + seed), device="cuda").half()
+        keep = torch.zeros(rows, heads, dtype=torch.bool, device="cuda")
+        keep.view(-1)[::3] = True
+        got = []
+        for by in (0, 8):
+            x = torch.where(keep[..., None], q, q * by)
+            out, lse = _attention(ops, c, x.view(rows, -1), heads, [rows], [L], 0.1)
+            got.append((out[:rows, : heads * D].reshape(rows, heads, D), lse[:rows]))
+        assert torch.equal(got[0][0][keep], got[1][0][keep]) and torch.equal(got[0][1][keep], got[1][1][keep])
+        assert not torch.equal(got[0][0], got[1][0])
+
+
 def test_cache_attention_long_cache(ops):
     """70001 positions, more than 2^31 bytes into the codes' array for the last pages."""
     H, D, page, L = 8, 128, 64, 70001
