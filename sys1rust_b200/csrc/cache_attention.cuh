@@ -732,11 +732,11 @@ __global__ void __launch_bounds__(WARPS * 32) cache_attention_join_kernel(const 
   if (i >= a.cu[seq + 1] - first) return;
   const float* lse = a.part_lse + item * a.chunks;
   float top = -INFINITY;
-  for (int s = threadIdx.x; s < a.chunks; s += WARPS * 32) top = fmaxf(top, lse[s]);
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  for (int s = threadIdx.x; s < a.chunks; s += WARPS * 32) top = max_nan(top, lse[s]);  // NaN: so is the row
+  for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) tops[w] = top;
   __syncthreads();
-  for (int j = 0; j < WARPS; ++j) top = fmaxf(top, tops[j]);
+  for (int j = 0; j < WARPS; ++j) top = max_nan(top, tops[j]);
   float sum = 0.f, o[E] = {};
   if (top != -INFINITY) {
 #pragma unroll 8
@@ -748,7 +748,7 @@ __global__ void __launch_bounds__(WARPS * 32) cache_attention_join_kernel(const 
       for (int e = 0; e < E; ++e) v[e] = p[e];
       sum += by;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] += by == 0.f ? 0.f : by * v[e];  // a chunk without a key has written no output
+      for (int e = 0; e < E; ++e) o[e] += by * v[e];  // a chunk without a key has written zeros
     }
   }
   if (lane == 0) sums[w] = sum;

@@ -562,6 +562,29 @@ def test_cache_attention_rows_do_not_depend_on_each_other(ops, D, H, G, rows, L)
         assert not torch.equal(got[0][0], got[1][0])
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("D,H,G,rows,L", [(64, 2, 3, 2, 100), (128, 2, 3, 2, 3000), (128, 1, 4, 3, 70001), (64, 1, 8, 30, 120),
+                                          (128, 2, 8, 20, 3000)])
+def test_cache_attention_queries_that_are_not_finite(ops, D, H, G, rows, L, dt):
+    """A query with a NaN or infinity gives NaN, whether its keys are split between blocks (and joined) or not,
+    for few rows and for many; every other row and head keeps its bits."""
+    heads = H * G
+    c = Paged(ops, 1, L, H, D, 16, 71)
+    q = torch.randn(rows, heads * D, generator=_gen(72), device="cuda").to(DT[dt])
+    clean, clean_lse = _attention(ops, c, q, heads, [rows], [L], 0.1)
+    assert torch.isfinite(clean).all()
+    q = q.view(rows, heads, D)
+    bad = torch.zeros(rows, heads, dtype=torch.bool, device="cuda")
+    for r, h, d, value in [(0, 1, 5, math.nan), (rows - 1, heads - 1, D - 1, math.nan), (rows // 2, 0, 0, math.inf),
+                           (rows - 1, 0, 33, -math.inf)]:
+        q[r, h, d], bad[r, h] = value, True
+    out, lse = _attention(ops, c, q.view(rows, -1), heads, [rows], [L], 0.1)
+    have = out[:rows, : heads * D].reshape(rows, heads, D)
+    assert torch.isnan(have[bad]).all() and torch.isnan(lse[:rows][bad]).all()
+    assert torch.equal(have[~bad], clean[:rows, : heads * D].reshape(rows, heads, D)[~bad])
+    assert torch.equal(lse[:rows][~bad], clean_lse[:rows][~bad])
+
+
 def test_cache_attention_long_cache(ops):
     """70001 positions, more than 2^31 bytes into the codes' array for the last pages."""
     H, D, page, L = 8, 128, 64, 70001
