@@ -145,17 +145,21 @@ S1C_DEV void attn_issue(const CacheView& c, const AttnUnit& u, const float4* lis
   __syncwarp();
 }
 
-// The power of two that brings a row's largest value to [2^14, 2^15); rows with an infinity or NaN keep theirs.
-S1C_DEV int attn_up(float top) {
-  const int ex = (int)((__float_as_uint(top) >> 23) & 255u) - 127;
-  return ex == 128 ? 0 : min(14 - ex, 100);
+// A row's power of two, which brings its largest value to [2^14, 2^15), and the factor that undoes it. A row with
+// an infinity or NaN counts as zeros, marked by a factor of -0, up to its end, where its sum becomes NaN if it
+// has seen a key: nothing of it can then reach a place without one.
+S1C_DEV float attn_up(float top, float scale, float& factor) {
+  const int up = min(14 - ((int)(__float_as_uint(top) >> 23) - 127), 100);
+  factor = top < INFINITY ? scale * __uint_as_float((uint32_t)(127 - up) << 23) + 0.f : -0.f;
+  return __uint_as_float((uint32_t)(127 + up) << 23);
 }
+S1C_DEV float attn_sum(float l, float m, float factor) { return __float_as_uint(factor) == 0x80000000u && m != -INFINITY ? NAN : l; }
 
 // One thread's part of two query rows, g and g + 8 of a tile from row `r0` on (rows past the last repeat it).
 struct AttnRows {
   int64_t at[2];
   int head[2], pos[2];
-  float factor[2];       // scale * log2(e) and what undoes the rows' scaling
+  float factor[2];       // scale * log2(e) and what undoes the rows' scaling; -0: not finite
   float start[2];        // -128 * 2^-24 * sum(q)
   float m[2], l[2];      // running maximum and sum
   S1C_DEV void setup(const AttnUnit& u, int r0) {
@@ -184,16 +188,14 @@ struct AttnRows {
         for (int j = 0; j < 4; ++j) top = max_nan(top, fabsf(f[i][j]));
       }
       for (int o = 1; o < 4; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const int up = attn_up(top);
-      const float by = __uint_as_float((uint32_t)(127 + up) << 23);
+      const float by = attn_up(top, a.scale_log2, factor[e]);
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[i][j] *= by, sum += f[i][j];
+        for (int j = 0; j < 4; ++j) f[i][j] = top < INFINITY ? f[i][j] * by : 0.f, sum += f[i][j];
         qa[i][e] = pack_f16x2(f[i][0], f[i][1]), qa[i][e + 2] = pack_f16x2(f[i][2], f[i][3]);
       }
       for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      factor[e] = a.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
       start[e] = sum * -0x1p-17f;
     }
   }
@@ -260,6 +262,7 @@ struct AttnRows {
     for (int e = 0; e < 2; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+      l[e] = attn_sum(l[e], m[e], factor[e]);
     }
   }
 };
@@ -605,17 +608,15 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(x[j]));
       }
-      const int up = attn_up(top);
-      const float by = __uint_as_float((uint32_t)(127 + up) << 23);
+      const float by = attn_up(top, a.scale_log2 * 0x1p-24f, factor);  // the list's key scales have 2^24
 #pragma unroll 4
       for (int i = 0; i < D / 8; ++i) {
         float x[8];
-        unpack8<T>(q[i], x);
+        unpack8<T>(top < INFINITY ? q[i] : make_uint4(0, 0, 0, 0), x);
         *reinterpret_cast<uint4*>(sm.q[i / 8] + tid * 128 + ((i % 8 ^ (tid & 7)) << 4)) =
             make_uint4(pack_f16x2(x[0] * by, x[1] * by), pack_f16x2(x[2] * by, x[3] * by), pack_f16x2(x[4] * by, x[5] * by),
                        pack_f16x2(x[6] * by, x[7] * by));
       }
-      factor = a.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23) * 0x1p-24f;  // the list's key scales have 2^24
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.q_full);
@@ -703,7 +704,7 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       for (int d = 0; d < D; d += 32) {
         float t[32];
         tmem_ld32(tmem + lanes + CATP_TMEM_O + d, t);
-        if (real) attn_put<T, D>(a, u, at_row, head, d, t, v_top, l, m);
+        if (real) attn_put<T, D>(a, u, at_row, head, d, t, v_top, attn_sum(l, m, factor), m);
       }
     }
   }

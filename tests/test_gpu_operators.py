@@ -585,6 +585,24 @@ def test_cache_attention_queries_that_are_not_finite(ops, D, H, G, rows, L, dt):
     assert torch.equal(lse[:rows][~bad], clean_lse[:rows][~bad])
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("H,G,D,lens,keys", [(2, 2, 64, [3, 2, 2], [2, 40, 60]), (1, 4, 128, [40, 33, 50], [30, 200, 90]),
+                                             (1, 3, 64, [3, 2, 1], [2, 3000, 5])])
+def test_cache_attention_queries_that_are_not_finite_and_see_no_key(ops, H, G, D, lens, keys, dt):
+    """NaN and infinities in a query whose keys all lie on pages outside the cache, or which stands before the first
+    position: 0 and -inf as for any query without a key."""
+    heads = H * G
+    c = Paged(ops, 3, max(keys), H, D, 16, 75)
+    c.table[1] = -1
+    q = torch.randn(sum(lens), heads * D, generator=_gen(76), device="cuda").to(DT[dt])
+    q[0, 3], q[lens[0], 5], q[lens[0] + 1, 0] = math.nan, math.nan, -math.inf
+    out, lse = _attention(ops, c, q, heads, lens, keys, 0.1)
+    for rows in (slice(0, lens[0] - keys[0]), slice(lens[0], lens[0] + lens[1])):
+        assert (out[rows, : heads * D] == 0).all() and (lse[rows] == -math.inf).all()
+    seen = torch.cat([out[lens[0] - keys[0]: lens[0]], out[lens[0] + lens[1]: sum(lens)]])[:, : heads * D]
+    assert torch.isfinite(seen).all() and seen.any()
+
+
 def test_cache_attention_long_cache(ops):
     """70001 positions, more than 2^31 bytes into the codes' array for the last pages."""
     H, D, page, L = 8, 128, 64, 70001
