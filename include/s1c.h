@@ -251,6 +251,12 @@ S1C_API s1c_status s1c_gemm_splitk_noalloc(int32_t epi, const void* d_A, const v
  * success (0). Returns S1C_OK when the kernel ended; the device stays usable. */
 S1C_API s1c_status s1c_selftest_wait_timeout(int32_t device, int64_t budget_ns, int32_t* codes);
 
+/* The same for s1c_cache_attention: a small cache is attended to while each tile of keys is waited for beyond what
+ * comes, with a budget of `budget_ns` a wait. codes[0..3] (few rows over few keys, few over keys split between
+ * blocks, many rows, many over split keys) become 1 where every row gave up and came out as NaN, and the same call
+ * without the fault came out without one; 0 otherwise. Allocates, synchronises and frees. */
+S1C_API s1c_status s1c_selftest_cache_attention_timeout(int32_t device, int64_t budget_ns, int32_t* codes);
+
 /* Number of this library's kernel launches the last forward on this handle enqueued. */
 S1C_API int64_t s1c_last_launch_count(const s1c_backend* b);
 
@@ -324,7 +330,8 @@ S1C_API size_t s1c_cache_attention_workspace(const s1c_cache* cache, int32_t hea
  * -inf; one that sees a key and holds an infinity or NaN gets NaN. No sequence may have more than max_q
  * query rows or max_kv positions: what is past them is not computed. Scores, softmax statistics and sums are held in fp32; a key's weight times its value scale is
  * rounded to 11 bits, or to 2^-38 of the row's largest where that is more. The workspace (16-byte aligned) is free
- * for other use when the call's work has run; calls that overlap on the GPU need one each. */
+ * for other use when the call's work has run; calls that overlap on the GPU need one each. Waits inside the
+ * kernels are bounded (2 s each); rows for which one runs out get NaN in out and lse. */
 S1C_API s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, const void* d_q, int64_t q_stride,
                                        void* d_out, int64_t out_stride, float* d_lse, int32_t heads,
                                        const int32_t* d_cu, const int32_t* d_len, const int32_t* d_pages,

@@ -236,6 +236,7 @@ extern "C" {
                       d_uniform: *const f32, d_token: *mut i32, d_prob: *mut f32, stream: *mut c_void) -> s1c_status;
 
     pub fn s1c_selftest_wait_timeout(device: i32, budget_ns: i64, codes: *mut i32) -> s1c_status;
+    pub fn s1c_selftest_cache_attention_timeout(device: i32, budget_ns: i64, codes: *mut i32) -> s1c_status;
 
     // ---- checkpoint files (laya_core::Weights) ----
     pub fn s1c_weights_open(model_dir: *const c_char, out: *mut *mut s1c_weights) -> s1c_status;

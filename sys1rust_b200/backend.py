@@ -169,6 +169,7 @@ def lib() -> C.CDLL:
         "s1c_server_destroy": (None, [P]),
         "s1c_decode": (I32, [P, P, I32, I32, I32, P, P, P, C.POINTER(CActHead), P, C.POINTER(CAnswer)]),
         "s1c_selftest_wait_timeout": (I32, [I32, I64, C.POINTER(C.c_int32)]),
+        "s1c_selftest_cache_attention_timeout": (I32, [I32, I64, C.POINTER(C.c_int32)]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -507,6 +508,18 @@ def selftest_wait_timeout(device: int = 0, budget_ns: int = 50_000_000) -> list:
     L = lib()
     codes = (C.c_int32 * 4)()
     rc = L.s1c_selftest_wait_timeout(device, budget_ns, codes)
+    if rc != S1C_OK:
+        _raise(rc, L.s1c_create_error().decode())
+    return list(codes)
+
+
+def selftest_cache_attention_timeout(device: int = 0, budget_ns: int = 20_000_000) -> list:
+    """Run the waits of the attention over the 8-bit cache into their budget
+    (``s1c_selftest_cache_attention_timeout``): 1 for each of [few rows, few rows over split keys, many rows, many
+    rows over split keys] that gave up as it should."""
+    L = lib()
+    codes = (C.c_int32 * 4)()
+    rc = L.s1c_selftest_cache_attention_timeout(device, budget_ns, codes)
     if rc != S1C_OK:
         _raise(rc, L.s1c_create_error().decode())
     return list(codes)

@@ -24,6 +24,8 @@
 // ring of loads, so nothing waits inside the loop; the four warps' results are joined at the end. Long
 // caches are split over blocks, whose results a second kernel joins.
 //
+// A wait that runs out makes the rows of its block NaN.
+//
 // Many rows: a block of 128 rows on the 5th-generation tensor cores. Four warps convert a tile of 64 keys
 // once for all rows, to f16 in shared memory (whole codes, so no scale enters before the scores); one
 // thread issues S = Q K^T into one of two buffers of TMEM, a tile ahead, and O += P V; four warps have a
@@ -61,6 +63,8 @@ struct CacheAttnArgs {
   float scale_log2;  // scale * log2(e)
   float* part;       // [n * max_q * heads, chunks, dim]: normalised outputs of the chunks
   float* part_lse;   // [n * max_q * heads, chunks]: their log2 sums
+  uint64_t wait_ns = S1C_WAIT_BUDGET_NS;  // of a wait; rows of a block in which one runs out become NaN
+  int beyond = 0;                         // bytes that a tile waits for beyond its own (a self-test: they never come)
 };
 
 constexpr int CATT_TK = 32;   // keys of a tile: few rows
@@ -129,13 +133,13 @@ S1C_DEV float attn_pages(const CacheView& c, const CacheAttnArgs& a, const AttnU
 // TMA of one tile's keys and values to `dst`, by a whole warp: a lane for each page or 32 rows of one.
 // Pages outside the cache are not read.
 template <int D, int TK>
-S1C_DEV void attn_issue(const CacheView& c, const AttnUnit& u, const float4* list, const CUtensorMap& k_map, const CUtensorMap& v_map, int i,
+S1C_DEV void attn_issue(const CacheView& c, const CacheAttnArgs& a, const AttnUnit& u, const float4* list, const CUtensorMap& k_map, const CUtensorMap& v_map, int i,
                         uint8_t* dst, uint64_t* bar) {
   const int lane = threadIdx.x % 32, per = min(c.page, CATT_BOX), boxes = TK / per;
   const int at = u.lo + i * TK + lane * per;
   const int page = lane < boxes && at < u.hi ? __float_as_int(list[(at >> u.shift) - (u.lo >> u.shift)].w) : -1;
   const int count = __popc(__ballot_sync(0xffffffffu, page >= 0));
-  if (lane == 0) mbar_arrive_expect_tx(bar, count * 2 * per * D);
+  if (lane == 0) mbar_arrive_expect_tx(bar, count * 2 * per * D + a.beyond);
   __syncwarp();
   if (page >= 0) {
     const int y = (page * c.heads + u.h) * c.page + (at & (c.page - 1));
@@ -333,7 +337,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   }
   const auto issue = [&](int i) {
     const int slot = i / CATT_WARPS % S::STAGES;
-    attn_issue<D, CATT_TK>(c, u, sm.page, k_map, v_map, i, sm.ring[w][slot], &sm.full[w][slot]);
+    attn_issue<D, CATT_TK>(c, a, u, sm.page, k_map, v_map, i, sm.ring[w][slot], &sm.full[w][slot]);
   };
   for (int s = 0; s < S::STAGES; ++s)
     if (w + s * CATT_WARPS < u.tiles) issue(w + s * CATT_WARPS);
@@ -373,9 +377,16 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
 
   int turn = 0;  // tiles this ring has been through
+  bool late = false;
   for (int i = w; i < u.tiles; i += CATT_WARPS, ++turn) {
     const int slot = turn % S::STAGES;
-    if (!mbar_wait_warp(&sm.full[w][slot], turn / S::STAGES & 1, nullptr, 0, nullptr)) break;
+    if (!mbar_wait_warp(&sm.full[w][slot], turn / S::STAGES & 1, nullptr, 0, nullptr, a.wait_ns)) {
+      late = true;
+      // what is in flight lands before the block ends
+      for (int j = 0; j < S::STAGES && i + j * CATT_WARPS < u.tiles; ++j)
+        mbar_wait_warp(&sm.full[w][(turn + j) % S::STAGES], (turn + j) / S::STAGES & 1, nullptr, 0, nullptr, a.wait_ns);
+      break;
+    }
     const uint32_t base = smem_u32(sm.ring[w][slot]);
 
     float s[4][4];
@@ -417,8 +428,15 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   }
   row.finish();
 
+  if (__syncthreads_or(late)) {  // also: the rings are free
+    const float none[4] = {};
+    for (int i = tid; i < 16 * D / 4 && u.row0 + i / (D / 4) < u.rows; i += CATT_WARPS * 32) {
+      const int r = u.row0 + i / (D / 4);
+      attn_put<T, D>(a, u, u.first + r / u.G, u.h * u.G + r % u.G, i % (D / 4) * 4, none, 0.f, NAN, 0.f);
+    }
+    return;
+  }
   // join the four warps; a lane has eight neighbouring dimensions of each 32
-  __syncthreads();  // the rings are free
   float* all = reinterpret_cast<float*>(sm.ring[0][0]);  // [warp][16][D]
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -516,7 +534,7 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     if (lane == 0) {
       constexpr uint32_t idS = idesc_f16_f32(CATP_ROWS, CATP_TK, false), idO = idesc_f16_f32(CATP_ROWS, 64, true);
       const auto scores = [&](int i) {
-        if (!mbar_wait(&sm.k_full, i & 1, nullptr, 0, abort)) return false;
+        if (!mbar_wait(&sm.k_full, i & 1, nullptr, 0, abort, a.wait_ns)) return false;
         tc_fence_after();
 #pragma unroll
         for (int b = 0; b < D / 64; ++b)
@@ -528,10 +546,10 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         umma_commit(&sm.k_free);
         return true;
       };
-      bool ok = mbar_wait(&sm.q_full, 0, nullptr, 0, abort) && scores(0) && (u.tiles < 2 || scores(1));
+      bool ok = mbar_wait(&sm.q_full, 0, nullptr, 0, abort, a.wait_ns) && scores(0) && (u.tiles < 2 || scores(1));
       for (int i = 0; ok && i < u.tiles; ++i) {
         const int b = i & 1;
-        ok = mbar_wait(&sm.p_full[b], i >> 1 & 1, nullptr, 0, abort) && mbar_wait(&sm.v_full[b], i >> 1 & 1, nullptr, 0, abort);
+        ok = mbar_wait(&sm.p_full[b], i >> 1 & 1, nullptr, 0, abort, a.wait_ns) && mbar_wait(&sm.v_full[b], i >> 1 & 1, nullptr, 0, abort, a.wait_ns);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -546,15 +564,16 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         if (i + 2 < u.tiles) ok = scores(i + 2);
       }
       umma_commit(&sm.drain);
-      mbar_wait(&sm.drain, 0, nullptr, 0, nullptr);
+      mbar_wait(&sm.drain, 0, nullptr, 0, nullptr, a.wait_ns);
     }
   } else if (w >= 4) {
     // 16 codes at a time: 64 x D / 16 pieces of keys and as many of values over 128 threads
     constexpr int ITEMS = CATP_TK * (D / 16) / 128;
     const int t = tid - 128;
-    if (w == 4) attn_issue<D, CATP_TK>(c, u, sm.page, k_map, v_map, 0, sm.codes, &sm.raw_full);
-    for (int i = 0; i < u.tiles; ++i) {
-      if (!mbar_wait_warp(&sm.raw_full, i & 1, nullptr, 0, abort)) break;
+    int i = 0, issued = 1;  // tiles taken, tiles asked for
+    if (w == 4) attn_issue<D, CATP_TK>(c, a, u, sm.page, k_map, v_map, 0, sm.codes, &sm.raw_full);
+    for (; i < u.tiles; ++i) {
+      if (!mbar_wait_warp(&sm.raw_full, i & 1, nullptr, 0, abort, a.wait_ns)) break;
       uint4 codes[2][ITEMS];
 #pragma unroll
       for (int x = 0; x < 2 * ITEMS; ++x) {
@@ -565,14 +584,15 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.raw_free);
       if (w == 4 && i + 1 < u.tiles) {  // the next tile may come when all codes are in registers
-        if (!mbar_wait_warp(&sm.raw_free, i & 1, nullptr, 0, abort)) break;
-        attn_issue<D, CATP_TK>(c, u, sm.page, k_map, v_map, i + 1, sm.codes, &sm.raw_full);
+        if (!mbar_wait_warp(&sm.raw_free, i & 1, nullptr, 0, abort, a.wait_ns)) break;
+        attn_issue<D, CATP_TK>(c, a, u, sm.page, k_map, v_map, i + 1, sm.codes, &sm.raw_full);
+        ++issued;
       }
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         // the product that read this buffer last
-        if (which == 0 && i > 0 && !mbar_wait_warp(&sm.k_free, (i - 1) & 1, nullptr, 0, abort)) goto done;
-        if (which == 1 && i > 1 && !mbar_wait_warp(&sm.pv_done[i & 1], ((i >> 1) - 1) & 1, nullptr, 0, abort)) goto done;
+        if (which == 0 && i > 0 && !mbar_wait_warp(&sm.k_free, (i - 1) & 1, nullptr, 0, abort, a.wait_ns)) goto done;
+        if (which == 1 && i > 1 && !mbar_wait_warp(&sm.pv_done[i & 1], ((i >> 1) - 1) & 1, nullptr, 0, abort, a.wait_ns)) goto done;
 #pragma unroll
         for (int x = 0; x < ITEMS; ++x) {
           const int j = t + x * 128, row = j / (D / 16), piece = j % (D / 16);
@@ -594,7 +614,9 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         if (lane == 0) mbar_arrive(which ? &sm.v_full[i & 1] : &sm.k_full);
       }
     }
-  done:;
+  done:
+    // what is in flight lands before the block ends
+    if (w == 4 && i < u.tiles) mbar_wait_warp(&sm.raw_full, (issued - 1) & 1, nullptr, 0, nullptr, a.wait_ns);
   } else {
     // the row as f16, in the order of the products' operand
     float factor;
@@ -628,7 +650,7 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       const int b = i & 1, key = u.lo + i * CATP_TK, pg = (key >> u.shift) - (u.lo >> u.shift), in = key & (c.page - 1);
       // columns that this row sees: [from, upto)
       const int upto = min(pos + 1, u.hi) - key, from = pos - u.window - key;
-      if (!mbar_wait_warp(&sm.s_full[b], i >> 1 & 1, nullptr, 0, abort)) {
+      if (!mbar_wait_warp(&sm.s_full[b], i >> 1 & 1, nullptr, 0, abort, a.wait_ns)) {
         ok = false;
         break;
       }
@@ -665,7 +687,7 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       }
       if (i > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
         // the outputs so far, when the product before has completed
-        if (!mbar_wait_warp(&sm.pv_done[b ^ 1], (i - 1) >> 1 & 1, nullptr, 0, abort)) {
+        if (!mbar_wait_warp(&sm.pv_done[b ^ 1], (i - 1) >> 1 & 1, nullptr, 0, abort, a.wait_ns)) {
           ok = false;
           break;
         }
@@ -698,7 +720,7 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.p_full[b]);
     }
-    if (ok && mbar_wait_warp(&sm.o_full, 0, nullptr, 0, abort)) {
+    if (ok && mbar_wait_warp(&sm.o_full, 0, nullptr, 0, abort, a.wait_ns)) {
       tc_fence_after();
 #pragma unroll 1
       for (int d = 0; d < D; d += 32) {
@@ -706,6 +728,10 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         tmem_ld32(tmem + lanes + CATP_TMEM_O + d, t);
         if (real) attn_put<T, D>(a, u, at_row, head, d, t, v_top, attn_sum(l, m, factor), m);
       }
+    } else if (real) {  // a wait has run out
+      const float none[8] = {};
+#pragma unroll 1
+      for (int d = 0; d < D; d += 8) attn_put<T, D>(a, u, at_row, head, d, none, 0.f, NAN, 0.f);
     }
   }
   __syncwarp();

@@ -8,6 +8,7 @@
 #include <climits>
 #include <cmath>
 #include <string>
+#include <vector>
 
 #include "errors.h"
 #include "launch.h"
@@ -158,6 +159,51 @@ void launch_attention(const CacheView& c, const CacheAttnArgs& a, bool prompt, i
   c.dim == 64 ? launch_attention<T, 64>(c, a, prompt, dev, st) : launch_attention<T, 128>(c, a, prompt, dev, st);
 }
 
+// Attention of `rows` queries over `keys` positions whose loads are waited for in vain; true if every row came
+// out as NaN, and a call without the fault has none.
+bool attention_gives_up(int device, int dim, int rows, int keys, uint64_t wait_ns) {
+  struct Buffer {
+    void* p = nullptr;
+    explicit Buffer(size_t bytes) {
+      CK(cudaMalloc(&p, bytes));
+      const cudaError_t e = cudaMemset(p, 0, bytes);
+      if (e != cudaSuccess) cudaFree(p);
+      CK(e);
+    }
+    ~Buffer() { cudaFree(p); }
+  };
+  const int page = 16, pages = (keys + page - 1) / page;
+  Buffer k((size_t)pages * page * dim), v((size_t)pages * page * dim), ks(pages * 4), vs(pages * 4), q((size_t)rows * dim * 2),
+      out((size_t)rows * dim * 2), lse(rows * 4), cu(8), len(4), table(pages * 4);
+  const CacheView c{{static_cast<int8_t*>(k.p), static_cast<int8_t*>(v.p)}, {static_cast<float*>(ks.p), static_cast<float*>(vs.p)}, pages, page, 1, dim};
+  const AttnPlan p = plan_attention(c, 1, 1, rows, keys);
+  Buffer ws(std::max<size_t>(16, attention_workspace(p, c, 1, 1, rows)));
+  std::vector<int> order(pages);
+  for (int i = 0; i < pages; ++i) order[i] = i;
+  const int ends[2] = {0, rows};
+  CK(cudaMemcpy(table.p, order.data(), pages * 4, cudaMemcpyHostToDevice));
+  CK(cudaMemcpy(cu.p, ends, 8, cudaMemcpyHostToDevice));
+  CK(cudaMemcpy(len.p, &keys, 4, cudaMemcpyHostToDevice));
+  CacheAttnArgs a{q.p, out.p, static_cast<float*>(lse.p), dim, dim, static_cast<int*>(cu.p), static_cast<int*>(len.p),
+                  static_cast<int*>(table.p), 1, 1, pages, rows, -1, p.tiles, p.chunk, p.chunks, 1.f};
+  a.part = static_cast<float*>(ws.p);
+  a.part_lse = a.part + (size_t)rows * p.chunks * dim;
+  a.wait_ns = wait_ns;
+  for (int beyond : {16, 0}) {
+    a.beyond = beyond;
+    launch_attention<__half>(c, a, p.prompt, device, nullptr);
+    CK(cudaDeviceSynchronize());
+    std::vector<uint16_t> o((size_t)rows * dim);
+    std::vector<float> l(rows);
+    CK(cudaMemcpy(o.data(), out.p, o.size() * 2, cudaMemcpyDeviceToHost));
+    CK(cudaMemcpy(l.data(), lse.p, l.size() * 4, cudaMemcpyDeviceToHost));
+    const auto nan = [](uint16_t h) { return (h & 0x7fff) > 0x7c00; };
+    const int64_t nans = std::count_if(o.begin(), o.end(), nan) + std::count_if(l.begin(), l.end(), [](float x) { return std::isnan(x); });
+    if (nans != (beyond ? (int64_t)(o.size() + l.size()) : 0)) return false;
+  }
+  return true;
+}
+
 // A row is shared by a cluster of up to eight blocks, as long as there are SMs for them and each keeps a
 // thousand logits.
 template <typename T>
@@ -289,6 +335,17 @@ s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, const void
       launch_attention<__half>(c, a, p.prompt, dev.device, st);
     else
       launch_attention<__nv_bfloat16>(c, a, p.prompt, dev.device, st);
+  });
+}
+
+s1c_status s1c_selftest_cache_attention_timeout(int32_t device, int64_t budget_ns, int32_t* codes) {
+  return enter([&] {
+    need(codes && budget_ns >= 1000000 && budget_ns <= 2000000000, "budget_ns must lie in [1e6, 2e9] and codes must not be null");
+    CK(cudaSetDevice(device));
+    for (int i = 0; i < 4; ++i) {
+      const int rows = i < 2 ? 3 : 40, keys = i % 2 ? 1000 : 100;
+      codes[i] = attention_gives_up(device, 64, rows, keys, (uint64_t)budget_ns) && attention_gives_up(device, 128, rows, keys, (uint64_t)budget_ns);
+    }
   });
 }
 

@@ -603,6 +603,20 @@ def test_cache_attention_queries_that_are_not_finite_and_see_no_key(ops, H, G, D
     assert torch.isfinite(seen).all() and seen.any()
 
 
+def test_cache_attention_waits_that_run_out_give_nan(ops):
+    """A tile of keys that never comes (short waits, the library's own self-test): the rows are NaN, split keys or not,
+    few rows or many, and the kernels end; calls behind it are as ever."""
+    import time
+    from sys1rust_b200 import backend
+    t = time.perf_counter()
+    assert backend.selftest_cache_attention_timeout(0, 10_000_000) == [1, 1, 1, 1]
+    assert time.perf_counter() - t < 5
+    c = Paged(ops, 1, 300, 2, 64, 16, 77)
+    q = torch.randn(2, 4 * 64, generator=_gen(78), device="cuda").half()
+    out, lse = _attention(ops, c, q, 4, [2], [300], 0.1)
+    _check_attention(c, q, 4, [2], [300], 0.1, -1, out, lse)
+
+
 def test_cache_attention_long_cache(ops):
     """70001 positions, more than 2^31 bytes into the codes' array for the last pages."""
     H, D, page, L = 8, 128, 64, 70001

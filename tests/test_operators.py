@@ -214,3 +214,10 @@ def test_kernels_hold_their_tmem_before_a_successor_may_start():
                 assert trigger is None or re.search("__syncthreads|cluster_sync_all|attn_pages", body[alloc.end(): trigger.start()]), name
                 checked.append(name)
     assert "cache_attention.cuh" in checked and "gemm_sm100_csk.cuh" in checked
+
+
+def test_attention_timeout_selftest_checks_its_arguments():
+    for budget in (0, 10, 3 * 10 ** 9):
+        with pytest.raises(BackendError):
+            bk.selftest_cache_attention_timeout(0, budget)
+    assert bk.lib().s1c_selftest_cache_attention_timeout(0, 10 ** 7, None) == bk.S1C_ERR_ARG
