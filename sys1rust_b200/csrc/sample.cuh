@@ -611,8 +611,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
   const int k = a.top_k ? a.top_k[r] : 0;
   const float p = a.top_p ? a.top_p[r] : 1.f, mp = a.min_p ? a.min_p[r] : 0.f;
   const bool by_k = k > 0 && k < a.vocab, by_p = p < 1.f, by_m = mp > 0.f;
-  // e >= min_p as a bound on the logit
-  const double least = by_m ? (double)top + (double)T_ * log(fmin((double)mp, 1.0)) : -INFINITY;
+  // e >= min_p as a bound on the logit; an infinite T makes all e 1
+  const double least = by_m && T_ < INFINITY ? (double)top + (double)T_ * log(fmin((double)mp, 1.0)) : -INFINITY;
 
   // 2. Counts of the bins, and a bin that ends before anything that is kept.
   unsigned long long total = 0;

@@ -785,6 +785,34 @@ def test_sample_rows_without_a_distribution_and_odd_parameters(ops, dt):
         assert near < 3e-7 or (token[r] == want and abs(prob[r] - pw) <= 3e-7 * pw), r
 
 
+@pytest.mark.parametrize("V", [5, 700, 50368])
+def test_sample_infinite_temperature_with_filters(ops, V):
+    """At T = inf every finite logit has e = 1: min-p keeps all of them, up to its largest value of 1; top-k and top-p
+    keep the first ones in the order of the logits. 1 and above is one value of min-p at any temperature."""
+    R = 12
+    x = torch.randn(R, V, generator=_gen(98), device="cuda")
+    x[:, 1] = -math.inf
+    u = torch.rand(R, generator=_gen(99), device="cuda")
+    T = torch.full((R,), math.inf, device="cuda")
+    m = torch.tensor([0.0, 0.3, 1.0, 7.0, math.inf, 1e-38] * 2, device="cuda")
+    k = torch.where(torch.arange(R, device="cuda") < 6, 0, 3).to(torch.int32)
+    p = torch.where(torch.arange(R, device="cuda") % 2 == 0, 1.0, 0.49)
+    for top_p in (None, p):
+        token, prob = _sample(ops, x, u, T, k, top_p, m)
+        for r in range(R):
+            row = x[r].cpu().numpy()
+            order = np.lexsort((np.arange(V), -row))[: V - 1]
+            order = order[: 3] if k[r] else order
+            if top_p is not None and p[r] < 1:  # those before which less than p of the mass lies
+                order = order[: int(np.ceil(float(p[r]) * order.size))]
+            order = np.sort(order)
+            at = float(u[r]) * order.size
+            assert abs(at - round(at)) < 1e-3 or token[r] == order[int(at)], (r, token[r])
+            assert abs(prob[r] * order.size - 1) < 1e-6
+    token, prob = _sample(ops, x, u, None, None, None, torch.full((R,), 3.0, device="cuda"))
+    assert (token == x.argmax(1).cpu().numpy()).all() and (prob == 1).all()
+
+
 def test_sample_values_over_the_whole_range(ops):
     """Logits from the smallest to the largest floats: a cut far below the largest, in one bin with others."""
     V, R = 3000, 8
