@@ -18,10 +18,11 @@
 //     one value is left. What is kept is summed and walked. More than fit in the list are worked on in place.
 //
 // Masses are integers: e = m * 2^(n - 24), m an integer of 25 bits, and all e in one bin share n. So their
-// sums are exact and depend neither on the order of atomics nor on how a row is shared. One sum is not of
-// this kind: where top-p counts the mass of a whole row, what lies below 1/16 of the largest is summed in
-// fp32 by each thread first, in a fixed order. Logits more than 45 powers of two below the largest have no
-// mass.
+// sums are exact and depend neither on the order of atomics nor on how a row is shared. One sum is rounded:
+// where top-p counts the mass of a whole row, what lies below 1/16 of the largest, or below min-p, enters as
+// fp32 sums of the four or eight neighbours that a load brings, and these as integers. They do not depend on
+// how a row is shared either, so a row gets the same token in every batch. Logits more than 45 powers of two
+// below the largest have no mass.
 //
 // Measured: 1 x 50368 fp32, top-k 50 and top-p: 17.0 us, of which the exchanges of the eight blocks are
 // about half; 256 x 50368 bf16, top-p and min-p: 49 us, where the pass that counts and sums (25 instructions
@@ -623,11 +624,10 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
     const bool sums = by_p && !by_k;
     // what min-p drops is not counted, unless top-p needs the mass of all that top-k keeps
     if (by_m && !(by_k && by_p)) bound = min(bound, (int)fmin(-log2(fmin((double)mp, 1.0)) * 32.0, (double)SMP_ZBINS) + 1);
-    float small = 0.f;  // masses below 1/16, by the hardware's exp2: errors of 2^-22 of them are far below the sum's own
     const float reach = (bound + 1) * 0.03125f;
 #pragma unroll 2
     for (int i = t * E; i < n; i += SMP_THREADS * E) {
-      float x[E];
+      float x[E], small = 0.f;  // by the hardware's exp2: errors of 2^-22 of masses that are small or that min-p drops
       load(x, i);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -639,8 +639,9 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_kernel(const SampleArgs
         }
         if (sums && !(z < fminf(4.f, reach))) small += exp2_approx(-fminf(z, 200.f));
       }
+      if (sums) total += (unsigned long long)(small * 0x1p44f);
     }
-    if (sums) total = sample_sum(s, total + (unsigned long long)(small * 0x1p44f));
+    if (sums) total = sample_sum(s, total);
     __syncthreads();
     // the counts of this thread's bins, in this block and in all
     constexpr int PER = (SMP_ZBINS + SMP_THREADS * 4 - 1) / (SMP_THREADS * 4) * 4;

@@ -813,6 +813,23 @@ def test_sample_infinite_temperature_with_filters(ops, V):
     assert (token == x.argmax(1).cpu().numpy()).all() and (prob == 1).all()
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("m,size", [(0.0, 2.5), (0.2, 0.5)])
+def test_sample_rows_do_not_depend_on_their_batch(ops, dt, m, size):
+    """The same row with the same numbers gives the same token and the same bits of its share alone (shared by eight
+    blocks) and in a batch (one block a row), with values of top-p right at a border between two tokens."""
+    V, R = 50368, 160
+    x = (torch.randn(1, V, generator=_gen(96), device="cuda") * size).to(DT[dt])
+    cum = np.cumsum(np.exp(np.sort(x[0].double().cpu().numpy())[::-1] - x.double().max().item()))
+    p = torch.from_numpy((cum / cum[-1])[np.linspace(1, 3000, R).astype(int)].astype(np.float32)).cuda()
+    u, mp = torch.full((R,), 0.9999, device="cuda"), torch.full((R,), m, device="cuda")
+    token, prob = _sample(ops, x.expand(R, V).contiguous(), u, None, None, p, mp)
+    alone = [_sample(ops, x, u[r: r + 1], None, None, p[r: r + 1], mp[r: r + 1]) for r in range(R)]
+    assert token.tolist() == [int(t[0]) for t, _ in alone]
+    assert prob.tolist() == [float(q[0]) for _, q in alone]
+    assert len(set(prob.tolist())) > R / 2
+
+
 def test_sample_values_over_the_whole_range(ops):
     """Logits from the smallest to the largest floats: a cut far below the largest, in one bin with others."""
     V, R = 3000, 8
