@@ -114,23 +114,49 @@ struct AttnPlan {
   bool prompt;
   int tiles, chunk, chunks;
 };
+constexpr int ATTN_FEW_ROWS = 32;                              // of a key head: up to here blocks of 16 rows
+constexpr int ATTN_FEW_ROUND = 444, ATTN_PROMPT_ROUND = 296;  // blocks that 148 SMs hold: three each, or two of a prompt's
+constexpr int ATTN_PROMPT_WHOLE = 148;                         // prompts' blocks from which keys stay together where they may
+int64_t chunk_most(const CacheView& c, bool prompt) {
+  return prompt ? (int64_t)CATP_PAGES * c.page - 128 : std::min<int64_t>(2048, (int64_t)CATT_PAGES * c.page);
+}
 AttnPlan plan_attention(const CacheView& c, int heads, int n, int max_q, int max_kv) {
   const int64_t rows = (int64_t)max_q * (heads / c.heads);
   AttnPlan p;
-  p.prompt = rows > 32;
+  p.prompt = rows > ATTN_FEW_ROWS;
   const int per = p.prompt ? CATP_ROWS : 16;
   p.tiles = (int)((rows + per - 1) / per);
   const int64_t units = (int64_t)n * c.heads * p.tiles;
-  // one round of the blocks that 148 SMs hold, three each, or two of a prompt's
-  const int64_t round = p.prompt ? 296 : 444, want = (units * max_kv + round - 1) / round;
-  const int64_t most = p.prompt ? (int64_t)CATP_PAGES * c.page - 128 : std::min<int64_t>(2048, (int64_t)CATT_PAGES * c.page);
+  // one round of blocks
+  const int64_t round = p.prompt ? ATTN_PROMPT_ROUND : ATTN_FEW_ROUND, want = (units * max_kv + round - 1) / round;
+  const int64_t most = chunk_most(c, p.prompt);
   p.chunk = (int)std::max<int64_t>(128, std::min(most, (want + 127) / 128 * 128));
-  if (p.prompt && units >= 148 && max_kv <= most) p.chunk = (int)most;
+  if (p.prompt && units >= ATTN_PROMPT_WHOLE && max_kv <= most) p.chunk = (int)most;
   p.chunks = (int)std::max<int64_t>(1, ((int64_t)max_kv + p.chunk - 1) / p.chunk);
   return p;
 }
-size_t attention_workspace(const AttnPlan& p, const CacheView& c, int heads, int n, int max_q) {
+// What a call writes there: dim + 1 numbers for each row, head and chunk.
+size_t attention_partials(const AttnPlan& p, const CacheView& c, int heads, int n, int max_q) {
   return p.chunks == 1 ? 0 : (size_t)n * max_q * heads * p.chunks * (c.dim + 1) * sizeof(float);
+}
+// What a call needs if it splits keys at all: enough for every call with bounds up to these, so that one buffer
+// serves all of them, although a smaller call may split its keys more. A chunk has its largest size, and there
+// are ceil(kv / most); or at least units * kv / round keys, so ceil(round / units) of them at most, for no more
+// than `per` rows and heads in each of fewer than `round` units; and 128 keys at least.
+size_t attention_workspace(const CacheView& c, int heads, int n, int max_q, int max_kv) {
+  const int64_t G = heads / c.heads, least = ((int64_t)max_kv + 127) / 128;
+  int64_t parts = 0;
+  const auto form = [&](bool prompt, int64_t q, int64_t per, int64_t round, int64_t units) {
+    const int64_t items = (int64_t)n * q * heads, largest = (max_kv + chunk_most(c, prompt) - 1) / chunk_most(c, prompt);
+    if (max_kv > chunk_most(c, prompt))
+      parts = std::max(parts, items * largest);
+    else if (prompt)
+      units = std::min<int64_t>(units, ATTN_PROMPT_WHOLE);
+    if (least > 1) parts = std::max(parts, std::min(items * least, per * (round + units - 1)));
+  };
+  form(false, std::min<int64_t>(max_q, ATTN_FEW_ROWS / G), 16, ATTN_FEW_ROUND, ATTN_FEW_ROUND);
+  if (max_q * G > ATTN_FEW_ROWS) form(true, max_q, CATP_ROWS, ATTN_PROMPT_ROUND, ATTN_PROMPT_ROUND);
+  return (size_t)parts * (c.dim + 1) * sizeof(float);
 }
 
 template <typename T, int D>
@@ -177,7 +203,7 @@ bool attention_gives_up(int device, int dim, int rows, int keys, uint64_t wait_n
       out((size_t)rows * dim * 2), lse(rows * 4), cu(8), len(4), table(pages * 4);
   const CacheView c{{static_cast<int8_t*>(k.p), static_cast<int8_t*>(v.p)}, {static_cast<float*>(ks.p), static_cast<float*>(vs.p)}, pages, page, 1, dim};
   const AttnPlan p = plan_attention(c, 1, 1, rows, keys);
-  Buffer ws(std::max<size_t>(16, attention_workspace(p, c, 1, 1, rows)));
+  Buffer ws(std::max<size_t>(16, attention_partials(p, c, 1, 1, rows)));
   std::vector<int> order(pages);
   for (int i = 0; i < pages; ++i) order[i] = i;
   const int ends[2] = {0, rows};
@@ -296,7 +322,7 @@ size_t s1c_cache_attention_workspace(const s1c_cache* cache, int32_t heads, int3
   try {
     const CacheView c = check_cache(cache);
     if (heads <= 0 || heads % c.heads || n <= 0 || max_q <= 0 || max_kv <= 0) return 0;
-    return attention_workspace(plan_attention(c, heads, n, max_q, max_kv), c, heads, n, max_q);
+    return attention_workspace(c, heads, n, max_q, max_kv);
   } catch (...) {
     return 0;  // a cache that the call refuses
   }
@@ -321,7 +347,8 @@ s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, const void
     if (n == 0 || max_q == 0) return;
     need((int64_t)n * max_q <= INT_MAX / heads, "n * max_q * heads must stay below 2^31");
     const AttnPlan p = plan_attention(c, heads, n, max_q, max_kv);
-    const size_t bytes = attention_workspace(p, c, heads, n, max_q);
+    const size_t used = attention_partials(p, c, heads, n, max_q);
+    const size_t bytes = used ? std::max(used, attention_workspace(c, heads, n, max_q, max_kv)) : 0;
     need(p.chunks <= 65535, "max_kv is too large");
     need(workspace_bytes >= bytes && (!bytes || (d_workspace && aligned(d_workspace, 16))),
          "workspace too small, null or not 16-byte aligned");

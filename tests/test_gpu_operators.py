@@ -603,6 +603,31 @@ def test_cache_attention_queries_that_are_not_finite_and_see_no_key(ops, H, G, D
     assert torch.isfinite(seen).all() and seen.any()
 
 
+def test_cache_attention_one_workspace_for_smaller_calls(ops):
+    """One buffer of the largest batch's size, with known bytes behind it, through calls that shrink in every
+    direction and split their keys more than the largest does."""
+    H, G, D, L = 2, 4, 64, 3000
+    c = Paged(ops, 40, L, H, D, 16, 79)
+    size = ops.cache_attention_workspace(c.handle, H * G, 40, 20, L)
+    ws = torch.full((size + 64,), 7, dtype=torch.uint8, device="cuda")
+    split = 0
+    for n, rows, keys in [(40, 1, 2000), (9, 1, L), (1, 1, L), (1, 1, 200), (2, 20, L), (1, 9, 700), (40, 2, 150), (1, 1, 64)]:
+        lens, at = [rows] * n, [max(rows, keys - 3 * i) for i in range(n)]
+        q = torch.randn(n * rows, H * G * D, generator=_gen(80), device="cuda").bfloat16()
+        out = torch.full((n * rows + 1, H * G * D + 8), 5.0, dtype=torch.bfloat16, device="cuda")
+        lse = torch.full((n * rows + 1, H * G), 5.0, device="cuda")
+        cu, ln = _i32([i * rows for i in range(n + 1)]), _i32(at)
+        ws[:size] = 7
+        ops.cache_attention(c.handle, ops.DT_BF16, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), H * G, cu.data_ptr(),
+                            ln.data_ptr(), c.table.data_ptr(), c.table.shape[1], n, rows, keys, 0.125, lse_ptr=lse.data_ptr(),
+                            workspace_ptr=ws.data_ptr(), workspace_bytes=size, stream=_stream())
+        torch.cuda.synchronize()
+        assert (ws[size:] == 7).all()
+        split += int((ws[:size] != 7).any())
+        _check_attention(c, q, H * G, lens, at, 0.125, -1, out, lse)
+    assert 2 <= split < 8
+
+
 def test_cache_attention_waits_that_run_out_give_nan(ops):
     """A tile of keys that never comes (short waits, the library's own self-test): the rows are NaN, split keys or not,
     few rows or many, and the kernels end; calls behind it are as ever."""

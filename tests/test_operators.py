@@ -112,6 +112,36 @@ def test_cache_attention_refuses_a_short_workspace():
     assert bk.lib().s1c_cache_attention_workspace(None, 4, 1, 1, 100000) == 0
 
 
+@pytest.mark.parametrize("heads,kv_heads,page,dim", [(8, 8, 16, 64), (32, 8, 16, 128), (4, 4, 64, 128), (80, 2, 32, 64),
+                                                     (16, 1, 16, 128)])
+def test_cache_attention_workspace_serves_smaller_calls(heads, kv_heads, page, dim):
+    """The workspace of some bounds is accepted by every call with smaller ones, however these split their keys; sizes
+    next to those at which the split changes are among them. The calls stop at their host memory, behind the check."""
+    c = _cache(kv_heads=kv_heads, head_dim=dim, page=page)
+    rng = np.random.default_rng(5)
+    kvs = [1, 128, 129, 2048, 2049, 256 * page - 128, 256 * page - 127, 30000, 131072]
+    qs = sorted({1, 2, 32 * kv_heads // heads or 1, 32 * kv_heads // heads + 1, 128, 500})
+
+    def call(n, q, kv, size):
+        with pytest.raises(BackendError) as e:
+            ops.cache_attention(**_attend(cache=c, heads=heads, q_stride=heads * dim, out_stride=heads * dim, n=n, max_q=q, max_kv=kv,
+                                          workspace_bytes=size))
+        return str(e.value)
+
+    for n, q, kv in [(64, 1, 2048), (64, 1, 8192), (37, 1, 131072), (4, 500, 4000), (300, 40, 5000), (148, 128, 3968), (1, 1, 200)]:
+        size = ops.cache_attention_workspace(c, heads, n, q, kv)
+        # what the call itself checks for
+        if size:
+            short = call(n, q, kv, size - 1)
+            assert "workspace" in short or "workspace" not in call(n, q, kv, 0)  # a call that needs none takes none
+        assert "workspace" not in call(n, q, kv, size)
+        smaller = [(a, b, k) for a in (1, 2, 3, 5, 18, 19, 55, 56, 64, 148) for b in qs for k in kvs]
+        for a, b, k in [smaller[i] for i in rng.permutation(len(smaller))[:150]] + [(1, 1, kv), (1, q, kv), (n // 2, q, kv // 2)]:
+            a, b, k = max(1, min(a, n)), min(b, q), max(1, min(k, kv))
+            assert ops.cache_attention_workspace(c, heads, a, b, k) <= size, (a, b, k)
+            assert "workspace" not in call(a, b, k, size), (a, b, k)
+
+
 @pytest.mark.parametrize("bad,text", [
     (dict(dtype=3), "dtype"), (dict(logits_ptr=0), "null"), (dict(uniform_ptr=0), "null"), (dict(token_ptr=0), "null"),
     (dict(rows=-1), "rows"), (dict(vocab=0), "vocab"), (dict(vocab=(1 << 20) + 1, row_stride=1 << 22), "vocab"),
