@@ -55,6 +55,9 @@ struct CskArgs {
   // 16 bytes at a 16-byte-aligned address.
   const void* pf;
   size_t pf_bytes;
+  // B is not written on the stream (a handle's weights): it is loaded before the wait for the kernel before.
+  // Where B is the caller's, that kernel may be what writes it.
+  int fixed_b;
 };
 
 // Largest cluster the launch plan uses. In the single-request forward (CUDA graph, weights streaming from HBM) clusters of 8 measured slower than
@@ -348,6 +351,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           tma_load_2d(sB + s * B_BYTES, &tmB, &full[s], kb * BK, n0);
         }
       };
+      if (!args.fixed_b) pdl_wait();
       const int pre = nkb < STAGES ? nkb : STAGES;
       for (int i = 0; i < pre; ++i) {
         mbar_arrive_expect_tx(&full[i], STAGE_BYTES);

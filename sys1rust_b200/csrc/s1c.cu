@@ -235,9 +235,7 @@ struct SplitCtx {
   size_t ws_bytes;
   void* out;
   int ldo;
-  // B is not written on the stream (a handle's weights): the cluster kernel loads it before it waits for the
-  // kernel before it. Where B is the caller's, that kernel may be what writes it.
-  bool fixed_b = true;
+  bool fixed_b = true;  // CskArgs::fixed_b
 };
 
 // Split-K factor for a GEMM with few output tiles: enough splits to cover the SMs, at least one
@@ -277,7 +275,7 @@ CskPlan plan_csk(int M, int N, int K, int num_sms, bool geglu) {
 }
 
 template <int BN, int EPI>
-void launch_csk_bn(const CUtensorMap& ta, const CUtensorMap& tb, const CskArgs& a, int tiles, bool fixed_b, cudaStream_t st) {
+void launch_csk_bn(const CUtensorMap& ta, const CUtensorMap& tb, const CskArgs& a, int tiles, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * a.C));
   cfg.blockDim = dim3(GEMM_THREADS);
@@ -291,7 +289,7 @@ void launch_csk_bn(const CUtensorMap& ta, const CUtensorMap& tb, const CskArgs& 
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = t_pdl && fixed_b ? 2 : 1;
+  cfg.numAttrs = t_pdl ? 2 : 1;
   CK(cudaLaunchKernelEx(&cfg, gemm_csk_sm100<BN, EPI>, ta, tb, a));
 }
 
@@ -306,11 +304,12 @@ void launch_csk(const CUtensorMap& ta, const WeightMap& tb, const GemmArgs& g, c
   a.pos = g.pos; a.inv_freq = g.inv_freq; a.rope_cols = g.rope_cols; a.out_cols = g.out_cols;
   a.status = g.status;
   a.pf = g.pf; a.pf_bytes = g.pf_bytes;
+  a.fixed_b = sk.fixed_b;
   if constexpr (EPI == EPI_GEGLU) {
-    launch_csk_bn<128, EPI>(ta, tb.quarter, a, p.tiles, sk.fixed_b, st);
+    launch_csk_bn<128, EPI>(ta, tb.quarter, a, p.tiles, st);
   } else {
-    if (p.bn == 128) launch_csk_bn<128, EPI>(ta, tb.half, a, p.tiles, sk.fixed_b, st);
-    else launch_csk_bn<64, EPI>(ta, tb.quarter, a, p.tiles, sk.fixed_b, st);
+    if (p.bn == 128) launch_csk_bn<128, EPI>(ta, tb.half, a, p.tiles, st);
+    else launch_csk_bn<64, EPI>(ta, tb.quarter, a, p.tiles, st);
   }
 }
 

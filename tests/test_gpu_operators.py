@@ -1168,3 +1168,37 @@ def test_gemm_whose_second_matrix_an_operator_wrote(ops, eager):
     want = a.double() @ seen.double().transpose(1, 2)
     most = a.double().abs() @ seen.double().abs().transpose(1, 2)
     assert ((out.double() - want).abs() <= _u(torch.bfloat16) * want.abs() + (1 + 2.0 ** -8) * K * 2.0 ** -22 * most).all()
+
+
+def test_gemm_with_few_rows_is_scheduled_while_the_kernel_before_it_ends(ops):
+    """In a captured graph the edge into ``s1c_gemm``'s cluster kernel is a programmatic one, so that its set-up
+    overlaps the end of the kernel before it."""
+    import ctypes
+    from sys1rust_b200 import backend
+    M, N, K = 16, 64, 2048
+    g = _gen(7)
+    a, b = [torch.randn(r, K, generator=g, device="cuda").bfloat16() for r in (M, N)]
+    out = torch.zeros(2, M, N, dtype=torch.bfloat16, device="cuda")
+
+    def run():
+        for o in out:
+            backend.gemm(backend.EPI_STORE, a.data_ptr(), b.data_ptr(), o.data_ptr(), M, N, K, stream=_stream())
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        run()
+
+    class Edge(ctypes.Structure):
+        _fields_ = [("from_port", ctypes.c_ubyte), ("to_port", ctypes.c_ubyte), ("type", ctypes.c_ubyte), ("reserved", ctypes.c_ubyte * 5)]
+
+    get = ctypes.CDLL("libcudart.so.12").cudaGraphGetEdges_v2
+    handle, count = ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t(8)
+    ends, edges = [(ctypes.c_void_p * 8)() for _ in range(2)], (Edge * 8)()
+    assert get(handle, ends[0], ends[1], edges, ctypes.byref(count)) == 0
+    assert [e.type for e in edges[: count.value]] == [1]  # the one edge: programmatic
+    graph.instantiate()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], out[1]) and out.any()
