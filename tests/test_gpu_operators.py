@@ -183,6 +183,85 @@ def test_nibble_gemm_is_bitwise_repeatable_and_row_independent(ops):
     assert ((out.double() - ref).abs() <= xs.double().abs() @ (0.51 * step).t() + 1e-3).all()
 
 
+WIDE = [(1, 70, 90001, 128), (10, 17, 100000, 32), (3, 300, 120001, 64), (8, 33, 300000, 128), (64, 31, 5000, 64), (45, 70, 9000, 32),
+        (64, 50, 16000, 128), (17, 129, 9900, 64), (8, 100, 9000, 32), (16, 70, 6001, 64), (12, 300, 8192, 128), (6, 40, 30000, 64),
+        (3, 2400, 12000, 128), (1, 5000, 2624, 64), (33, 260, 2047, 32)]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("M,N,K,group", WIDE)
+def test_nibble_gemm_whole_numbers_are_exact(ops, M, N, K, group, zeros, dt):
+    """Whole x, scales that are powers of two and whole zero points: every sum is a multiple of a half below
+    2^23, so the result is exact in whatever order it is formed, and equal to the definition's. One row has larger values
+    in its second half and one zeros in its first, so that the scaling of rows whose x passes in blocks of columns
+    changes on the way."""
+    g = _gen(K + M)
+    x = torch.randint(-1, 2, (M, K), generator=g, device="cuda").double()
+    some = torch.rand(M, K, generator=g, device="cuda") < 1 / 128
+    half = torch.arange(K, device="cuda") >= K // 2
+    if M > 1:
+        x[M // 2] = torch.where(half & some[0], x[M // 2] * 32, torch.where(some[1], x[M // 2], 0.0))
+    x[M - 1] *= half
+    _, codes, _, _ = _nibble_inputs(1, N, K, group, DT[dt], False, K)
+    groups = -(-K // group)
+    scales = torch.exp2(torch.randint(-1, 2, (N, groups), generator=g, device="cuda").double()).to(DT[dt])
+    z = torch.randint(0, 16, (N, groups), generator=g, device="cuda").to(DT[dt]) if zeros else None
+    if K > 100000:  # keep to 2^23
+        x *= torch.rand(M, K, generator=g, device="cuda") < 100000 / K / 3
+    w = _nibble_weights(codes, scales, z, K, group)
+    # q and z stand apart in a group's sum; each is at most 15
+    at = torch.arange(K, device="cuda") // group
+    assert (x.abs() @ scales.double()[:, at].t()).max() * 30 * 2 < 2 ** 24
+    out = torch.empty(M, N, device="cuda")
+    _nibble(ops, x.to(DT[dt]), codes, scales, z, out, K, group)
+    want = x @ w.t()
+    assert torch.equal(out.double(), want), (out.double() - want).abs().max()
+    assert (want != 0).double().mean() > 0.9
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("M,N,K,group", WIDE)
+def test_nibble_gemm_wide_rows(ops, M, N, K, group, dt):
+    """Any values, with a bound that stays far below the result however wide the rows are. A group's sum takes `group`
+    products and its first value, each off by at most 2^-23 of the magnitudes in the group (truncating adders),
+    and x loses at most 2^-35 of its row's largest; the groups' results, and the pieces of a tile, then add up with one rounding
+    each, of 2^-24 of a sum of neighbouring groups, which is at most twice the largest of the running sums."""
+    x, codes, scales, z = _nibble_inputs(M, N, K, group, DT[dt], True, 17)
+    q = torch.stack((codes & 15, codes >> 4), -1).flatten(1)[:, :K].double()
+    groups = -(-K // group)
+    pad = groups * group - K
+    xs, qs = [torch.nn.functional.pad(t, (0, pad)).view(-1, groups, group) for t in (x.double(), q)]
+    s, zz = scales.double(), z.double()
+    part = s * (torch.einsum("mgk,ngk->mng", xs, qs) - zz * xs.sum(2)[:, None])
+    mag = s * (torch.einsum("mgk,ngk->mng", xs.abs(), qs) + zz * xs.abs().sum(2)[:, None])
+    ref = part.sum(2)
+    run = torch.nn.functional.pad(part.cumsum(2), (1, 0))
+    spread = run.amax(2) - run.amin(2)
+    bound = (group + 16) * 2.0 ** -23 * mag.sum(2) + 2 * (groups + 40) * 2.0 ** -24 * spread + _u(torch.float32) * ref.abs()
+    out = torch.empty(M, N, device="cuda")
+    _nibble(ops, x, codes, scales, z, out, K, group)
+    err = (out.double() - ref).abs()
+    assert (err <= bound).all(), (err / bound).max()
+    assert bound.mean() < 0.05 * ref.abs().mean()  # so that a wrong result fails
+
+
+@pytest.mark.parametrize("M,N,K,group", [(7, 515, 3001, 64), (16, 100, 2624, 128), (40, 64, 9000, 32), (8, 40, 100000, 64)])
+def test_nibble_gemm_rows_do_not_depend_on_each_other(ops, M, N, K, group):
+    """A row's bits are the same whatever the other rows of the call hold."""
+    x, codes, scales, z = _nibble_inputs(M, N, K, group, torch.bfloat16, True, 19)
+    outs = []
+    for by in (1.0, 1e4, math.nan):
+        y = x.clone()
+        y[::3] *= by
+        out = torch.empty(M, N, device="cuda")
+        _nibble(ops, y, codes, scales, z, out, K, group)
+        outs.append(out)
+    keep = torch.arange(M, device="cuda") % 3 != 0
+    assert torch.equal(outs[0][keep], outs[1][keep]) and torch.equal(outs[0][keep], outs[2][keep])
+    assert not torch.equal(outs[0], outs[1]) and torch.isnan(outs[2][~keep]).all()
+
+
 # ---------------------------------------------------------------------------------------------
 # the cache
 
@@ -601,6 +680,36 @@ def test_cache_attention_queries_that_are_not_finite_and_see_no_key(ops, H, G, D
         assert (out[rows, : heads * D] == 0).all() and (lse[rows] == -math.inf).all()
     seen = torch.cat([out[lens[0] - keys[0]: lens[0]], out[lens[0] + lens[1]: sum(lens)]])[:, : heads * D]
     assert torch.isfinite(seen).all() and seen.any()
+
+
+@pytest.mark.parametrize("H,G,D,page,n,L", [(8, 2, 128, 64, 2, 70001), (1, 1, 64, 16, 1, 131072), (4, 16, 128, 32, 40, 20000)])
+def test_cache_attention_long_caches_add_up(ops, H, G, D, page, n, L):
+    """Long caches with a bound that stays far below the result. A warp's sums over its share of a chunk (at most 4096
+    keys) take one step a key, each off by at most 2^-23 of what is summed; the four warps and then the chunks add
+    one each. Scores and weights as in _check_attention."""
+    c = Paged(ops, 1, L, H, D, page, 83)
+    heads = H * G
+    q = torch.randn(n, heads * D, generator=_gen(84), device="cuda").half() * 1.5
+    scale = 1 / math.sqrt(D)
+    out, lse = _attention(ops, c, q, heads, [n], [L], scale)
+    steps = 4096 + 4 + -(-L // 128)
+    K, V = [c.rows(which, 0, L)[0].cuda() for which in (0, 1)]
+    x = q.double().view(n, heads, D)
+    pos = torch.arange(L - n, L, device="cuda")[:, None]
+    hidden = torch.arange(L, device="cuda")[None] > pos
+    vs = c.scales[1].max().item()
+    larger = []
+    for h in range(heads):
+        s = (x[:, h] @ K[:, h // G].t() * scale).masked_fill(hidden, -math.inf)
+        d = (D + 8) * 2.0 ** -22 * scale * (x[:, h].abs() @ K[:, h // G].abs().t()).amax(1)
+        p = torch.softmax(s, 1)
+        want, mass = p @ V[:, h // G], p @ V[:, h // G].abs()
+        bound = _u(q.dtype) * want.abs() + mass * (2.0 ** -11 + 2 * d[:, None] + 2 * steps * 2.0 ** -23) + L * 2.0 ** -39 * 128 * vs * p.amax(1)[:, None]
+        err = (out[:n, h * D: (h + 1) * D].double() - want).abs()
+        assert (err <= bound).all(), (h, (err / bound).max().item())
+        assert ((lse[:n, h].double() - torch.logsumexp(s, 1)).abs() <= d + steps * 2.0 ** -23 + 2.0 ** -22 * (1 + torch.logsumexp(s, 1).abs())).all()
+        larger.append((bound < 0.5 * want.abs()).double().mean().item())
+    assert np.mean(larger) > 0.75, np.mean(larger)  # so that a wrong result fails
 
 
 def test_cache_attention_one_workspace_for_smaller_calls(ops):
