@@ -17,8 +17,8 @@
 //  - a page's value scale differs from its neighbours' inside one sum, so it goes into the weight: with t = log2(scale /
 //    largest scale of the block), the weight is exp2(s + t - m + 14), m a running maximum of s + t, and the sum of
 //    the softmax adds weight * 2^-t. m follows the true maximum only when that is 1.75 ahead, so outputs are
-//    seldom rescaled. Weights are held as f16: at most 2^15.75, with all 11 bits down to 2^-28 of the
-//    largest; scores, maxima, sums and outputs are fp32.
+//    seldom rescaled. Weights are held as f16 (two of them for f16 results): at most 2^15.75, with all 11 bits
+//    down to 2^-28 of the largest; scores, maxima, sums and outputs are fp32.
 //
 // Few query rows (bound by the cache's bytes): each warp has its own tiles of the block's keys and its own
 // ring of loads, so nothing waits inside the loop; the four warps' results are joined at the end. Long
@@ -271,13 +271,32 @@ struct AttnRows {
   }
 };
 
+// Weights are rounded to 11 bits for a bf16 result, whose own rounding to 8 bits is eight times as large. A result in
+// f16 would be a quarter further from its exact value (2.6e-4 instead of 2.1e-4 for one row over 131072 keys), so
+// there a second product takes what the rounding has left of each weight: 22 bits together. That costs 12 to 17 %
+// (37.1 -> 41.7 us for that row; bf16 would take 191 instead of 170 us for 64 rows over 4096 to 8192 keys, 134
+// instead of 115 us for 4 x 512 rows, for the same distance of 1.7e-3 from the exact values).
+template <typename T>
+constexpr bool ATTN_SPLIT = false;
+template <>
+constexpr bool ATTN_SPLIT<__half> = true;
+// Two weights as f16, and what that leaves of them.
+S1C_DEV uint32_t attn_split(float x, float y, uint32_t& rest) {
+  const uint32_t v = pack_f16x2(x, y);
+  const float2 f = unpack_f16x2(v);
+  rest = pack_f16x2(x - f.x, y - f.y);
+  return v;
+}
 // The weights of a tile as operands of two products over 16 keys each.
-S1C_DEV void attn_pack(const float (&s)[4][4], uint32_t (&pa)[2][4]) {
+template <bool SPLIT>
+S1C_DEV void attn_pack(const float (&s)[4][4], uint32_t (&pa)[2][4], uint32_t (&pr)[2][4]) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    pa[k][0] = pack_f16x2(s[2 * k][0], s[2 * k][1]), pa[k][1] = pack_f16x2(s[2 * k][2], s[2 * k][3]);
-    pa[k][2] = pack_f16x2(s[2 * k + 1][0], s[2 * k + 1][1]), pa[k][3] = pack_f16x2(s[2 * k + 1][2], s[2 * k + 1][3]);
-  }
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = s[2 * k + i / 2][i % 2 * 2], y = s[2 * k + i / 2][i % 2 * 2 + 1];
+      pa[k][i] = SPLIT ? attn_split(x, y, pr[k][i]) : pack_f16x2(x, y);
+    }
 }
 
 // N neighbouring dimensions, from d on, of one row's result: v * v_top / sum, with log2 of the sum beside
@@ -404,8 +423,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       });
     });
     row.weights(c, u, sm.page, u.lo + i * CATT_TK, kc0, kc1, s, o);
-    uint32_t pa[2][4];
-    attn_pack(s, pa);
+    uint32_t pa[2][4], pr[2][4];
+    attn_pack<ATTN_SPLIT<T>>(s, pa, pr);
 #pragma unroll
     for (int q = 0; q < SEG; ++q) {
       const uint32_t at0 = base + v_at[0][q], at1 = base + v_at[1][q];
@@ -420,7 +439,10 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
           b[2][e] = code_pair(__byte_perm(even, 0x64646464u, 0x4341)), b[3][e] = code_pair(__byte_perm(odd, 0x64646464u, 0x4341));
         });
 #pragma unroll
-        for (int d = 0; d < 4; ++d) mma_f16(o[q * 4 + d], pa[k], b[d][0], b[d][1]);
+        for (int d = 0; d < 4; ++d) {
+          mma_f16(o[q * 4 + d], pa[k], b[d][0], b[d][1]);
+          if (ATTN_SPLIT<T>) mma_f16(o[q * 4 + d], pr[k], b[d][0], b[d][1]);
+        }
       });
     }
     __syncwarp();
@@ -469,8 +491,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 
 // Many query rows: warps 0 to 3 softmax (thread = row = TMEM lane), 4 to 7 conversion, 8 products.
 constexpr int CATP_ROWS = 128, CATP_WARPS = 9, CATP_PAGES = 256;
-// TMEM columns: scores (then weights, f16 pairs, over the first 32 columns) of even tiles [0, 64), of odd
-// tiles [64, 128); outputs from 128 on
+// TMEM columns: scores (then weights, f16 pairs, over the first 32 columns, and what is left of them, over the
+// others) of even tiles [0, 64), of odd tiles [64, 128); outputs from 128 on
 constexpr uint32_t CATP_TMEM = 256, CATP_TMEM_O = 128;
 
 template <int D>
@@ -555,8 +577,8 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll
         for (int n = 0; n < D / 64; ++n)
 #pragma unroll
-          for (int k = 0; k < CATP_TK / 16; ++k)
-            umma_bf16_ts(tmem + CATP_TMEM_O + 64 * n, tmem + 64 * b + 8 * k, sdesc_mnmajor_sw128(smem_u32(sm.v[b][n]) + k * 2048), idO,
+          for (int k = 0; k < CATP_TK / (ATTN_SPLIT<T> ? 8 : 16); ++k)  // the weights, then what is left of them
+            umma_bf16_ts(tmem + CATP_TMEM_O + 64 * n, tmem + 64 * b + 8 * k, sdesc_mnmajor_sw128(smem_u32(sm.v[b][n]) + k % 4 * 2048), idO,
                          (i | k) ? 1u : 0u);
         umma_commit(&sm.pv_done[b]);
         if (i == u.tiles - 1) umma_commit(&sm.o_full);
@@ -702,7 +724,7 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         }
       }
       const float off = m == -INFINITY ? 0.f : 14.f - m;
-      float pk[32];
+      float pk[32], pr[ATTN_SPLIT<T> ? 32 : 1];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float sum = 0.f;
@@ -710,11 +732,18 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         for (int x = 8 * j; x < 8 * j + 8; ++x) {
           const float p0 = exp2_approx(s[2 * x] + off), p1 = exp2_approx(s[2 * x + 1] + off);
           sum += p0 + p1;
-          pk[x] = __uint_as_float(pack_f16x2(p0, p1));
+          if constexpr (ATTN_SPLIT<T>) {
+            uint32_t rest;
+            pk[x] = __uint_as_float(attn_split(p0, p1, rest));
+            pr[x] = __uint_as_float(rest);
+          } else {
+            pk[x] = __uint_as_float(pack_f16x2(p0, p1));
+          }
         }
         l = fmaf(sum, inv[j], l);
       }
       tmem_st32(tmem + lanes + 64 * b, pk);
+      if constexpr (ATTN_SPLIT<T>) tmem_st32(tmem + lanes + 64 * b + 32, pr);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
