@@ -318,7 +318,7 @@ S1C_API s1c_status s1c_cache_read(const s1c_cache* cache, int32_t dtype, void* d
                                   const int32_t* d_pages, int32_t max_pages, int32_t n, int32_t max_rows, void* stream);
 
 /* Bytes of device workspace that serve every s1c_cache_attention with bounds up to these (n, max_q and max_kv;
- * it may be 0). A call that does not split its keys takes none. With n * max_q * heads rows and heads it is at most
+ * it is 0 for a cache or bounds that the call refuses). A call that does not split its keys takes none. With n * max_q * heads rows and heads it is at most
  * 4 (head_dim + 1) bytes for each of them and each chunk of the keys: 2048 keys, or for more than 32 rows a key
  * head 256 pages less 128 keys; where few blocks share long keys, 39 MB at most instead. Long pieces of
  * prompts over very long caches need gigabytes (8192 rows, 32 heads of 128, 131072 positions in pages of 16:

@@ -321,10 +321,11 @@ s1c_status s1c_cache_read(const s1c_cache* cache, int32_t dtype, void* d_k, int6
 size_t s1c_cache_attention_workspace(const s1c_cache* cache, int32_t heads, int32_t n, int32_t max_q, int32_t max_kv) {
   try {
     const CacheView c = check_cache(cache);
-    if (heads <= 0 || heads % c.heads || n <= 0 || max_q <= 0 || max_kv <= 0) return 0;
+    if (heads <= 0 || heads % c.heads || n <= 0 || max_q <= 0 || max_kv <= 0 || max_kv > (1 << 30) || (int64_t)n * max_q > INT_MAX / heads)
+      return 0;
     return attention_workspace(c, heads, n, max_q, max_kv);
   } catch (...) {
-    return 0;  // a cache that the call refuses
+    return 0;
   }
 }
 

@@ -112,6 +112,13 @@ def test_cache_attention_refuses_a_short_workspace():
     assert bk.lib().s1c_cache_attention_workspace(None, 4, 1, 1, 100000) == 0
 
 
+def test_cache_attention_workspace_of_refused_bounds_is_zero():
+    big = 2 ** 31 - 1
+    for bounds in [(4, big, big, 4096), (4, 1, 1, big), (2 ** 30, 4, 1, 4096), (4, 1, big, 4096), (4, 0, 1, 4096), (3, 1, 1, 4096)]:
+        assert ops.cache_attention_workspace(_cache(), *bounds) == 0, bounds
+    assert ops.cache_attention_workspace(_cache(), 4, 2 ** 15, 2 ** 13, 2 ** 30) > 2 ** 50  # the largest: no overflow
+
+
 @pytest.mark.parametrize("heads,kv_heads,page,dim", [(8, 8, 16, 64), (32, 8, 16, 128), (4, 4, 64, 128), (80, 2, 32, 64),
                                                      (16, 1, 16, 128)])
 def test_cache_attention_workspace_serves_smaller_calls(heads, kv_heads, page, dim):
