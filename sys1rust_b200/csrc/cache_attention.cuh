@@ -804,7 +804,7 @@ __global__ void __launch_bounds__(WARPS * 32) cache_attention_join_kernel(const 
       for (int e = 0; e < E; ++e) v[e] = p[e];
       sum += by;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] += by * v[e];  // a chunk without a key has written zeros
+      for (int e = 0; e < E; ++e) o[e] += by == 0.f ? 0.f : by * v[e];  // 0 also times an output past fp32
     }
   }
   if (lane == 0) sums[w] = sum;
