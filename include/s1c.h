@@ -335,7 +335,7 @@ S1C_API size_t s1c_cache_attention_workspace(const s1c_cache* cache, int32_t hea
  * -inf; one that sees a key and holds an infinity or NaN gets NaN. No sequence may have more than max_q
  * query rows or max_kv positions: what is past them is not computed. Scores, softmax statistics and sums are
  * held in fp32; a key's weight times its value scale is rounded to 11 bits (F16: 22 bits), or to 2^-38 of the row's
- * largest where that is more. Value scales below 2^-90 of the largest in the call count as that. The workspace
+ * largest where that is more. The workspace
  * (16-byte aligned) is free for other use when the call's work has run; calls that overlap on the GPU need one
  * each. Waits inside the kernels are bounded (2 s each); rows for which one runs out get NaN in out and lse. */
 S1C_API s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, const void* d_q, int64_t q_stride,

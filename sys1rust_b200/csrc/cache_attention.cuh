@@ -76,6 +76,7 @@ constexpr int ATTN_BEYOND = 4;  // entries of the list of pages behind the last 
 // What a block works on: `rows` rows from row0 on of one sequence and key head, keys [lo, hi) in `tiles` tiles.
 struct AttnUnit {
   int h, seq, first, count, L, rows, row0, chunk, lo, hi, tiles, window, shift, G;
+  bool wide = false;  // value scales more than 2^90 apart
 };
 template <int ROWS, int TK>
 S1C_DEV bool attn_unit(const CacheView& c, const CacheAttnArgs& a, AttnUnit& u) {
@@ -98,36 +99,56 @@ S1C_DEV bool attn_unit(const CacheView& c, const CacheAttnArgs& a, AttnUnit& u) 
 
 // The chunk's pages: (key scale * 2^24, t, 2^-t, page), a few more than there are, without a page (-1) 0,
 // -inf, 0. Returns the largest value scale, which the outputs are multiplied by. All threads call.
+//
+// 2^-t times a weight stays in range down to t = -90: the sum is then below 2^(15.75 + 90 + 14) for the 2^14 keys
+// of a chunk. Where scales lie further apart (padding of any bits may have got into a page), u.wide is set, and
+// the sum is formed from weights of its own, without t (attn_wide). Zero scales, whose codes are zero, count as the
+// smallest t.
 template <int WARPS>
-S1C_DEV float attn_pages(const CacheView& c, const CacheAttnArgs& a, const AttnUnit& u, float4* list, float* tops) {
+S1C_DEV float attn_pages(const CacheView& c, const CacheAttnArgs& a, AttnUnit& u, float4* list, float2* ends) {
   const int tid = threadIdx.x, p0 = u.lo >> u.shift, pages = ((u.hi - 1) >> u.shift) - p0 + 1;  // and more behind them than a tile has
-  float top = 0.f;
+  float top = 0.f, low = INFINITY;  // the largest scale, the smallest but 0
   for (int i = tid; i < pages + ATTN_BEYOND; i += WARPS * 32) {
     const int page = i < pages ? cache_page(a.table, a.max_pages, u.seq, p0 + i, c.num_pages) : -1;
     float ks = 0.f, vs = 0.f;
     if (page >= 0) {
       const int64_t slot = (int64_t)page * c.heads + u.h;
-      ks = c.scales[0][slot], vs = c.scales[1][slot];
+      ks = c.scales[0][slot], vs = c.scales[1][slot] + 0.f;  // no -0
     }
     list[i] = make_float4(ks * 0x1p24f, vs, 0.f, __int_as_float(page));
-    top = fmaxf(top, vs);
+    top = fmaxf(top, vs), low = vs > 0.f ? fminf(low, vs) : low;
   }
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (tid % 32 == 0) tops[tid / 32] = top;
+  top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));  // not negative: ordered as integers are
+  low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(low)));
+  if (tid % 32 == 0) ends[tid / 32] = make_float2(top, low);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < WARPS; ++i) top = fmaxf(top, tops[i]);
+  for (int i = 0; i < WARPS; ++i) top = fmaxf(top, ends[i].x), low = fminf(low, ends[i].y);
+  u.wide = low < top * 0x1p-90f;
   for (int i = tid; i < pages + ATTN_BEYOND; i += WARPS * 32) {
     float4 e = list[i];
-    // scales below 2^-90 of the largest (and zero ones, whose codes are zero) count as that: the sum then stays
-    // below 2^(15.75 + 90 + 14) for the 2^14 keys of a chunk
-    const float l2 = top > 0.f ? fmaxf(log2f(e.y / top), -90.f) : 0.f;
+    const float l2 = !(top > 0.f) ? 0.f : u.wide ? fmaxf(log2f(e.y) - log2f(top), -300.f) : fmaxf(log2f(e.y / top), -90.f);
     const bool in = __float_as_int(e.w) >= 0;
-    e.y = in ? l2 : -INFINITY, e.z = in ? exp2f(-l2) : 0.f;
+    e.y = in ? l2 : -INFINITY, e.z = in && !u.wide ? exp2f(-l2) : 0.f;
     list[i] = e;
   }
   __syncthreads();
   return top;
+}
+
+// A running maximum and sum of exp2(score) in shared memory, one for each row of a thread: (maximum, sum).
+template <int N>
+S1C_DEV void attn_wide_add(float2& w, float top, const float (&scores)[N]) {
+  const float n = fmaxf(w.x, top), from = n == -INFINITY ? 0.f : n;
+  w.y *= exp2f(w.x - from);
+  w.x = n;
+#pragma unroll
+  for (int i = 0; i < N; ++i) w.y += exp2_approx(scores[i] - from);
+}
+// What outputs o are multiplied by, by and with log2 of the sum, where scales lie far apart: o is in units of
+// v_top * 2^(m - 14).
+S1C_DEV float attn_wide_out(float o, float v_top, float m, float2 w) {
+  return w.y == 0.f ? 0.f : (float)((double)o * v_top * exp2((double)m - 14.0 - w.x) / w.y);
 }
 
 // TMA of one tile's keys and values to `dst`, by a whole warp: a lane for each page or 32 rows of one.
@@ -207,7 +228,8 @@ struct AttnRows {
   // sums take them, and the outputs o are rescaled when the maximum has grown. kc0, kc1: where a lane's two
   // columns stand among eight keys.
   template <int N>
-  S1C_DEV void weights(const CacheView& c, const AttnUnit& u, const float4* list, int key, int kc0, int kc1, float (&s)[4][4], float (&o)[N][4]) {
+  S1C_DEV void weights(const CacheView& c, const AttnUnit& u, const float4* list, int key, int kc0, int kc1, float2* wide, float (&s)[4][4],
+                       float (&o)[N][4]) {
     const bool open = key + CATT_TK - 1 <= pos[0] && key >= pos[1] - u.window && key + CATT_TK <= u.hi;
     float top[2] = {-INFINITY, -INFINITY}, inv[4];
     const int pg = (key >> u.shift) - (u.lo >> u.shift);
@@ -229,6 +251,21 @@ struct AttnRows {
           if (j * 8 + kc0 > last || j * 8 + kc0 < from) s[j][2 * e] = -INFINITY;
           if (j * 8 + kc1 > last || j * 8 + kc1 < from) s[j][2 * e + 1] = -INFINITY;
         }
+      }
+    }
+    if (u.wide) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float r[8], big = -INFINITY;  // scores without t
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float t = list[pg + (((key & (c.page - 1)) + j / 2 * 8) >> u.shift)].y;
+          r[j] = t == -INFINITY ? t : s[j / 2][2 * e + j % 2] - t;
+          big = fmaxf(big, r[j]);
+        }
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        attn_wide_add(wide[e], big, r);
       }
     }
 #pragma unroll
@@ -261,9 +298,14 @@ struct AttnRows {
         l[e / 2] = fmaf(s[j][e], inv[j], l[e / 2]);
       }
   }
-  S1C_DEV void finish() {
+  S1C_DEV void finish(const AttnUnit& u, float2* wide) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
+      if (u.wide) {
+        wide[e].y += __shfl_xor_sync(0xffffffffu, wide[e].y, 1);
+        wide[e].y += __shfl_xor_sync(0xffffffffu, wide[e].y, 2);
+        wide[e].y = attn_sum(wide[e].y, m[e], factor[e]);
+      }
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
       l[e] = attn_sum(l[e], m[e], factor[e]);
@@ -299,11 +341,12 @@ S1C_DEV void attn_pack(const float (&s)[4][4], uint32_t (&pa)[2][4], uint32_t (&
     }
 }
 
-// N neighbouring dimensions, from d on, of one row's result: v * v_top / sum, with log2 of the sum beside
-// dimension 0. Without a key the sum is 0: outputs 0 and -inf.
+// N neighbouring dimensions, from d on, of one row's result: v * by, by = v_top / sum, with log2 of the sum,
+// top - 14 + log2(sum), beside dimension 0. Without a key the sum is 0: outputs 0 and -inf.
+S1C_DEV float attn_by(float v_top, float sum) { return sum == 0.f ? 0.f : v_top / sum; }
+S1C_DEV float attn_log(float top, float sum) { return sum == 0.f ? -INFINITY : top - 14.f + log2f(sum); }
 template <typename T, int D, int N>
-S1C_DEV void attn_put(const CacheAttnArgs& a, const AttnUnit& u, int64_t row, int head, int d, const float (&v)[N], float v_top, float sum, float top) {
-  const float by = sum == 0.f ? 0.f : v_top / sum, log_sum = sum == 0.f ? -INFINITY : top - 14.f + log2f(sum);
+S1C_DEV void attn_put(const CacheAttnArgs& a, const AttnUnit& u, int64_t row, int head, int d, const float (&v)[N], float by, float log_sum) {
   if (a.chunks > 1) {
     const int64_t at = ((u.seq * (int64_t)a.max_q + (row - u.first)) * a.heads + head) * a.chunks + u.chunk;
 #pragma unroll
@@ -329,8 +372,9 @@ struct CacheAttnSmem {
   uint4 q[D / 16][32];  // operands of the query rows
   uint64_t full[CATT_WARPS][STAGES];
   float4 page[CATT_PAGES + ATTN_BEYOND];
-  float top[CATT_WARPS];
+  float2 top[CATT_WARPS];
   float row_m[CATT_WARPS][16], row_l[CATT_WARPS][16];
+  float2 wide[CATT_WARPS * 32][2], row_wide[CATT_WARPS][16];
 };
 
 template <typename T, int D>
@@ -363,6 +407,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
 
   AttnRows row;
   row.setup(u, u.row0);
+  float2* wide = sm.wide[tid];
+  if (u.wide) wide[0] = wide[1] = make_float2(-INFINITY, 0.f);
   {
     uint32_t qa[QK][4];
     row.operands<T, D>(a, qa);
@@ -422,7 +468,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
         mma_f16(s[j], qa, __byte_perm(v, 0, 0x4140), __byte_perm(v, 0, 0x4342));
       });
     });
-    row.weights(c, u, sm.page, u.lo + i * CATT_TK, kc0, kc1, s, o);
+    row.weights(c, u, sm.page, u.lo + i * CATT_TK, kc0, kc1, wide, s, o);
     uint32_t pa[2][4], pr[2][4];
     attn_pack<ATTN_SPLIT<T>>(s, pa, pr);
 #pragma unroll
@@ -448,13 +494,13 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
     __syncwarp();
     if (i + S::STAGES * CATT_WARPS < u.tiles) issue(i + S::STAGES * CATT_WARPS);
   }
-  row.finish();
+  row.finish(u, wide);
 
   if (__syncthreads_or(late)) {  // also: the rings are free
     const float none[4] = {};
     for (int i = tid; i < 16 * D / 4 && u.row0 + i / (D / 4) < u.rows; i += CATT_WARPS * 32) {
       const int r = u.row0 + i / (D / 4);
-      attn_put<T, D>(a, u, u.first + r / u.G, u.h * u.G + r % u.G, i % (D / 4) * 4, none, 0.f, NAN, 0.f);
+      attn_put<T, D>(a, u, u.first + r / u.G, u.h * u.G + r % u.G, i % (D / 4) * 4, none, NAN, NAN);
     }
     return;
   }
@@ -464,6 +510,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
   for (int e = 0; e < 2; ++e) {
     const int r = g + 8 * e;
     if (cq == 0) sm.row_m[w][r] = row.m[e], sm.row_l[w][r] = row.l[e];
+    if (cq == 0 && u.wide) sm.row_wide[w][r] = wide[e];
 #pragma unroll
     for (int q = 0; q < SEG; ++q) {
       float4* at = reinterpret_cast<float4*>(all + (w * 16 + r) * D + q * 32 + cq * 8);
@@ -485,7 +532,19 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_c
       sum += sm.row_l[x][r] * by;
       v[0] += p.x * by, v[1] += p.y * by, v[2] += p.z * by, v[3] += p.w * by;
     }
-    attn_put<T, D>(a, u, u.first + (u.row0 + r) / u.G, u.h * u.G + (u.row0 + r) % u.G, d, v, v_top, sum, big);
+    float by = attn_by(v_top, sum), log_sum = attn_log(big, sum);
+    if (u.wide) {
+      float2 all2 = make_float2(-INFINITY, 0.f);
+      for (int x = 0; x < CATT_WARPS; ++x) {
+        const float2 p = sm.row_wide[x][r];
+        const float none[1] = {-INFINITY};
+        attn_wide_add(all2, p.x, none);
+        if (p.x != -INFINITY) all2.y += p.y * exp2f(p.x - all2.x);
+      }
+      for (int x = 0; x < 4; ++x) v[x] = attn_wide_out(v[x], v_top, big, all2);
+      by = 1.f, log_sum = attn_log(all2.x + 14.f, all2.y);
+    }
+    attn_put<T, D>(a, u, u.first + (u.row0 + r) / u.G, u.h * u.G + (u.row0 + r) % u.G, d, v, by, log_sum);
   }
 }
 
@@ -504,10 +563,11 @@ struct CachePromptSmem {
   alignas(1024) uint8_t v[2][D / 64][CATP_TK * 128];
   alignas(1024) uint8_t codes[2 * CATP_TK * D];  // one tile's keys and values as they are in the cache
   float4 page[CATP_PAGES + ATTN_BEYOND];
-  float top[CATP_WARPS];
+  float2 top[CATP_WARPS];
   uint64_t raw_full, raw_free, q_full, k_full, k_free, v_full[2], s_full[2], p_full[2], pv_done[2], o_full, drain;
   uint32_t tmem;
   int abort;
+  float2 wide[CATP_ROWS];
 };
 
 template <typename T, int D>
@@ -529,7 +589,7 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   if (u.tiles == 0) {
     const float zero[8] = {};
     if (real)
-      for (int d = 0; d < D; d += 8) attn_put<T, D>(a, u, at_row, head, d, zero, 0.f, 0.f, 0.f);
+      for (int d = 0; d < D; d += 8) attn_put<T, D>(a, u, at_row, head, d, zero, 0.f, -INFINITY);
     return;
   }
   if (tid == 0) {
@@ -667,6 +727,7 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     }
     const uint32_t lanes = (uint32_t)(w * 32) << 16;
     float m = -INFINITY, l = 0.f;
+    if (u.wide) sm.wide[tid] = make_float2(-INFINITY, 0.f);
     bool ok = true;
     for (int i = 0; i < u.tiles; ++i) {
       const int b = i & 1, key = u.lo + i * CATP_TK, pg = (key >> u.shift) - (u.lo >> u.shift), in = key & (c.page - 1);
@@ -677,6 +738,20 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         break;
       }
       tc_fence_after();
+      if (u.wide) {  // a first look at the scores
+        float2 all = sm.wide[tid];
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+          const float4 p = sm.page[pg + ((in + 16 * j) >> u.shift)];
+          float r[16], big = -INFINITY;
+          tmem_ld16(tmem + lanes + 64 * b + 16 * j, r);
+          if (p.y == -INFINITY) continue;
+#pragma unroll
+          for (int x = 0; x < 16; ++x) r[x] = 16 * j + x >= from && 16 * j + x < upto ? r[x] * (factor * p.x) : -INFINITY, big = fmaxf(big, r[x]);
+          attn_wide_add(all, big, r);
+        }
+        sm.wide[tid] = all;
+      }
       float s[64];
       tmem_ld32x2(tmem + lanes + 64 * b, true, true, s);
       const bool open = __all_sync(0xffffffffu, from <= 0 && upto >= CATP_TK);
@@ -755,12 +830,20 @@ cache_prompt_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       for (int d = 0; d < D; d += 32) {
         float t[32];
         tmem_ld32(tmem + lanes + CATP_TMEM_O + d, t);
-        if (real) attn_put<T, D>(a, u, at_row, head, d, t, v_top, attn_sum(l, m, factor), m);
+        const float sum = attn_sum(l, m, factor);
+        float by = attn_by(v_top, sum), log_sum = attn_log(m, sum);
+        if (u.wide) {
+          const float2 all = make_float2(sm.wide[tid].x, attn_sum(sm.wide[tid].y, m, factor));
+#pragma unroll
+          for (int x = 0; x < 32; ++x) t[x] = attn_wide_out(t[x], v_top, m, all);
+          by = 1.f, log_sum = attn_log(all.x + 14.f, all.y);
+        }
+        if (real) attn_put<T, D>(a, u, at_row, head, d, t, by, log_sum);
       }
     } else if (real) {  // a wait has run out
       const float none[8] = {};
 #pragma unroll 1
-      for (int d = 0; d < D; d += 8) attn_put<T, D>(a, u, at_row, head, d, none, 0.f, NAN, 0.f);
+      for (int d = 0; d < D; d += 8) attn_put<T, D>(a, u, at_row, head, d, none, NAN, NAN);
     }
   }
   __syncwarp();

@@ -732,6 +732,45 @@ def test_cache_attention_results_are_as_near_as_their_type_allows(ops, H, G, D, 
     assert rms(out[:n, : heads * D].double() - want) <= 1.05 * least
 
 
+FAR = [(64, 2, 4, [1, 2, 1], [100, 90, 300]), (128, 1, 4, [2], [3000]), (64, 1, 8, [30, 5, 50], [120, 90, 50]), (128, 2, 3, [40], [2500])]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("D,H,G,lens,keys", FAR)
+def test_cache_attention_far_larger_values_without_weight(ops, D, H, G, lens, keys, dt):
+    """Pages with values up to the end of fp32 (what padding of any bits may leave), at keys whose weights are far below
+    its smallest number or that a row does not see, change nothing; rows in one block with them and rows whose keys
+    are split."""
+    n, heads = len(lens), H * G
+    c = Paged(ops, n, max(keys), H, D, 16, 87)
+    last = [int(c.table[i, (L - 1) // 16]) for i, L in enumerate(keys)]  # hidden from the rows before it
+    for p in c.table[:, 2::5].flatten().tolist() + last:
+        c.codes[0][p], c.codes[1][p] = -127, 127
+        c.scales[0][p], c.scales[1][p] = 1.0, 3e38
+    q = (torch.rand(sum(lens), heads * D, generator=_gen(88), device="cuda") + 0.5).to(DT[dt])
+    out, lse = _attention(ops, c, q, heads, lens, keys, 0.3)
+    _check_attention(c, q, heads, lens, keys, 0.3, -1, out, lse)
+    assert out[: sum(lens), : heads * D].abs().max() < 10
+
+
+@pytest.mark.parametrize("D,H,G,lens,keys", FAR)
+def test_cache_attention_value_scales_over_the_whole_range(ops, D, H, G, lens, keys):
+    """Value scales from 2^-120 to 2^100, with zero scales (and zero codes) among them; half of the sequences' pages
+    lie within a narrower range, so that some blocks take the common way."""
+    n, heads = len(lens), H * G
+    c = Paged(ops, n, max(keys), H, D, 16, 89)
+    g = _gen(90)
+    c.scales[1] = torch.exp2(torch.rand(c.count, H, generator=g, device="cuda") * 220 - 120)
+    c.scales[1][::7], c.codes[1][::7] = 0, 0
+    if n > 1:
+        c.scales[1][c.table[1].long()] = torch.exp2(torch.rand(c.table.shape[1], H, generator=g, device="cuda") * 80)
+    c.handle = ops.Cache(c.codes[0].data_ptr(), c.codes[1].data_ptr(), c.scales[0].data_ptr(), c.scales[1].data_ptr(), c.count, 16, H, D)
+    q = torch.randn(sum(lens), heads * D, generator=g, device="cuda").bfloat16()
+    q[::2] *= 8  # weights far apart too
+    out, lse = _attention(ops, c, q, heads, lens, keys, 0.1)
+    _check_attention(c, q, heads, lens, keys, 0.1, -1, out, lse)
+
+
 def test_cache_attention_one_workspace_for_smaller_calls(ops):
     """One buffer of the largest batch's size, with known bytes behind it, through calls that shrink in every
     direction and split their keys more than the largest does."""
