@@ -262,6 +262,24 @@ def test_nibble_gemm_rows_do_not_depend_on_each_other(ops, M, N, K, group):
     assert not torch.equal(outs[0], outs[1]) and torch.isnan(outs[2][~keep]).all()
 
 
+def test_nibble_gemm_codes_past_four_gigabytes(ops):
+    """A matrix of 4.6 GB of codes with rows of x and out past 2^31 elements: its first and last rows."""
+    M, N, K, group = 3, 1150000, 8000, 128
+    if torch.cuda.mem_get_info()[0] < 40 * 2 ** 30:
+        pytest.skip("needs 40 GB")
+    g = _gen(23)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.exp2(torch.randint(-1, 2, (N, 63), generator=g, device="cuda").float()).half()
+    stride = 2 ** 30 + 4
+    x = torch.empty(2 * stride + K, dtype=torch.float16, device="cuda").as_strided((M, K), (stride, 1))
+    x.copy_(torch.randint(-1, 2, (M, K), generator=g, device="cuda"))
+    out = torch.empty(2 * stride + N, dtype=torch.float32, device="cuda").as_strided((M, N), (stride, 1))
+    _nibble(ops, x, codes, scales, None, out, K, group)
+    for rows in (slice(0, 100), slice(N // 2, N // 2 + 100), slice(N - 100, N)):
+        want = x.double() @ _nibble_weights(codes[rows], scales[rows], None, K, group).t()
+        assert torch.equal(out[:, rows].double(), want)
+
+
 # ---------------------------------------------------------------------------------------------
 # the cache
 
@@ -771,6 +789,43 @@ def test_cache_attention_value_scales_over_the_whole_range(ops, D, H, G, lens, k
     _check_attention(c, q, heads, lens, keys, 0.1, -1, out, lse)
 
 
+@pytest.mark.parametrize("lens,keys", [([2, 0, 1, 0, 3], [300, 200, 90, 0, 64]), ([0, 40, 0, 5, 90], [7, 300, 2, 90, 90])])
+def test_cache_attention_sequences_without_queries_and_shared_pages(ops, lens, keys):
+    """Sequences with no query row between others, pages that several sequences name (a common beginning) and pages
+    that one table row names twice."""
+    c = Paged(ops, 5, 320, 2, 64, 16, 91)
+    c.table[1:, :3] = c.table[0, :3]
+    c.table[0, 4], c.table[2, 5] = c.table[0, 1], c.table[2, 3]
+    q = torch.randn(sum(lens), 6 * 64, generator=_gen(92), device="cuda").bfloat16()
+    out, lse = _attention(ops, c, q, 6, lens, keys, 0.125)
+    some = [i for i, n in enumerate(lens) if n]
+    c.table, c.n = c.table[some].contiguous(), len(some)
+    _check_attention(c, q, 6, [lens[i] for i in some], [keys[i] for i in some], 0.125, -1, out, lse)
+
+
+def test_cache_calls_with_rows_far_apart(ops):
+    """Row strides that take offsets past 2^31 elements, in every call on a cache."""
+    H, D, n, stride = 2, 64, 3, 2 ** 30 + 8
+    if torch.cuda.mem_get_info()[0] < 60 * 2 ** 30:
+        pytest.skip("needs 60 GB")
+    c = Paged(ops, 1, 40, H, D, 16, 93)
+    big = [torch.empty(2 * stride + 4 * H * D, dtype=torch.float16, device="cuda") for _ in range(4)]
+    k, v, q, out = [x.as_strided((n, H * D), (stride, 1)) for x in big]
+    for i, x in enumerate((k, v, q)):
+        x.copy_(torch.randn(n, H * D, generator=_gen(94 + i), device="cuda"))
+    c.write(k, v, [n], [20])
+    c.check()
+    lse, cu, ln = torch.empty(n, H, device="cuda"), _i32([0, n]), _i32([20 + n])
+    ops.cache_attention(c.handle, ops.DT_F16, q.data_ptr(), stride, out.data_ptr(), stride, H, cu.data_ptr(), ln.data_ptr(),
+                        c.table.data_ptr(), c.table.shape[1], 1, n, 20 + n, 0.125, lse_ptr=lse.data_ptr(), stream=_stream())
+    want, want_lse = _attention(ops, c, q.contiguous(), H, [n], [20 + n], 0.125)
+    assert torch.equal(out, want[:n, : H * D]) and torch.equal(lse, want_lse[:n])
+    ops.cache_read(c.handle, ops.DT_F16, k.data_ptr(), stride, v.data_ptr(), stride, cu.data_ptr(), _i32([20]).data_ptr(),
+                   c.table.data_ptr(), c.table.shape[1], 1, n, stream=_stream())
+    near = c.read([n], [20], torch.float16)
+    assert torch.equal(k, near[0][:n, : H * D]) and torch.equal(v, near[1][:n, : H * D])
+
+
 def test_cache_attention_one_workspace_for_smaller_calls(ops):
     """One buffer of the largest batch's size, with known bytes behind it, through calls that shrink in every
     direction and split their keys more than the largest does."""
@@ -1021,6 +1076,21 @@ def test_sample_rows_do_not_depend_on_their_batch(ops, dt, m, size):
     assert token.tolist() == [int(t[0]) for t, _ in alone]
     assert prob.tolist() == [float(q[0]) for _, q in alone]
     assert len(set(prob.tolist())) > R / 2
+
+
+def test_sample_rows_far_apart_and_the_largest_vocabulary(ops):
+    """Rows whose offsets pass 2^31 elements; 2^18 logits, many equal, whose masses and counts fill their sums."""
+    V, stride = 2 ** 18, 2 ** 31 + 2 ** 18
+    if torch.cuda.mem_get_info()[0] < 20 * 2 ** 30:
+        pytest.skip("needs 20 GB")
+    x = torch.empty(stride + V, dtype=torch.bfloat16, device="cuda").as_strided((2, V), (stride, 1))
+    g = _gen(94)
+    for size in (0.0, 0.01, 3.0):
+        x.copy_(torch.randn(2, V, generator=g, device="cuda") * size)
+        u = torch.rand(2, generator=g, device="cuda")
+        for k, p in [(None, None), (_i32([200000, 100]), None), (None, torch.tensor([0.9, 0.3], device="cuda")),
+                     (_i32([50000, 0]), torch.tensor([0.77, 1.0], device="cuda"))]:
+            _check_sample(ops, x, u, None, k, p, None)
 
 
 def test_sample_values_over_the_whole_range(ops):
