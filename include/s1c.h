@@ -276,8 +276,9 @@ S1C_API int64_t s1c_last_launch_count(const s1c_backend* b);
  * codes, whose padding is read and ignored. Each group of 32, 64 or 128 columns of a row has a scale s
  * and, where d_zeros is given, a zero point z (8 otherwise), in [N, ceil(K / group)] arrays of row
  * stride scale_stride. x, scales, zeros and out are F16 or BF16 (dtype); out_f32 = 1 makes out fp32.
- * bias (fp32) is nullable; act 0 none, 1 ReLU, 2 GELU. Sums are held in fp32. A row of x with an infinity or
- * NaN gives NaN or infinities, in that row only. */
+ * bias (fp32) is nullable; act 0 none, 1 ReLU, 2 GELU. Sums are held in fp32; values of x below 2^-28 of their
+ * row's largest lose low bits, at most 2^-35 of the largest. A row of x with an infinity or NaN gives NaN or
+ * infinities, in that row only; rows do not depend on each other. */
 S1C_API s1c_status s1c_nibble_gemm(int32_t dtype, const void* d_x, int64_t x_stride, const void* d_codes,
                                    int64_t code_pitch, const void* d_scales, const void* d_zeros, int64_t scale_stride,
                                    int32_t group, void* d_out, int64_t out_stride, int32_t M, int32_t N, int32_t K,
@@ -351,8 +352,9 @@ S1C_API s1c_status s1c_cache_attention(const s1c_cache* cache, int32_t dtype, co
  * which the kept mass summed so far exceeds u times the kept mass (u >= 1 or NaN: the last kept one); prob
  * (nullable) is its share of the kept mass. T <= 0 or NaN takes the largest logit, the lowest index among
  * equals, with prob 1. temperature, top_k, top_p and min_p hold a value for each row and are nullable (1,
- * off, off, off). Logits of -inf are never chosen; a row with a NaN or +inf, or with nothing above -inf,
- * gets token -1 and prob 0. vocab is at most 2^18. */
+ * off, off, off). An e_i below 2^-45 counts as 0. Logits of -inf are never chosen; a row with a NaN or +inf, or
+ * with nothing above -inf, gets token -1 and prob 0. A row's result does not depend on the other rows. vocab is at
+ * most 2^18. */
 S1C_API s1c_status s1c_sample(int32_t dtype, const void* d_logits, int64_t row_stride, int32_t rows, int32_t vocab,
                               const float* d_temperature, const int32_t* d_top_k, const float* d_top_p,
                               const float* d_min_p, const float* d_uniform, int32_t* d_token, float* d_prob,

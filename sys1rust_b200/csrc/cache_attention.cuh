@@ -10,15 +10,16 @@
 //
 //  - keys: the byte code + 128 at the bottom of a half is the subnormal (code + 128) * 2^-24, which the tensor
 //    cores take exactly; the products' sum starts at -128 * 2^-24 * sum(q), so nothing is subtracted. q is
-//    scaled by a power of two for each row to about 2^14, which keeps all bits of bf16 and f16. The order of dimensions inside the
-//    sum is free: a lane's 32-bit word holds four neighbours.
+//    scaled by a power of two for each row to about 2^14, which keeps all bits of bf16 and f16. The order of
+//    dimensions inside the sum is free: a lane's 32-bit word holds four neighbours.
 //  - values: the sum runs over keys, so a register pairs two keys' codes of one dimension; words of two
 //    keys are interleaved by byte permutes, put under the exponent of 1024 and 1152 subtracted.
-//  - a page's value scale differs from its neighbours' inside one sum, so it goes into the weight: with t = log2(scale /
-//    largest scale of the block), the weight is exp2(s + t - m + 14), m a running maximum of s + t, and the sum of
-//    the softmax adds weight * 2^-t. m follows the true maximum only when that is 1.75 ahead, so outputs are
-//    seldom rescaled. Weights are held as f16 (two of them for f16 results): at most 2^15.75, with all 11 bits
-//    down to 2^-28 of the largest; scores, maxima, sums and outputs are fp32.
+//  - a page's value scale differs from its neighbours' inside one sum, so it goes into the weight: with t =
+//    log2(scale / largest scale of the block), the weight is exp2(s + t - m + 14), m a running maximum of s + t,
+//    and the sum of the softmax adds weight * 2^-t (scales more than 2^90 apart: weights of its own). m follows
+//    the true maximum only when that is 1.75 ahead, so outputs are seldom rescaled. Weights are held as f16 (two
+//    of them for f16 results): at most 2^15.75, with all 11 bits down to 2^-28 of the largest; scores, maxima,
+//    sums and outputs are fp32.
 //
 // Few query rows (bound by the cache's bytes): each warp has its own tiles of the block's keys and its own
 // ring of loads, so nothing waits inside the loop; the four warps' results are joined at the end. Long
@@ -32,11 +33,12 @@
 // row in each thread, and write the weights P over the scores they come from, where the second product
 // reads them as its first operand.
 //
-// Measured: 64 sequences of 4096 to 8192 keys, 32 heads on 8 of 128, pages of 16: 165 us, 4.7 TB/s; what is
-// left there is instructions (850 for a tile of 32 keys, most of them conversions) at three blocks an SM. 1
-// x 131072 keys: 36 us, 3.7 TB/s, with one round of blocks and 3 us to join them; 1 x 700: 7.9 us, two
-// launches. Prompts, 4 x 512 rows over 2048 to 4096 keys, 16 heads on 4: 116 us, 461 TFLOP/s; on
-// mma.m16n8k16 the same took 326 us, of shared memory reads. There 256 blocks lie unevenly on 148 SMs, and
+// Measured: 64 sequences of 4096 to 8192 keys, 32 heads on 8 of 128, pages of 16: 163 us, 4.8 TB/s. Its 850
+// instructions for a tile of 32 keys, most of them conversions, fill half of the issue slots; at three blocks an SM
+// (168 registers) a scheduler has three warps, and waits for their dependent instructions the other half. 1 x
+// 131072 keys in f16: 40 us, 3.4 TB/s (36 us with weights of 11 bits), with one round of blocks and 3 us to join them;
+// 1 x 700: 8.1 us, two launches. Prompts, 4 x 512 rows over 2048 to 4096 keys, 16 heads on 4: 115 us, 465 TFLOP/s;
+// on mma.m16n8k16 the same took 326 us, of shared memory reads. There 256 blocks lie unevenly on 148 SMs, and
 // the softmax threads wait for the scores a third of the time.
 #pragma once
 #include <cuda.h>
@@ -316,7 +318,7 @@ struct AttnRows {
 // Weights are rounded to 11 bits for a bf16 result, whose own rounding to 8 bits is eight times as large. A result in
 // f16 would be a quarter further from its exact value (2.6e-4 instead of 2.1e-4 for one row over 131072 keys), so
 // there a second product takes what the rounding has left of each weight: 22 bits together. That costs 12 to 17 %
-// (37.1 -> 41.7 us for that row; bf16 would take 191 instead of 170 us for 64 rows over 4096 to 8192 keys, 134
+// (36 -> 40 us for that row; bf16 would take 191 instead of 170 us for 64 rows over 4096 to 8192 keys, 134
 // instead of 115 us for 4 x 512 rows, for the same distance of 1.7e-3 from the exact values).
 template <typename T>
 constexpr bool ATTN_SPLIT = false;

@@ -8,7 +8,9 @@
 // become round-half-even(code * s_old / s), both of the exact quotient.
 //
 // Measured on eight ragged prompts of up to 8192 rows (8 heads of 128, pages of 64): write 70 us and read
-// 74 us for 300 MB each, 4.1 TB/s. A quotient costs one product, with an exact second look only near a half
+// 74 us for 300 MB each, 4.1 TB/s. Issue slots are two thirds (write) and half (read) used; beside its rows each kernel
+// stores 250 MB of its own arguments to local memory, which every thread copies because it indexes their arrays by
+// blockIdx.z. A quotient costs one product, with an exact second look only near a half
 // (an IEEE division for each value took 224 us, the second look inside the unrolled code 144 us, of
 // instruction fetches).
 #pragma once

@@ -108,8 +108,11 @@ CacheRows check_rows(const CacheView& c, const void* k, int64_t k_stride, const 
   return r;
 }
 
-// How an attention call is laid out: blocks of 16 rows, or of many that share the keys' conversion; keys of
-// a block.
+// How an attention call is laid out: blocks of 16 rows, or of 128 that share the keys' conversion; keys of a block.
+// Up to 32 rows of a key head take blocks of 16 (4 key heads of 128, pages of 16, both ways in us): 16 sequences of
+// 16384 keys with 32 rows 113 and 132, with 40 rows 161 and 133; 64 of 4096 with 32 rows 121 and 132, with 40 rows
+// 169 and 136. A single sequence leans to either side: 16384 keys with 64 rows 23 and 26, 131072 with 24 rows 77
+// and 67.
 struct AttnPlan {
   bool prompt;
   int tiles, chunk, chunks;

@@ -89,7 +89,7 @@ def cache_read(cache: Cache, dtype: int, k_ptr: int, k_stride: int, v_ptr: int, 
 
 
 def cache_attention_workspace(cache: Cache, heads: int, n: int, max_q: int, max_kv: int) -> int:
-    """Bytes of device workspace that ``cache_attention`` with these bounds needs."""
+    """Bytes of device workspace that serve every ``cache_attention`` with bounds up to these."""
     return int(lib().s1c_cache_attention_workspace(C.byref(cache), heads, n, max_q, max_kv))
 
 
