@@ -1440,3 +1440,41 @@ def test_gemm_with_few_rows_is_scheduled_while_the_kernel_before_it_ends(ops):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out[0], out[1]) and out.any()
+
+
+@pytest.mark.parametrize("eager", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_of_many_rows_and_gemms_share_the_tensor_memory(ops, D, eager):
+    """Attention of many rows and ``s1c_gemm`` with few rows in turn, both in tensor memory and each scheduled while the
+    one before it ends: B of the product is what the attention has written."""
+    from sys1rust_b200 import backend
+    H, G, rows, L, N, rounds = 2, 4, 64, 700, 16, 30
+    c = Paged(ops, 1, L, H, D, 16, 95)
+    K = H * G * D
+    q = torch.randn(rows, K, generator=_gen(96), device="cuda").bfloat16()
+    a = torch.randn(N, K, generator=_gen(97), device="cuda").bfloat16()
+    att = torch.zeros(rounds, rows, K, dtype=torch.bfloat16, device="cuda")
+    out = torch.zeros(rounds, N, rows, device="cuda")
+    cu, ln = _i32([0, rows]), _i32([L])
+    ws = torch.empty(max(1, ops.cache_attention_workspace(c.handle, H * G, 1, rows, L)), dtype=torch.uint8, device="cuda")
+
+    def run():
+        for i in range(rounds):
+            ops.cache_attention(c.handle, ops.DT_BF16, q.data_ptr(), K, att[i].data_ptr(), K, H * G, cu.data_ptr(), ln.data_ptr(),
+                                c.table.data_ptr(), c.table.shape[1], 1, rows, L, 0.1, workspace_ptr=ws.data_ptr(),
+                                workspace_bytes=ws.numel(), stream=_stream())
+            backend.gemm(backend.EPI_STORE, a.data_ptr(), att[i].data_ptr(), out[i].data_ptr(), N, rows, K, out_f32=True, stream=_stream())
+
+    run()
+    if not eager:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        att.zero_(), out.zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(att[0], x) for x in att) and all(torch.equal(out[0], x) for x in out)
+    want = a.double() @ att[0].double().t()
+    # K products summed in fp32
+    assert ((out[0].double() - want).abs() <= K * 2.0 ** -22 * (a.double().abs() @ att[0].double().abs().t())).all() and want.any()
